@@ -190,6 +190,136 @@ int sc_mine_batch_device(sc_detector *d, const uint8_t *d_frames, int n, int w, 
                          int stride_bytes, sc_window *wins, float *d_features, int capacity,
                          int *n_out);
 
+/* ---- training on a mined sample matrix -----------------------------------
+ * sc_mine_*_device leaves the sample matrix of a boosting round on the GPU:
+ * one row per window, one descriptor of 32 values per template patch.  The
+ * entry points below are what CascadeClassifier::Train / GentleAdaboost::Train
+ * do with it (CascadeClassifier.cpp:11-56, GentleAdaboost.cpp:11-231): the
+ * responses of logistic weak learners (LogisticRegression::Predict,
+ * LogisticRegression.cpp:46-68) added to a running score, their gradient, the
+ * weighted logistic loss LogisticRegression::Train minimises (:35-44) with its
+ * gradient, and the roulette wheel that resamples the rows.
+ *
+ * A trainer owns one HIP stream.  Every call is asynchronous on it, reads and
+ * writes device memory of the trainer's GPU (checked: SC_ERR_INVALID), and may
+ * be captured into a HIP graph.  The stream rules are a detector's: see
+ * sc_detector_wait_stream, sc_stream_wait_detector, sc_detector_set_stream.
+ * Switching to or from a stream that is being captured sets up no order.
+ * Distinct trainers may be used from different threads, one is not thread-safe.
+ *
+ * Workspaces: a call that takes (ws, ws_bytes) uses that device memory
+ * (16-byte aligned, at least the bytes its *_workspace function says, free
+ * again when the call's work is done), or with ws == NULL memory of the
+ * trainer.  A call under stream capture has to bring its own if it needs one:
+ * it belongs to that graph alone.
+ *
+ * Results do not depend on the order of any sum but the one stated by the
+ * sizes: the same call gives the same bits. */
+typedef struct sc_trainer sc_trainer;
+int sc_trainer_create(int device, sc_trainer **out);
+void sc_trainer_destroy(sc_trainer *t);
+void *sc_trainer_stream(sc_trainer *t); /* hipStream_t */
+int sc_trainer_wait_stream(sc_trainer *t, void *stream);
+int sc_stream_wait_trainer(sc_trainer *t, void *stream);
+int sc_trainer_set_stream(sc_trainer *t, void *stream, int use_own);
+int sc_trainer_synchronize(sc_trainer *t);
+
+#define SC_F32 0
+#define SC_F16 1
+#define SC_BF16 2
+
+/* The rows a call reads.  Sample i's descriptor of patch p is the 32 elements
+ * at data + i*ld + 32*p (elements; any element alignment).  Row r reads sample
+ * rows[r], or sample r when rows == NULL; a row whose number is outside [0, n)
+ * (sc_sample's -1, say) is absent: it has no response, adds nothing to a loss
+ * or gradient, and nothing is read for it.  A number may occur again. */
+typedef struct {
+    const void *data; /* device */
+    int32_t dtype;    /* SC_F32, SC_F16 or SC_BF16                   */
+    int32_t n_patches;
+    int64_t n;  /* samples, at most 2^30                             */
+    int64_t ld; /* elements from sample to sample, >= 32 * n_patches */
+    const int32_t *rows; /* device int32[n_rows], or NULL            */
+    int64_t n_rows;      /* at most 2^30; ignored when rows == NULL  */
+} sc_samples;
+
+/* m weak learners with h parameter sets each (h = 1 for one classifier per
+ * patch; more for several regularisation strengths, steps of a line search or
+ * views fitted at once).  Learner j reads patch patch[j], or patch j when
+ * patch == NULL (m <= n_patches then); one whose patch is outside
+ * [0, n_patches) is absent, as a row.  The same patch may occur again. */
+typedef struct {
+    int32_t m, h;         /* m * h <= 2^25, h <= 1024 */
+    const int32_t *patch; /* device int32[m], or NULL */
+    const float *w;       /* device float[m][h][32]   */
+    const float *b;       /* device float[m][h], or NULL: 0 */
+} sc_weak_bank;
+
+#define SC_ACT_NONE 0    /* act(z) = z               */
+#define SC_ACT_SIGMOID 1 /* act(z) = 1 / (1 + e^-z)  */
+#define SC_RES_NONE 0    /* no residual                                      */
+#define SC_RES_ROW 1     /* one value per row: res[r * res_ld]               */
+#define SC_RES_FULL 2    /* one per result: res[r * res_ld + j*h + k]        */
+
+/* y[r * y_ld + j*h + k] = alpha * act(x[row r, patch j] . w[j][k] + b[j][k])
+ *                         + beta * residual
+ * for every row r, learner j and set k; the first term is 0 for an absent row
+ * or learner.  Dots and results in 32 bits.  y may be res itself (SC_RES_FULL,
+ * same leading size); it overlaps no other operand. */
+int sc_lr_response(sc_trainer *t, const sc_samples *x, const sc_weak_bank *k, int act, float alpha,
+                   const float *res, int res_kind, int64_t res_ld, float beta, float *y,
+                   int64_t y_ld);
+
+/* Workspace of sc_lr_response_grad and sc_lr_loss for these sizes (pointers
+ * other than rows are not looked at). */
+int sc_lr_workspace(const sc_samples *x, const sc_weak_bank *k, size_t *bytes);
+
+/* The backward pass of sc_lr_response for dy[r * dy_ld + j*h + k]:
+ *   g = alpha * dy * act'(z), 0 for an absent row or learner
+ *   dw[j][k] = sum_r g x[row r, patch j], db[j][k] = sum_r g
+ *   dres = beta * dy, summed over a row's results for SC_RES_ROW
+ * (dres NULL with SC_RES_NONE).  Sums over rows in 32 bits over a chunk of
+ * rows and in 64 bits over the chunks, dres sums in 64 bits.  There is no
+ * gradient of the descriptors: they are read off images. */
+int sc_lr_response_grad(sc_trainer *t, const sc_samples *x, const sc_weak_bank *k, int act,
+                        float alpha, const float *dy, int64_t dy_ld, float *dw, float *db,
+                        int res_kind, float beta, float *dres, int64_t dres_ld, void *ws,
+                        size_t ws_bytes);
+
+/* The weighted logistic loss of every learner and set, with its gradient:
+ *   loss[j][k] = sum_r c (log(1 + e^z) - t z)
+ *   g = c (1 / (1 + e^-z) - t), dw and db as above
+ * target t (in [0, 1]) and weight c are by sample: float[n], the entry of the
+ * sample that a row reads; weight NULL: 1.  A row with c == 0 is absent,
+ * whatever its descriptors hold. */
+int sc_lr_loss(sc_trainer *t, const sc_samples *x, const sc_weak_bank *k, const float *target,
+               const float *weight, float *loss, float *dw, float *db, void *ws, size_t ws_bytes);
+
+typedef struct {
+    double temperature; /* > 0; 0: every draw is the best place, the lowest one of equals */
+    int32_t top_k;      /* keep the top_k best places (0: off)                     */
+    double top_p;       /* ... of those the fewest with top_p of their mass (>= 1: off) */
+    double min_p;       /* ... of those the ones with at least min_p of the best's
+                           weight (0: off) */
+} sc_sample_params;
+void sc_sample_params_default(sc_sample_params *p);
+int sc_sample_workspace(int b, int v, int s, size_t *bytes);
+/* s draws with replacement from each of b rows of v scores (log-weights,
+ * scores + i*ld, dtype as sc_samples; lens != NULL: row i has lens[i] scores,
+ * clamped to [0, v]).  Place i of a row weighs exp((s_i - max) / temperature);
+ * -inf and NaN are absent, +inf outweighs every finite score.  The kept places
+ * are a prefix of the order by descending score (ties: ascending place), as
+ * the parameters say.  For u in [0, 1) (values outside are clamped; NaN: 0)
+ *   index[i * index_ld + j] = the smallest place whose kept weights up to and
+ *                             with it sum to more than u[i * u_ld + j] * all
+ * or -1 for a row without a place to draw; kept[i] (kept may be NULL) = the
+ * kept places.  Weights are 64-bit doubles, sums 64-bit integers of at least
+ * 36 bits after the point (52 for short rows), so they have no order. */
+int sc_sample(sc_trainer *t, const void *scores, int dtype, int b, int v, int64_t ld,
+              const int32_t *lens, const sc_sample_params *prm, const double *u, int s,
+              int64_t u_ld, int32_t *index, int64_t index_ld, int32_t *kept, void *ws,
+              size_t ws_bytes);
+
 /* ---- introspection / parity dumps -------------------------------------- */
 #define SC_INFO_LEVELS 1        /* levels used for the last geometry         */
 #define SC_INFO_GRID_WINDOWS 2  /* stride-step grid windows per frame        */

@@ -20,7 +20,7 @@ import numpy as np
 __all__ = ["ScanParams", "Model", "CascadeClassifier", "StageClassifier", "LogisticRegression",
            "Detector", "SurfCascadeError", "WINDOW_DTYPE", "RECORD_DTYPE", "library_path",
            "load_library", "extract_patches", "RECT_DTYPE", "groupRectangles", "group_detections",
-           "fddb_format", "Miner"]
+           "fddb_format", "Miner", "Trainer"]
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -63,6 +63,10 @@ EXPORTS = ("sc_scan_params_default", "sc_model_load", "sc_model_parse", "sc_mode
            "sc_detector_set_shard", "sc_detector_set_option", "sc_detector_set_debug", "sc_debug_dump", "sc_set_timing", "sc_get_timing",
            "sc_group_rectangles", "sc_group_detections", "sc_fddb_format",
            "sc_miner_create", "sc_mine", "sc_mine_device", "sc_mine_batch", "sc_mine_batch_device", "sc_fast_nms", "sc_decode_jpeg_gray", "sc_imread_gray",
+           "sc_trainer_create", "sc_trainer_destroy", "sc_trainer_stream", "sc_trainer_wait_stream",
+           "sc_stream_wait_trainer", "sc_trainer_set_stream", "sc_trainer_synchronize",
+           "sc_lr_response", "sc_lr_workspace", "sc_lr_response_grad", "sc_lr_loss",
+           "sc_sample_params_default", "sc_sample_workspace", "sc_sample",
            "sc_selftest_rn", "sc_normalize_operand_range", "sc_last_error", "sc_version",
            "sc_build_info")
 
@@ -171,6 +175,24 @@ def load_library():
     L.sc_fast_nms.argtypes = [vp, i32, ctypes.c_double, vp, i32, P(i32)]
     L.sc_decode_jpeg_gray.argtypes = [vp, sz, vp, sz, P(i32), P(i32)]
     L.sc_imread_gray.argtypes = [ctypes.c_char_p, vp, sz, P(i32), P(i32)]
+    f32 = ctypes.c_float
+    L.sc_trainer_create.argtypes = [i32, P(vp)]
+    L.sc_trainer_destroy.argtypes = [vp]
+    L.sc_trainer_destroy.restype = None
+    L.sc_trainer_stream.argtypes = [vp]
+    L.sc_trainer_stream.restype = vp
+    L.sc_trainer_wait_stream.argtypes = [vp, vp]
+    L.sc_stream_wait_trainer.argtypes = [vp, vp]
+    L.sc_trainer_set_stream.argtypes = [vp, vp, i32]
+    L.sc_trainer_synchronize.argtypes = [vp]
+    L.sc_lr_response.argtypes = [vp, vp, vp, i32, f32, vp, i32, i64, f32, vp, i64]
+    L.sc_lr_workspace.argtypes = [vp, vp, P(sz)]
+    L.sc_lr_response_grad.argtypes = [vp, vp, vp, i32, f32, vp, i64, vp, vp, i32, f32, vp, i64, vp, sz]
+    L.sc_lr_loss.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, sz]
+    L.sc_sample_params_default.argtypes = [vp]
+    L.sc_sample_params_default.restype = None
+    L.sc_sample_workspace.argtypes = [i32, i32, i32, P(sz)]
+    L.sc_sample.argtypes = [vp, vp, i32, i32, i32, i64, vp, vp, vp, i32, i64, vp, i64, vp, vp, sz]
     L.sc_selftest_rn.argtypes = [i32, i32, ctypes.c_uint32, ctypes.c_uint32, P(ctypes.c_uint64)]
     L.sc_normalize_operand_range.argtypes = [i32, i32, P(ctypes.c_double), P(ctypes.c_double)]
     L.sc_normalize_operand_range.restype = None
@@ -731,3 +753,6 @@ class Miner(Detector):
         if rc != -6:
             _check(rc)
         return wins[:min(n.value, capacity)].copy(), n.value
+
+
+from .train import Trainer  # noqa: E402  (uses the binding above)

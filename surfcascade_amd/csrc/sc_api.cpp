@@ -23,11 +23,14 @@
 
 #include "sc_kernels.hpp"
 #include "sc_group.hpp"
+#include "sc_host.hpp"
 #include "sc_jpeg.hpp"
 #include "sc_model.hpp"
 #include "surfcascade.h"
 
+using sc::DevBuf;
 using sc::Error;
+using sc::guarded;
 
 struct sc_model {
     sc::Cascade c;
@@ -58,30 +61,6 @@ int fail(int code, const std::string &msg) {
     g_err = msg;
     return code;
 }
-
-#define HIPCHK(expr)                                                                        \
-    do {                                                                                    \
-        hipError_t e_ = (expr);                                                             \
-        if (e_ != hipSuccess)                                                               \
-            throw Error{SC_ERR_DEVICE, std::string(#expr) + ": " + hipGetErrorString(e_)}; \
-    } while (0)
-
-template <class T>
-struct DevBuf {
-    T *p = nullptr;
-    size_t n = 0;
-    void ensure(size_t want) {
-        if (want <= n) return;
-        release();
-        HIPCHK(hipMalloc(&p, std::max<size_t>(want, 1) * sizeof(T)));
-        n = want;
-    }
-    void release() {
-        if (p) (void)hipFree(p);
-        p = nullptr;
-        n = 0;
-    }
-};
 
 // Pinned host staging for frames handed over in pageable host memory: the
 // DMA engine reads pinned pages directly, while a pageable 2-D copy is
@@ -120,6 +99,27 @@ struct Geometry {
 };
 
 }  // namespace
+
+namespace sc {
+
+int set_error(int code, const std::string &msg) { return fail(code, msg); }
+
+void check_device_ptr(int device, const char *owner, const void *p, const char *what) {
+    if (!p) return;
+    hipPointerAttribute_t at{};
+    const hipError_t e = hipPointerGetAttributes(&at, p);
+    if (e != hipSuccess) {
+        (void)hipGetLastError();  // an unregistered host pointer: clear the error
+        throw Error{SC_ERR_INVALID, std::string(what) + " is not device memory"};
+    }
+    if (at.type != hipMemoryTypeDevice && at.type != hipMemoryTypeManaged)
+        throw Error{SC_ERR_INVALID, std::string(what) + " is not device memory"};
+    if (at.device != device)
+        throw Error{SC_ERR_INVALID, std::string(what) + " is on device " + std::to_string(at.device) + ", the " +
+                                        owner + " on device " + std::to_string(device)};
+}
+
+}  // namespace sc
 
 struct sc_detector {
     int device = 0;
@@ -1021,22 +1021,8 @@ void check_chain(sc_detector *d) {
     }
 }
 
-// A caller's device pointer must be device memory of this detector's GPU: a
-// host pointer or another GPU's memory would fault in a kernel instead of
-// returning SC_ERR_INVALID.
 void check_device_ptr(const sc_detector *d, const void *p, const char *what) {
-    if (!p) return;
-    hipPointerAttribute_t at{};
-    const hipError_t e = hipPointerGetAttributes(&at, p);
-    if (e != hipSuccess) {
-        (void)hipGetLastError();  // an unregistered host pointer: clear the error
-        throw Error{SC_ERR_INVALID, std::string(what) + " is not device memory"};
-    }
-    if (at.type != hipMemoryTypeDevice && at.type != hipMemoryTypeManaged)
-        throw Error{SC_ERR_INVALID, std::string(what) + " is not device memory"};
-    if (at.device != d->device)
-        throw Error{SC_ERR_INVALID, std::string(what) + " is on device " + std::to_string(at.device) +
-                                        ", the detector on device " + std::to_string(d->device)};
+    sc::check_device_ptr(d->device, "detector", p, what);
 }
 
 bool rec_less(const sc_det_record &a, const sc_det_record &b) {
@@ -1193,19 +1179,6 @@ int mine_sync(sc_detector *d, const uint8_t *d_frames, int n, int W, int H, int 
         return SC_ERR_CAPACITY;
     }
     return SC_OK;
-}
-
-template <class F>
-int guarded(F &&f) {
-    try {
-        return f();
-    } catch (const Error &e) {
-        return fail(e.code, e.msg);
-    } catch (const std::bad_alloc &) {
-        return fail(SC_ERR_NOMEM, "out of host memory");
-    } catch (const std::exception &e) {
-        return fail(SC_ERR_INVALID, e.what());
-    }
 }
 
 }  // namespace

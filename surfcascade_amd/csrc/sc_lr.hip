@@ -1,0 +1,428 @@
+// sc_lr.hip -- gfx950 kernels of the weak learners over a sample matrix
+// (LogisticRegression::Predict and its training sums, LogisticRegression.cpp:
+// 35-68, over the descriptors ExtractFeatures leaves,
+// DenseSURFFeatureExtractor.cpp:88-93), for R rows x M learners x H parameter
+// sets:
+//   z[r,m,h]   = x[row r, patch m] . w[m,h] + b[m,h]
+//   response   : y = alpha * act(z) + beta * residual
+//   gradient   : g = alpha * dy * act'(z); dw = sum_r g x, db = sum_r g
+//   loss       : L = sum_r c (softplus(z) - t z), g = c (sigmoid(z) - t)
+// A (row, patch) descriptor is 128 B (64 B in 16 bits) that feeds 64 flops per
+// parameter set, so each is read once and everything else is done on it in
+// registers.  All sums are in 32 bits; the chunks of a gradient are joined in
+// 64 bits in a fixed order (no atomics: the same call gives the same bits).
+//
+// Narrow form (this file's lr_kernel): one descriptor on LPI = 8 lanes (4 in
+// 16 bits), 16 B each, so a wave's load is 8 (16) neighbouring descriptors of
+// one row = 1 KB in one piece.  A wave keeps its learners' weights in
+// registers and walks rows, LPI of them at a time: the LPI x LPI partial dots
+// are summed by a butterfly that also transposes, leaving lane q with row q's
+// dot, so the sigmoid runs once per result on full lanes.
+#include <hip/hip_runtime.h>
+
+#include "sc_train.hpp"
+#include "surfcascade.h"
+
+namespace sc {
+
+namespace {
+
+constexpr int kWaves = 4;  // waves per workgroup
+
+struct F32 {
+    static constexpr int kSize = 4;
+};
+struct F16 {
+    static constexpr int kSize = 2;
+};
+struct BF16 {
+    static constexpr int kSize = 2;
+};
+
+// 16 B with the alignment of an element (the sample matrix may start, and its
+// rows may lie, at any element)
+typedef unsigned uint4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned uint4_a2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned uint4_v __attribute__((ext_vector_type(4)));
+typedef _Float16 half2_v __attribute__((ext_vector_type(2)));
+
+template <class T>
+__device__ __forceinline__ uint4_v load16(const char *p) {
+    if constexpr (T::kSize == 4) return *reinterpret_cast<const uint4_a4 *>(p);
+    else return *reinterpret_cast<const uint4_a2 *>(p);
+}
+
+// the 16 / kSize values of a 16-B piece
+template <class T>
+__device__ __forceinline__ void unpack(uint4_v v, float *f) {
+    if constexpr (T::kSize == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) f[i] = __uint_as_float(v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const unsigned u = v[i];
+            if constexpr (__is_same(T, BF16)) {
+                f[2 * i] = __uint_as_float(u << 16);
+                f[2 * i + 1] = __uint_as_float(u & 0xffff0000u);
+            } else {
+                const half2_v h = __builtin_bit_cast(half2_v, u);
+                f[2 * i] = (float)h[0];
+                f[2 * i + 1] = (float)h[1];
+            }
+        }
+    }
+}
+
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kReverse4 = 0x1B, kMirror8 = 0x141;  // DPP controls
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+
+// v[u] = this lane's part of row u's sum, over the LPI lanes of an item ->
+// lane q's return value is row q's sum.
+template <int LPI>
+__device__ __forceinline__ float sum_rows(float *v, int q) {
+    if constexpr (LPI == 8) {
+        const bool hi = q & 4;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {  // partner 7 - q
+            const float send = hi ? v[i] : v[i + 4];
+            v[i] = (hi ? v[i + 4] : v[i]) + dpp<kMirror8>(send);
+        }
+    }
+    const bool mid = q & 2, odd = q & 1;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const float send = mid ? v[i] : v[i + 2];
+        v[i] = (mid ? v[i + 2] : v[i]) + dpp<kXor2>(send);
+    }
+    const float send = odd ? v[0] : v[1];
+    return (odd ? v[1] : v[0]) + dpp<kXor1>(send);
+}
+
+// lane q holds row q's value -> all[u] = row u's, in every lane of the item
+template <int LPI>
+__device__ __forceinline__ void spread_rows(float v, int q, float *all) {
+    float low = v;
+    if constexpr (LPI == 8) {
+        const float other = dpp<kReverse4>(dpp<kMirror8>(v));  // lane q ^ 4's
+        low = (q & 4) ? other : v;
+        const float high = (q & 4) ? v : other;
+        all[4] = dpp<0x00>(high);
+        all[5] = dpp<0x55>(high);
+        all[6] = dpp<0xAA>(high);
+        all[7] = dpp<0xFF>(high);
+    }
+    all[0] = dpp<0x00>(low);
+    all[1] = dpp<0x55>(low);
+    all[2] = dpp<0xAA>(low);
+    all[3] = dpp<0xFF>(low);
+}
+
+// sum over the LPI lanes of an item, in each of them
+template <int LPI>
+__device__ __forceinline__ float sum_lanes(float v) {
+    v += dpp<kXor1>(v);
+    v += dpp<kXor2>(v);
+    if constexpr (LPI == 8) v += dpp<kMirror8>(v);
+    return v;
+}
+
+__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+
+enum Mode { kResponse = 0, kGrad = 1, kLoss = 2 };
+
+// g of one result and, for the loss, its term (e = exp(-|z|): neither
+// s = sigmoid(z) nor 1 - s = sigmoid(-z) is formed by a difference)
+template <int MODE>
+__device__ __forceinline__ float grad_of(const LrArgs &a, float z, float c, float t, float &loss) {
+    const float e = __expf(-fabsf(z)), d = __fdividef(1.0f, 1.0f + e);
+    if constexpr (MODE == kLoss) {
+        const float s = z >= 0.0f ? d : e * d, s1 = z >= 0.0f ? e * d : d;
+        loss += c * (log1pf(e) + (1.0f - t) * fmaxf(z, 0.0f) + t * fmaxf(-z, 0.0f));
+        const float g = c * ((1.0f - t) * s - t * s1);
+        return z != z ? z : g;  // (fmaxf drops a NaN; the gradient keeps it)
+    } else {
+        return a.act == SC_ACT_SIGMOID ? c * e * d * d : c;  // c = alpha * dy
+    }
+}
+
+template <class T, int H, int MODE>
+__global__ __launch_bounds__(64 * kWaves) void lr_kernel(LrArgs a) {
+    constexpr int LPI = kDesc * T::kSize / 16;  // lanes per item
+    constexpr int EPL = 16 / T::kSize;          // descriptor values per lane
+    constexpr int IPW = 64 / LPI;               // items per wave
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int q = lane & (LPI - 1), item = lane / LPI;
+    // waves of a workgroup: neighbouring learners of one row range for a
+    // response (their stores meet in one line), row ranges of the same
+    // learners for a gradient (joined in LDS below)
+    const int mt = MODE == kResponse ? blockIdx.x * kWaves + wave : blockIdx.x;
+    const int range = MODE == kResponse ? blockIdx.y : blockIdx.y * kWaves + wave;
+    const int h0 = blockIdx.z * H;
+    const int m = mt * IPW + item;
+    const bool learner = m < a.M;
+    int p = 0;
+    bool present = false;
+    if (learner) {
+        p = a.patch ? a.patch[m] : m;
+        present = (unsigned)p < (unsigned)a.n_patches;
+        if (!present) p = 0;
+    }
+    const unsigned off = (unsigned)(p * kDesc * T::kSize + q * 16);
+    float w[H][EPL], bias[H];
+#pragma unroll
+    for (int h = 0; h < H; h++) {
+        const bool on = learner && h0 + h < a.H;
+        const long long mh = (long long)m * a.H + h0 + h;
+#pragma unroll
+        for (int e = 0; e < EPL; e++) w[h][e] = on ? a.w[mh * kDesc + q * EPL + e] : 0.0f;
+        bias[h] = on && a.b ? a.b[mh] : 0.0f;
+    }
+    float acc[H][EPL], sum_g[H], sum_l[H];
+#pragma unroll
+    for (int h = 0; h < H; h++) {
+        sum_g[h] = sum_l[h] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < EPL; e++) acc[h][e] = 0.0f;
+    }
+    const long long r_lo = (long long)range * a.rows_per_wave;
+    const int r0 = (int)(r_lo < a.R ? r_lo : a.R);
+    const int r1 = (int)(r_lo + a.rows_per_wave < a.R ? r_lo + a.rows_per_wave : a.R);
+    const char *x = static_cast<const char *>(a.x);
+    for (int r = r0; r < r1; r += LPI) {
+        const int rq = r + q;  // the row whose dot this lane will hold
+        int idx = -1;
+        if (rq < r1) {
+            idx = a.rows ? a.rows[rq] : rq;
+            if ((unsigned)idx >= (unsigned)a.n) idx = -1;
+        }
+        float c = 0.0f, t = 0.0f;
+        if constexpr (MODE == kLoss) {
+            if (idx >= 0) {
+                c = a.weight ? a.weight[idx] : 1.0f;
+                t = a.target[idx];
+                if (c == 0.0f) idx = -1;  // a row without weight is not looked at, whatever it holds
+            }
+        }
+        uint4_v xv[LPI];
+#pragma unroll
+        for (int u = 0; u < LPI; u++) {
+            const int iu = __builtin_amdgcn_readlane(idx, u);
+            xv[u] = uint4_v{0, 0, 0, 0};
+            if (iu >= 0) xv[u] = load16<T>(x + (long long)iu * a.ld * T::kSize + off);
+        }
+        float g_all[H][LPI];
+        float z[H];
+        {
+            float part[H][LPI];
+#pragma unroll
+            for (int u = 0; u < LPI; u++) {
+                float f[EPL];
+                unpack<T>(xv[u], f);
+#pragma unroll
+                for (int h = 0; h < H; h++) {
+                    float s = f[0] * w[h][0];
+#pragma unroll
+                    for (int e = 1; e < EPL; e++) s = __builtin_fmaf(f[e], w[h][e], s);
+                    part[h][u] = s;
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < H; h++) z[h] = sum_rows<LPI>(part[h], q) + bias[h];
+        }
+        if constexpr (MODE == kResponse) {
+            if (learner && rq < r1) {
+#pragma unroll
+                for (int h = 0; h < H; h++) {
+                    if (h0 + h >= a.H) break;
+                    const long long col = (long long)m * a.H + h0 + h;
+                    float v = 0.0f;  // an absent row or patch has no response
+                    if (idx >= 0 && present) v = a.alpha * (a.act == SC_ACT_SIGMOID ? sigmoid(z[h]) : z[h]);
+                    if (a.res_kind == SC_RES_ROW) v += a.beta * a.res[(long long)rq * a.res_ld];
+                    else if (a.res_kind == SC_RES_FULL) v += a.beta * a.res[(long long)rq * a.res_ld + col];
+                    a.y[(long long)rq * a.y_ld + col] = v;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int h = 0; h < H; h++) {
+                float g = 0.0f;
+                if (idx >= 0 && present && h0 + h < a.H) {
+                    if constexpr (MODE == kGrad)
+                        c = a.alpha * a.dy[(long long)rq * a.dy_ld + (long long)m * a.H + h0 + h];
+                    g = grad_of<MODE>(a, z[h], c, t, sum_l[h]);
+                }
+                sum_g[h] += g;
+                spread_rows<LPI>(g, q, g_all[h]);
+            }
+#pragma unroll
+            for (int u = 0; u < LPI; u++) {
+                float f[EPL];
+                unpack<T>(xv[u], f);
+#pragma unroll
+                for (int h = 0; h < H; h++)
+#pragma unroll
+                    for (int e = 0; e < EPL; e++) acc[h][e] = __builtin_fmaf(g_all[h][u], f[e], acc[h][e]);
+            }
+        }
+    }
+    if constexpr (MODE != kResponse) {
+        constexpr int kVals = H * (EPL + 2);
+        __shared__ float s_acc[kWaves][kVals][64];
+#pragma unroll
+        for (int h = 0; h < H; h++) {
+#pragma unroll
+            for (int e = 0; e < EPL; e++) s_acc[wave][h * (EPL + 2) + e][lane] = acc[h][e];
+            s_acc[wave][h * (EPL + 2) + EPL][lane] = sum_lanes<LPI>(sum_g[h]);
+            s_acc[wave][h * (EPL + 2) + EPL + 1][lane] = sum_lanes<LPI>(sum_l[h]);
+        }
+        __syncthreads();
+        if (!learner) return;
+        for (int v = wave; v < kVals; v += kWaves) {
+            float s = s_acc[0][v][lane];
+#pragma unroll
+            for (int k = 1; k < kWaves; k++) s += s_acc[k][v][lane];
+            const int h = v / (EPL + 2), e = v - h * (EPL + 2);
+            if (h0 + h >= a.H || (e >= EPL && q != 0)) continue;
+            if (e < EPL && !present) s = 0.0f;  // (0 * NaN of the patch read in its place)
+            const long long mh = (long long)m * a.H + h0 + h;
+            const int word = e < EPL ? q * EPL + e : kDesc + (e - EPL);
+            if (a.part) a.part[((long long)blockIdx.y * a.M * a.H + mh) * kPartWords + word] = s;
+            else if (word < kDesc) a.dw[mh * kDesc + word] = s;
+            else if (word == kDesc) a.db[mh] = s;
+            else if (MODE == kLoss) a.loss[mh] = s;
+        }
+    }
+}
+
+// Joins the row chunks' partial sums: 32 neighbouring words per workgroup, its
+// 8 lane rows each walk every eighth chunk, in 64 bits.  No chunk at all (no
+// rows): zeros.
+__global__ __launch_bounds__(256) void lr_join_kernel(LrArgs a, int loss) {
+    __shared__ double s_sum[8][32];
+    const long long words = (long long)a.M * a.H * kPartWords;
+    const long long i = (long long)blockIdx.x * 32 + (threadIdx.x & 31);
+    const int sub = threadIdx.x >> 5;
+    double s = 0.0;
+    if (i < words)
+        for (int k = sub; k < a.chunks; k += 8) s += (double)a.part[k * words + i];
+    s_sum[sub][threadIdx.x & 31] = s;
+    __syncthreads();
+    if (sub != 0 || i >= words) return;
+    for (int k = 1; k < 8; k++) s += s_sum[k][threadIdx.x];
+    const long long mh = i / kPartWords;
+    const int word = (int)(i - mh * kPartWords);
+    if (word < kDesc) a.dw[mh * kDesc + word] = (float)s;
+    else if (word == kDesc) a.db[mh] = (float)s;
+    else if (loss) a.loss[mh] = (float)s;
+}
+
+// gradient of a residual: beta * dy, or its sum over a row's results
+__global__ __launch_bounds__(256) void res_full_kernel(LrArgs a) {
+    const long long cols = (long long)a.M * a.H;
+    for (long long r = blockIdx.y; r < a.R; r += gridDim.y)
+        for (long long c = (long long)blockIdx.x * 256 + threadIdx.x; c < cols; c += (long long)gridDim.x * 256)
+            a.dres[r * a.dres_ld + c] = a.beta * a.dy[r * a.dy_ld + c];
+}
+
+__global__ __launch_bounds__(256) void res_row_kernel(LrArgs a) {
+    __shared__ double s_sum[4];
+    const long long cols = (long long)a.M * a.H;
+    for (long long r = blockIdx.x; r < a.R; r += gridDim.x) {
+        double s = 0.0;
+        for (long long c = threadIdx.x; c < cols; c += 256) s += (double)a.dy[r * a.dy_ld + c];
+#pragma unroll
+        for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d, 64);
+        if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = s;
+        __syncthreads();
+        if (threadIdx.x == 0)
+            a.dres[r * a.dres_ld] = (float)((double)a.beta * (s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]));
+        __syncthreads();
+    }
+}
+
+int items_per_wave(const LrArgs &a) { return a.dtype == SC_F32 ? 8 : 16; }
+int lanes_per_item(const LrArgs &a) { return a.dtype == SC_F32 ? 8 : 4; }
+int sets_per_wave(const LrArgs &a) { return a.H == 1 ? 1 : a.H == 2 ? 2 : 4; }
+
+long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+
+template <class T, int MODE>
+void launch_narrow(const LrArgs &a, dim3 grid, hipStream_t s) {
+    switch (sets_per_wave(a)) {
+        case 1: hipLaunchKernelGGL((lr_kernel<T, 1, MODE>), grid, dim3(64 * kWaves), 0, s, a); break;
+        case 2: hipLaunchKernelGGL((lr_kernel<T, 2, MODE>), grid, dim3(64 * kWaves), 0, s, a); break;
+        default: hipLaunchKernelGGL((lr_kernel<T, 4, MODE>), grid, dim3(64 * kWaves), 0, s, a); break;
+    }
+}
+
+template <int MODE>
+void launch_mode(const LrArgs &a, dim3 grid, hipStream_t s) {
+    switch (a.dtype) {
+        case SC_F32: launch_narrow<F32, MODE>(a, grid, s); break;
+        case SC_F16: launch_narrow<F16, MODE>(a, grid, s); break;
+        default: launch_narrow<BF16, MODE>(a, grid, s); break;
+    }
+}
+
+}  // namespace
+
+// Gradient and loss: rows are cut into chunks of kWaves wave ranges until the
+// grid has a few waves per SIMD of the 256 CUs.
+LrPlan lr_plan(const LrArgs &a) {
+    LrPlan p{0, 0, 0};
+    if (a.R == 0) return p;
+    const int lpi = lanes_per_item(a);
+    const long long tiles = ceil_div(a.M, items_per_wave(a)) * ceil_div(a.H, sets_per_wave(a));
+    const long long most = ceil_div(a.R, (long long)kWaves * lpi);
+    long long chunks = ceil_div(4096, tiles * kWaves);
+    if (chunks > most) chunks = most;
+    p.rows_per_wave = (int)(ceil_div(ceil_div(a.R, chunks * kWaves), lpi) * lpi);
+    p.chunks = (int)ceil_div(a.R, (long long)p.rows_per_wave * kWaves);
+    if (p.chunks > 1) p.part_bytes = (size_t)p.chunks * a.M * a.H * kPartWords * sizeof(float);
+    return p;
+}
+
+void launch_lr_response(const LrArgs &a0, hipStream_t s) {
+    LrArgs a = a0;
+    const int lpi = lanes_per_item(a);
+    const long long tiles = ceil_div(a.M, (long long)items_per_wave(a) * kWaves);
+    const long long hs = ceil_div(a.H, sets_per_wave(a));
+    // rows per wave: enough waves for the chip, at most 64 rows, at most 65535 chunks
+    long long rows = ceil_div(ceil_div(a.R, ceil_div(8192, tiles * hs * kWaves)), lpi) * lpi;
+    if (rows > 64) rows = 64;
+    const long long least = ceil_div(ceil_div(a.R, 65535), lpi) * lpi;
+    a.rows_per_wave = (int)(rows > least ? rows : least);
+    launch_mode<kResponse>(a, dim3((unsigned)tiles, (unsigned)ceil_div(a.R, a.rows_per_wave), (unsigned)hs), s);
+}
+
+void launch_lr_grad(const LrArgs &a, bool loss, hipStream_t s) {
+    if (a.chunks > 0) {
+        const dim3 grid((unsigned)ceil_div(a.M, items_per_wave(a)), (unsigned)a.chunks,
+                        (unsigned)ceil_div(a.H, sets_per_wave(a)));
+        if (loss) launch_mode<kLoss>(a, grid, s);
+        else launch_mode<kGrad>(a, grid, s);
+    }
+    if (a.chunks != 1) {
+        const long long words = (long long)a.M * a.H * kPartWords;
+        hipLaunchKernelGGL(lr_join_kernel, dim3((unsigned)ceil_div(words, 32)), dim3(256), 0, s, a, loss ? 1 : 0);
+    }
+}
+
+void launch_lr_res_grad(const LrArgs &a, hipStream_t s) {
+    if (a.R == 0) return;
+    if (a.res_kind == SC_RES_ROW) {
+        hipLaunchKernelGGL(res_row_kernel, dim3((unsigned)(a.R < 8192 ? a.R : 8192)), dim3(256), 0, s, a);
+    } else {
+        const long long cols = (long long)a.M * a.H;
+        const long long bx = ceil_div(cols, 256);
+        hipLaunchKernelGGL(res_full_kernel, dim3((unsigned)(bx < 64 ? bx : 64), (unsigned)(a.R < 4096 ? a.R : 4096)),
+                           dim3(256), 0, s, a);
+    }
+}
+
+}  // namespace sc

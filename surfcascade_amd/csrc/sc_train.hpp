@@ -1,0 +1,96 @@
+// sc_train.hpp -- launch interface of the training kernels over a mined
+// sample matrix (sc_lr.hip: weak-learner responses, their gradient and the
+// logistic loss; sc_sample.hip: draws from scores).
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace sc {
+
+constexpr int kDesc = 32;  // values per descriptor (CalcFeature's 4 cells x 8 channels)
+
+struct LrArgs {
+    // sample matrix: sample i, patch p at x + i*ld + 32*p (elements)
+    const void *x;
+    long long ld;
+    int n, n_patches, dtype;
+    const int *rows;  // row r reads sample rows[r] (NULL: sample r); out of range: absent
+    int R;
+    // weak learners: m of them, h parameter sets each
+    int M, H;
+    const int *patch;  // NULL: learner m reads patch m; out of range: absent
+    const float *w, *b;
+    int act;
+    float alpha, beta;
+    // response
+    const float *res;
+    int res_kind;
+    long long res_ld;
+    float *y;
+    long long y_ld;
+    // gradient of a response
+    const float *dy;
+    long long dy_ld;
+    float *dres;
+    long long dres_ld;
+    // loss
+    const float *target, *weight;  // by sample; weight NULL: 1
+    // gradient / loss outputs
+    float *dw, *db, *loss;
+    float *part;        // partial sums per row chunk (NULL: one chunk, results written directly)
+    int chunks;         // row chunks (grid y)
+    int rows_per_wave;  // rows a wave walks
+};
+
+constexpr int kPartWords = kDesc + 2;  // per learner and set: dW, db, loss
+
+// the launch shape of the gradient / loss kernels (workspace = part)
+struct LrPlan {
+    int chunks, rows_per_wave;
+    size_t part_bytes;
+};
+LrPlan lr_plan(const LrArgs &a);
+
+void launch_lr_response(const LrArgs &a, hipStream_t s);
+void launch_lr_grad(const LrArgs &a, bool loss, hipStream_t s);  // + the join of its chunks
+void launch_lr_res_grad(const LrArgs &a, hipStream_t s);
+
+struct SampleArgs {
+    const void *scores;
+    int dtype, B, V;
+    long long ld;
+    const int *lens;  // NULL: V each; clamped to [0, V]
+    double temperature, top_p, min_p;
+    int top_k;
+    int shift;  // a weight of 1 is 2^shift units of mass (sample_shift)
+    const double *u;
+    int S;
+    long long u_ld;
+    int *index;
+    long long index_ld;
+    int *kept;  // may be NULL
+    void *ws;   // sample_plan's bytes (NULL: none)
+};
+
+// the launch shape of the draws, from B, V and S alone
+struct SamplePlan {
+    size_t ws_bytes;
+};
+SamplePlan sample_plan(const SampleArgs &a);
+
+constexpr int kMaxPool = 1 << 26;
+
+// Masses are 64-bit integers, so that sums do not depend on their order: a
+// weight w in [0, 1] is rint(w * 2^shift), the largest shift with which V
+// weights of 1 stay below 2^62 (52 at most: a double's mantissa).
+inline int sample_shift(int V) {
+    int lg = 0;
+    while ((1 << lg) < V) lg++;
+    return 62 - lg < 52 ? 62 - lg : 52;
+}
+
+void launch_sample(const SampleArgs &a, hipStream_t s);
+
+}  // namespace sc

@@ -1,0 +1,233 @@
+"""Draws from scores (sc_sample) against the definition: numpy in 64 bits,
+sorting what the kernel selects.  Places are whole numbers and have to be
+equal.  Weights are rounded to units of 2^-36 at most and cumulated weights
+differ from numpy's by about 1e-13 of a typical weight, so a random number
+would have to lie that near to a border for another place."""
+import numpy as np
+import pytest
+import torch
+
+import surfcascade_amd as sc
+
+pytestmark = pytest.mark.gpu
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(scope="module")
+def tr():
+    return sc.Trainer()
+
+
+def reference(scores, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, lens=None):
+    """(index, kept) of [b, v] scores (float64 numpy) and [b, s] numbers."""
+    index, kept = np.zeros(u.shape, np.int64), np.zeros(len(scores), np.int64)
+    for i, s in enumerate(scores):
+        s = s[:len(s) if lens is None else min(max(int(lens[i]), 0), len(s))]
+        pool = np.flatnonzero(s > -np.inf)
+        if not len(pool):
+            index[i], kept[i] = -1, 0
+            continue
+        order = pool[np.lexsort((pool, -s[pool]))]
+        best = s[order[0]]
+        if temperature == 0:
+            order = order[:1]
+        if top_k > 0:
+            order = order[:top_k]
+        with np.errstate(invalid="ignore", over="ignore"):
+            w = np.where(s[order] == best, 1.0, np.exp((s[order] - best) / (temperature or 1.0)))
+        n = len(order)
+        if top_p < 1:
+            c = np.cumsum(w)
+            n = 1 + int(np.searchsorted(c, top_p * c[-1], side="left"))
+        n = max(min(n, int(np.count_nonzero(w >= min_p))), 1)
+        chosen, w = order[:n], w[:n]
+        by = np.argsort(chosen)
+        c = np.cumsum(w[by])
+        x = np.clip(np.nan_to_num(u[i], nan=0.0), 0.0, 1.0) * c[-1]
+        at = np.searchsorted(c, x, side="right")
+        last = int(np.flatnonzero(w[by] > 0)[-1])
+        index[i], kept[i] = chosen[by][np.minimum(at, last)], n
+    return index, kept
+
+
+def _check(tr, scores, u, lens=None, **kw):
+    """scores: CPU [b, v] tensor of a type; u: CPU float64 [b, s]."""
+    want, wkept = reference(scores.double().numpy(), u.numpy(), lens=None if lens is None else lens.numpy(), **kw)
+    idx, kept = tr.sample(scores.cuda(), u.cuda(), lens=None if lens is None else lens.cuda(), **kw)
+    assert idx.dtype == torch.int32 and idx.shape == u.shape and kept.shape == (scores.shape[0],)
+    np.testing.assert_array_equal(kept.cpu().numpy(), wkept)
+    np.testing.assert_array_equal(idx.cpu().numpy(), want)
+
+
+def _inputs(b, v, s, seed, dtype="f32"):
+    g = torch.Generator().manual_seed(seed)
+    return (2 * torch.randn(b, v, generator=g)).to(DT[dtype]), torch.rand(b, s, generator=g, dtype=torch.float64)
+
+
+SIZES = [(1, 1, 1), (1, 2, 5), (3, 63, 7), (2, 64, 64), (1, 65, 3), (2, 1023, 33), (2, 1024, 32), (1, 1025, 31),
+         (4, 2047, 9), (1, 2049, 1000), (64, 300, 1), (2, 20011, 128), (1, 32768, 17), (2, 32769, 40),
+         (1, 70000, 5000), (3, 131071, 3)]
+TRIMS = [dict(), dict(temperature=0.5), dict(top_k=1), dict(top_k=17), dict(top_p=0.9), dict(top_p=0.3, temperature=2.0),
+         dict(min_p=0.05), dict(top_k=500, top_p=0.8, min_p=0.02, temperature=0.7), dict(temperature=0.0),
+         dict(top_p=0.0), dict(min_p=1.0), dict(top_k=10**9, top_p=0.999)]
+
+
+@pytest.mark.parametrize("size", SIZES, ids=str)
+@pytest.mark.parametrize("trim", TRIMS, ids=str)
+def test_draws(tr, size, trim):
+    scores, u = _inputs(*size, seed=size[1])
+    _check(tr, scores, u, **trim)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("trim", TRIMS, ids=str)
+def test_half_scores_tie(tr, dtype, trim):
+    """8 or 11 bits of score: most places tie with others, also at the cut."""
+    scores, u = _inputs(2, 9000, 200, 5, dtype)
+    _check(tr, scores, u, **trim)
+
+
+@pytest.mark.parametrize("v", [16, 4096, 40000])
+@pytest.mark.parametrize("trim", [dict(top_k=5), dict(top_k=4095), dict(top_p=0.5), dict(top_k=13, top_p=0.5),
+                                  dict(top_p=0.25, min_p=0.5), dict()], ids=str)
+def test_equal_scores(tr, v, trim):
+    """Every place ties: the lowest places are kept, and numbers that are
+    exactly at a border belong to the place behind it."""
+    scores = torch.full((2, v), 1.25)
+    u = torch.cat([torch.arange(16).double() / 16, torch.rand(50, dtype=torch.float64,
+                   generator=torch.Generator().manual_seed(1))])[None].repeat(2, 1)
+    _check(tr, scores, u, **trim)
+
+
+@pytest.mark.parametrize("trim", TRIMS, ids=str)
+def test_masked_places(tr, trim):
+    """Rows with masked places: -inf, the type's lowest value, NaN, nothing
+    left at all, one place left, +inf and -0."""
+    inf, nan, low = float("inf"), float("nan"), torch.finfo(torch.float32).min
+    v = 1500
+    g = torch.Generator().manual_seed(3)
+    scores = torch.randn(9, v, generator=g)
+    scores[0] = -inf
+    scores[1] = nan
+    scores[2] = -inf
+    scores[2, 777] = -3.0
+    scores[3, ::2] = -inf
+    scores[4, ::3] = nan
+    scores[5] = low
+    scores[6, 5:] = low
+    scores[7, 100] = scores[7, 900] = inf
+    scores[8] = torch.where(torch.rand(v, generator=g) < 0.5, 0.0, -0.0)
+    u = torch.rand(9, 40, generator=g, dtype=torch.float64)
+    _check(tr, scores, u, **trim)
+
+
+@pytest.mark.parametrize("trim", [dict(), dict(top_k=40, top_p=0.9)], ids=str)
+def test_lengths(tr, trim):
+    """Rows of their own lengths; what lies behind them (NaN, +inf) is not read."""
+    scores, u = _inputs(8, 5000, 20, 9)
+    lens = torch.tensor([0, 1, 2, 4999, 5000, -3, 2**31 - 1, 1024], dtype=torch.int32)
+    for i, n in enumerate(lens.tolist()):
+        n = min(max(n, 0), 5000)
+        scores[i, n:] = float("inf") if i % 2 else float("nan")
+    _check(tr, scores, u, lens=lens, **trim)
+
+
+def test_random_numbers_at_the_ends(tr):
+    scores, _ = _inputs(1, 3000, 1, 2)
+    scores[0, :3] = -float("inf")
+    scores[0, -2:] = -float("inf")
+    u = torch.tensor([[0.0, -1.0, float("nan"), 1.0 - 2.0**-53, 1.0, 5.0, float("inf"), -float("inf"), 2.0**-70]],
+                     dtype=torch.float64)
+    idx, _ = tr.sample(scores.cuda(), u.cuda())
+    first, last = 3, 2997
+    assert idx.cpu()[0].tolist() == [first, first, first, last, last, last, last, first, first]
+
+
+def test_frequencies(tr):
+    """A grid of numbers draws each place as often as its weight says, to one."""
+    scores, _ = _inputs(1, 500, 1, 4)
+    u = (torch.arange(100000, dtype=torch.float64) + 0.5)[None] / 100000
+    idx, _ = tr.sample(scores.cuda(), u.cuda())
+    got = np.bincount(idx.cpu().numpy()[0], minlength=500)
+    w = np.exp(scores[0].double().numpy())
+    assert np.abs(got - 100000 * w / w.sum()).max() <= 1.0
+
+
+def test_wide_range_and_outliers(tr):
+    """Keys of every exponent, and one far outlier over a narrow cluster."""
+    g = torch.Generator().manual_seed(6)
+    a = torch.randn(30000, generator=g).sign() * torch.exp(torch.empty(30000).uniform_(-80, 80, generator=g))
+    b = 0.4 + 1e-4 * torch.randn(30000, generator=g)
+    b[12345] = 1e30
+    c = 0.4 + 1e-4 * torch.randn(30000, generator=g)
+    c[54] = -1e30
+    scores = torch.stack([a, b, c])
+    u = torch.rand(3, 100, generator=g, dtype=torch.float64)
+    for trim in (dict(), dict(top_k=7000), dict(top_p=0.5), dict(top_k=100, top_p=0.7), dict(temperature=1e-3, top_p=0.9),
+                 dict(temperature=1e30, top_p=0.5)):
+        _check(tr, scores, u, **trim)
+
+
+def test_large_pool(tr):
+    scores, u = _inputs(1, 1000003, 4000, 8)
+    for trim in (dict(), dict(top_k=400000, top_p=0.97), dict(min_p=0.001, temperature=0.6)):
+        _check(tr, scores, u, **trim)
+
+
+def test_strides(tr):
+    """Rows of wider buffers, and offsets past 32 bits."""
+    scores, u = _inputs(3, 700, 11, 10)
+    wide = torch.full((3, 1001), float("inf"))
+    wide[:, 5:705] = scores
+    wu = torch.full((3, 20), 0.5, dtype=torch.float64)
+    wu[:, 3:14] = u
+    a = tr.sample(scores.cuda(), u.cuda(), top_p=0.9)
+    b = tr.sample(wide.cuda()[:, 5:705], wu.cuda()[:, 3:14], top_p=0.9)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    ld = 2**31 + 7
+    big = torch.empty(ld + 700, dtype=torch.bfloat16, device="cuda")
+    far = big.as_strided((2, 700), (ld, 1))
+    far.copy_(scores[:2])
+    c = tr.sample(far, u[:2].cuda())
+    d = tr.sample(scores[:2].bfloat16().cuda(), u[:2].cuda())
+    assert torch.equal(c[0], d[0])
+
+
+def test_one_row_and_empty_sizes(tr):
+    scores, u = _inputs(1, 50, 6, 11)
+    i1, k1 = tr.sample(scores[0].cuda(), u[0].cuda())
+    i2, k2 = tr.sample(scores.cuda(), u.cuda())
+    assert i1.shape == (6,) and torch.equal(i1, i2[0]) and torch.equal(k1, k2)
+    e = dict(device="cuda")
+    i, k = tr.sample(torch.zeros(3, 0, **e), torch.zeros(3, 4, dtype=torch.float64, **e))
+    assert (i == -1).all() and not k.any()
+    i, k = tr.sample(torch.zeros(3, 5, **e), torch.zeros(3, 0, dtype=torch.float64, **e))
+    assert i.shape == (3, 0) and (k == 5).all()
+    i, k = tr.sample(torch.zeros(0, 5, **e), torch.zeros(0, 2, dtype=torch.float64, **e))
+    assert i.shape == (0, 2) and k.shape == (0,)
+
+
+def test_refused_tensors(tr):
+    s, u = _inputs(2, 10, 3, 12)
+    S, Q = s.cuda(), u.cuda()
+    for bad in (lambda: tr.sample(s, Q), lambda: tr.sample(S, u), lambda: tr.sample(S, Q.float()),
+                lambda: tr.sample(S.double(), Q), lambda: tr.sample(S, Q[:1]), lambda: tr.sample(S[0], Q),
+                lambda: tr.sample(S.t().contiguous().t(), Q), lambda: tr.sample(S[:, ::2], Q),
+                lambda: tr.sample(S[:1].expand(2, 10), Q),
+                lambda: tr.sample(S, Q, lens=torch.zeros(2, dtype=torch.int64).cuda()),
+                lambda: tr.sample(S, Q, lens=torch.zeros(3, dtype=torch.int32).cuda())):
+        with pytest.raises(ValueError):
+            bad()
+    for kw in (dict(temperature=-1.0), dict(top_k=-1), dict(top_p=-0.5), dict(min_p=2.0)):
+        with pytest.raises(sc.SurfCascadeError) as e:
+            tr.sample(S, Q, **kw)
+        assert e.value.code == -1
+
+
+def test_same_call_same_bits(tr):
+    scores, u = _inputs(1, 200000, 3000, 13)
+    S, Q = scores.cuda(), u.cuda()
+    a = tr.sample(S, Q, top_k=90000, top_p=0.95)
+    for _ in range(3):
+        b = tr.sample(S, Q, top_k=90000, top_p=0.95)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
