@@ -28,6 +28,7 @@ namespace sc {
 namespace {
 
 constexpr int kWaves = 4;  // waves per workgroup
+constexpr int kNarrowSets = 4;  // parameter sets per learner up to which the narrow form runs
 
 struct F32 {
     static constexpr int kSize = 4;
@@ -135,18 +136,37 @@ __device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f
 
 enum Mode { kResponse = 0, kGrad = 1, kLoss = 2 };
 
-// g of one result and, for the loss, its term (e = exp(-|z|): neither
-// s = sigmoid(z) nor 1 - s = sigmoid(-z) is formed by a difference)
+// log(1 + e) / e for e in [0, 1]: a polynomial of degree 8 fitted for the
+// least relative error (3.0e-8; 2.8 roundings of 2^-24 as evaluated)
+__device__ __forceinline__ float log1p_over(float e) {
+    float p = 0.005232677f;
+    p = __builtin_fmaf(p, e, -0.029505169f);
+    p = __builtin_fmaf(p, e, 0.078225836f);
+    p = __builtin_fmaf(p, e, -0.13663235f);
+    p = __builtin_fmaf(p, e, 0.19106002f);
+    p = __builtin_fmaf(p, e, -0.24842981f);
+    p = __builtin_fmaf(p, e, 0.33319098f);
+    p = __builtin_fmaf(p, e, -0.49999493f);
+    return __builtin_fmaf(p, e, 0.99999994f);
+}
+
+// What a row brings to its results' gradients: for the loss its weight on
+// either side, pos = c (1 - t) and neg = c t; for a response pos = alpha dy.
+// With e = exp(-|z|) and d = 1 / (1 + e) the loss and its slope are
+//   c (softplus(z) - t z) = c log(1 + e) + (z >= 0 ? pos : -neg) z
+//   c (sigmoid(z) - t)    = d (z >= 0 ? pos - neg e : pos e - neg)
+// neither of which takes a difference of nearly equal numbers.  A NaN z is a
+// NaN e, and stays one.
 template <int MODE>
-__device__ __forceinline__ float grad_of(const LrArgs &a, float z, float c, float t, float &loss) {
+__device__ __forceinline__ float grad_of(int act, float z, float pos, float neg, float &loss) {
     const float e = __expf(-fabsf(z)), d = __fdividef(1.0f, 1.0f + e);
     if constexpr (MODE == kLoss) {
-        const float s = z >= 0.0f ? d : e * d, s1 = z >= 0.0f ? e * d : d;
-        loss += c * (log1pf(e) + (1.0f - t) * fmaxf(z, 0.0f) + t * fmaxf(-z, 0.0f));
-        const float g = c * ((1.0f - t) * s - t * s1);
-        return z != z ? z : g;  // (fmaxf drops a NaN; the gradient keeps it)
+        const bool up = z >= 0.0f;
+        const float near = up ? pos : -neg, far = up ? -neg : pos;
+        loss = __builtin_fmaf((pos + neg) * e, log1p_over(e), __builtin_fmaf(near, z, loss));
+        return d * __builtin_fmaf(far, e, near);
     } else {
-        return a.act == SC_ACT_SIGMOID ? c * e * d * d : c;  // c = alpha * dy
+        return act == SC_ACT_SIGMOID ? pos * e * d * d : pos;
     }
 }
 
@@ -200,11 +220,12 @@ __global__ __launch_bounds__(64 * kWaves) void lr_kernel(LrArgs a) {
             idx = a.rows ? a.rows[rq] : rq;
             if ((unsigned)idx >= (unsigned)a.n) idx = -1;
         }
-        float c = 0.0f, t = 0.0f;
+        float pos = 0.0f, neg = 0.0f;
         if constexpr (MODE == kLoss) {
             if (idx >= 0) {
-                c = a.weight ? a.weight[idx] : 1.0f;
-                t = a.target[idx];
+                const float c = a.weight ? a.weight[idx] : 1.0f, t = a.target[idx];
+                pos = c * (1.0f - t);
+                neg = c * t;
                 if (c == 0.0f) idx = -1;  // a row without weight is not looked at, whatever it holds
             }
         }
@@ -253,8 +274,8 @@ __global__ __launch_bounds__(64 * kWaves) void lr_kernel(LrArgs a) {
                 float g = 0.0f;
                 if (idx >= 0 && present && h0 + h < a.H) {
                     if constexpr (MODE == kGrad)
-                        c = a.alpha * a.dy[(long long)rq * a.dy_ld + (long long)m * a.H + h0 + h];
-                    g = grad_of<MODE>(a, z[h], c, t, sum_l[h]);
+                        pos = a.alpha * a.dy[(long long)rq * a.dy_ld + (long long)m * a.H + h0 + h];
+                    g = grad_of<MODE>(a.act, z[h], pos, neg, sum_l[h]);
                 }
                 sum_g[h] += g;
                 spread_rows<LPI>(g, q, g_all[h]);
@@ -295,6 +316,215 @@ __global__ __launch_bounds__(64 * kWaves) void lr_kernel(LrArgs a) {
             else if (word < kDesc) a.dw[mh * kDesc + word] = s;
             else if (word == kDesc) a.db[mh] = s;
             else if (MODE == kLoss) a.loss[mh] = s;
+        }
+    }
+}
+
+// Wide form, for many parameter sets: a wave owns one learner and 16 of its
+// sets and multiplies 16 rows at a time on the matrix cores (16x16x4, f32 in
+// and out, so nothing is rounded that the narrow form does not round).
+//   z = X W^T : lane (i = lane % 16, q = lane / 16) holds 8 values of row i's
+//               descriptor, the same 8 places of set i's weights; any order of
+//               the places will do, so each lane keeps what one 16-B load
+//               brings.  Result: set i, rows 4q .. 4q+3.
+//   dW = G^T X: that result is already the operand layout of the second
+//               product; X is read again with lane i = descriptor place (its
+//               lines are in the vector L1 from the first read).
+template <class T>
+struct WideRow;  // the 8 values of a lane's row and which places they are
+template <>
+struct WideRow<F32> {  // places 4q..4q+3 and 16+4q..: each load covers half a line of 16 rows
+    uint4_v a, b;
+    __device__ __forceinline__ void load(const char *p, int q) {
+        a = load16<F32>(p + q * 16);
+        b = load16<F32>(p + 64 + q * 16);
+    }
+    __device__ __forceinline__ void clear() { a = b = uint4_v{0, 0, 0, 0}; }
+    __device__ __forceinline__ void values(float *f) const {
+        unpack<F32>(a, f);
+        unpack<F32>(b, f + 4);
+    }
+    static __device__ __forceinline__ int place(int q, int k) { return (k & 4) * 4 + q * 4 + (k & 3); }
+};
+template <class T>
+struct WideRow {  // places 8q..8q+7
+    uint4_v a;
+    __device__ __forceinline__ void load(const char *p, int q) { a = load16<T>(p + q * 16); }
+    __device__ __forceinline__ void clear() { a = uint4_v{0, 0, 0, 0}; }
+    __device__ __forceinline__ void values(float *f) const { unpack<T>(a, f); }
+    static __device__ __forceinline__ int place(int q, int k) { return q * 8 + k; }
+};
+
+template <class T>
+__device__ __forceinline__ float load_one(const char *p) {
+    if constexpr (__is_same(T, F32)) return *reinterpret_cast<const float *>(p);
+    else if constexpr (__is_same(T, F16)) return (float)*reinterpret_cast<const _Float16 *>(p);
+    else return __uint_as_float((unsigned)*reinterpret_cast<const unsigned short *>(p) << 16);
+}
+
+typedef float float4_v __attribute__((ext_vector_type(4)));
+
+template <class T, int MODE>
+__global__ __launch_bounds__(64 * kWaves) void lr_wide_kernel(LrArgs a) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int i = lane & 15, q = lane >> 4;
+    const int sets = (a.H + 15) / 16;
+    // neighbouring waves: the sets of a learner, then the next learner (whose
+    // descriptors lie in the same lines)
+    const int unit = blockIdx.x * kWaves + wave;
+    const int m = unit / sets, h = (unit - m * sets) * 16 + i;
+    if (m >= a.M) return;
+    int p = a.patch ? a.patch[m] : m;
+    const bool present = (unsigned)p < (unsigned)a.n_patches;
+    if (!present) p = 0;
+    const bool on = h < a.H;
+    const long long mh = (long long)m * a.H + h;
+    float w[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) w[k] = on ? a.w[mh * kDesc + WideRow<T>::place(q, k)] : 0.0f;
+    const float bias = on && a.b ? a.b[mh] : 0.0f;
+    const long long r_lo = (long long)blockIdx.y * a.rows_per_wave;
+    const int r0 = (int)(r_lo < a.R ? r_lo : a.R);
+    const int r1 = (int)(r_lo + a.rows_per_wave < a.R ? r_lo + a.rows_per_wave : a.R);
+    const char *x = static_cast<const char *>(a.x) + (long long)p * kDesc * T::kSize;
+    const long long step = a.ld * T::kSize;
+    float4_v acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    float sum_g = 0.0f, sum_l = 0.0f;
+    // Two stages ahead of the products: the rows' numbers (and weights), then
+    // their descriptors, so a wave always has one tile of loads in flight.
+    // Absent rows load sample 0 instead and are cleared where they are used:
+    // a tile without any (every tile but the last, mostly) has no branches.
+    struct Meta {
+        int idx;
+        float pos, neg;
+    };
+    auto load_meta = [&](int r) {
+        Meta u{-1, 0.0f, 0.0f};
+        if (r + i < r1) {
+            u.idx = a.rows ? a.rows[r + i] : r + i;
+            if ((unsigned)u.idx >= (unsigned)a.n) u.idx = -1;
+        }
+        if constexpr (MODE == kLoss) {
+            if (u.idx >= 0) {
+                const float c = a.weight ? a.weight[u.idx] : 1.0f, t = a.target[u.idx];
+                u.pos = c * (1.0f - t);
+                u.neg = c * t;
+                if (c == 0.0f) u.idx = -1;  // a row without weight is not looked at, whatever it holds
+            }
+        }
+        return u;
+    };
+    struct Tile {
+        Meta u;
+        WideRow<T> xr;
+        float xc[2][4];  // rows 4q .. 4q+3 (those of this lane's results), places i and 16+i
+        float d[4];      // dy or residual of those results
+        bool whole;      // no row of it is absent
+    };
+    const long long col = on ? mh : (long long)m * a.H;  // (lanes past the sets read the first one's)
+    auto load_tile = [&](int r, Meta u) {
+        Tile v;
+        v.u = u;
+        v.whole = present && __ballot(u.idx < 0) == 0;
+        const int j = u.idx < 0 ? 0 : u.idx;
+        v.xr.load(x + j * step, q);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int row = r + q * 4 + k < r1 ? r + q * 4 + k : r0;
+            if constexpr (MODE == kResponse) {
+                if (a.res_kind != SC_RES_NONE)
+                    v.d[k] = a.res[(long long)row * a.res_ld + (a.res_kind == SC_RES_FULL ? col : 0)];
+            } else {
+                if constexpr (MODE == kGrad) v.d[k] = a.dy[(long long)row * a.dy_ld + col];
+                const char *at = x + __shfl(j, q * 4 + k, 64) * step + i * T::kSize;
+                v.xc[0][k] = load_one<T>(at);
+                v.xc[1][k] = load_one<T>(at + 16 * T::kSize);
+            }
+        }
+        return v;
+    };
+    auto products = [&](int r, Tile &v) {
+        float f[8];
+        v.xr.values(f);
+        float4_v z = {bias, bias, bias, bias};
+#pragma unroll
+        for (int k = 0; k < 8; k++) z = __builtin_amdgcn_mfma_f32_16x16x4f32(f[k], w[k], z, 0, 0, 0);
+        if constexpr (MODE == kResponse) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int row = r + q * 4 + k;
+                float y = a.alpha * (a.act == SC_ACT_SIGMOID ? sigmoid(z[k]) : z[k]);
+                if (!v.whole && (!present || __shfl(v.u.idx, q * 4 + k, 64) < 0)) y = 0.0f;  // absent: no response
+                if (a.res_kind != SC_RES_NONE) y += a.beta * v.d[k];
+                if (on && row < r1) a.y[(long long)row * a.y_ld + mh] = y;
+            }
+        } else {
+            float g[4], l = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                float pos, neg = 0.0f;
+                if constexpr (MODE == kLoss) {
+                    pos = __shfl(v.u.pos, q * 4 + k, 64);
+                    neg = __shfl(v.u.neg, q * 4 + k, 64);
+                } else {
+                    pos = a.alpha * v.d[k];
+                }
+                if (v.whole) {
+                    g[k] = grad_of<MODE>(a.act, z[k], pos, neg, l);
+                } else {
+                    const bool there = present && __shfl(v.u.idx, q * 4 + k, 64) >= 0;
+                    float lk = 0.0f;
+                    const float gk = grad_of<MODE>(a.act, z[k], pos, neg, lk);
+                    g[k] = there ? gk : 0.0f;
+                    l += there ? lk : 0.0f;
+                    v.xc[0][k] = there ? v.xc[0][k] : 0.0f;
+                    v.xc[1][k] = there ? v.xc[1][k] : 0.0f;
+                }
+                sum_g += g[k];
+            }
+            sum_l += l;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                acc[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(g[k], v.xc[0][k], acc[0], 0, 0, 0);
+                acc[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(g[k], v.xc[1][k], acc[1], 0, 0, 0);
+            }
+        }
+    };
+    Meta meta = load_meta(r0 + 16);
+    Tile one = load_tile(r0, load_meta(r0)), two;
+    for (int r = r0; r < r1; r += 32) {
+        two = load_tile(r + 16, meta);
+        meta = load_meta(r + 32);
+        products(r, one);
+        if (r + 16 >= r1) break;
+        one = load_tile(r + 32, meta);
+        meta = load_meta(r + 48);
+        products(r + 16, two);
+    }
+    if constexpr (MODE != kResponse) {
+        sum_g += __shfl_xor(sum_g, 16, 64);
+        sum_g += __shfl_xor(sum_g, 32, 64);
+        sum_l += __shfl_xor(sum_l, 16, 64);
+        sum_l += __shfl_xor(sum_l, 32, 64);
+        const int h0 = (unit - m * sets) * 16;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {  // set 4q+k, places i and 16+i
+            const int hk = h0 + q * 4 + k;
+            if (hk >= a.H) continue;
+            const long long at = (long long)m * a.H + hk;
+            float *to = a.part ? a.part + ((long long)blockIdx.y * a.M * a.H + at) * kPartWords : a.dw + at * kDesc;
+            to[i] = acc[0][k];
+            to[16 + i] = acc[1][k];
+        }
+        if (on && q == 0) {
+            if (a.part) {
+                float *to = a.part + ((long long)blockIdx.y * a.M * a.H + mh) * kPartWords;
+                to[kDesc] = sum_g;
+                to[kDesc + 1] = sum_l;
+            } else {
+                a.db[mh] = sum_g;
+                if (MODE == kLoss) a.loss[mh] = sum_l;
+            }
         }
     }
 }
@@ -351,8 +581,14 @@ int sets_per_wave(const LrArgs &a) { return a.H == 1 ? 1 : a.H == 2 ? 2 : 4; }
 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
+bool wide(const LrArgs &a) { return a.H > kNarrowSets; }
+
 template <class T, int MODE>
-void launch_narrow(const LrArgs &a, dim3 grid, hipStream_t s) {
+void launch_form(const LrArgs &a, dim3 grid, hipStream_t s) {
+    if (wide(a)) {
+        hipLaunchKernelGGL((lr_wide_kernel<T, MODE>), grid, dim3(64 * kWaves), 0, s, a);
+        return;
+    }
     switch (sets_per_wave(a)) {
         case 1: hipLaunchKernelGGL((lr_kernel<T, 1, MODE>), grid, dim3(64 * kWaves), 0, s, a); break;
         case 2: hipLaunchKernelGGL((lr_kernel<T, 2, MODE>), grid, dim3(64 * kWaves), 0, s, a); break;
@@ -363,47 +599,49 @@ void launch_narrow(const LrArgs &a, dim3 grid, hipStream_t s) {
 template <int MODE>
 void launch_mode(const LrArgs &a, dim3 grid, hipStream_t s) {
     switch (a.dtype) {
-        case SC_F32: launch_narrow<F32, MODE>(a, grid, s); break;
-        case SC_F16: launch_narrow<F16, MODE>(a, grid, s); break;
-        default: launch_narrow<BF16, MODE>(a, grid, s); break;
+        case SC_F32: launch_form<F32, MODE>(a, grid, s); break;
+        case SC_F16: launch_form<F16, MODE>(a, grid, s); break;
+        default: launch_form<BF16, MODE>(a, grid, s); break;
     }
 }
 
 }  // namespace
 
-// Gradient and loss: rows are cut into chunks of kWaves wave ranges until the
-// grid has a few waves per SIMD of the 256 CUs.
+// Gradient and loss: rows are cut into chunks until the grid has a few waves
+// per SIMD of the 256 CUs; a chunk is one range of rows per wave of a
+// workgroup (narrow form), or one for all of them (wide form).
 LrPlan lr_plan(const LrArgs &a) {
     LrPlan p{0, 0, 0};
     if (a.R == 0) return p;
-    const int lpi = lanes_per_item(a);
-    const long long tiles = ceil_div(a.M, items_per_wave(a)) * ceil_div(a.H, sets_per_wave(a));
-    const long long most = ceil_div(a.R, (long long)kWaves * lpi);
-    long long chunks = ceil_div(4096, tiles * kWaves);
-    if (chunks > most) chunks = most;
-    p.rows_per_wave = (int)(ceil_div(ceil_div(a.R, chunks * kWaves), lpi) * lpi);
-    p.chunks = (int)ceil_div(a.R, (long long)p.rows_per_wave * kWaves);
+    const int step = wide(a) ? 16 : lanes_per_item(a), ranges = wide(a) ? 1 : kWaves;
+    const long long waves = wide(a) ? a.M * ceil_div(a.H, 16)
+                                    : ceil_div(a.M, items_per_wave(a)) * ceil_div(a.H, sets_per_wave(a)) * kWaves;
+    long long chunks = ceil_div(4096, waves);
+    if (chunks > ceil_div(a.R, (long long)ranges * step)) chunks = ceil_div(a.R, (long long)ranges * step);
+    p.rows_per_wave = (int)(ceil_div(ceil_div(a.R, chunks * ranges), step) * step);
+    p.chunks = (int)ceil_div(a.R, (long long)p.rows_per_wave * ranges);
     if (p.chunks > 1) p.part_bytes = (size_t)p.chunks * a.M * a.H * kPartWords * sizeof(float);
     return p;
 }
 
 void launch_lr_response(const LrArgs &a0, hipStream_t s) {
     LrArgs a = a0;
-    const int lpi = lanes_per_item(a);
-    const long long tiles = ceil_div(a.M, (long long)items_per_wave(a) * kWaves);
-    const long long hs = ceil_div(a.H, sets_per_wave(a));
+    const int step = wide(a) ? 16 : lanes_per_item(a);
+    const long long units = wide(a) ? a.M * ceil_div(a.H, 16) : ceil_div(a.M, items_per_wave(a));
+    const long long wgs = ceil_div(units, kWaves), hs = wide(a) ? 1 : ceil_div(a.H, sets_per_wave(a));
     // rows per wave: enough waves for the chip, at most 64 rows, at most 65535 chunks
-    long long rows = ceil_div(ceil_div(a.R, ceil_div(8192, tiles * hs * kWaves)), lpi) * lpi;
+    long long rows = ceil_div(ceil_div(a.R, ceil_div(8192, wgs * hs * kWaves)), step) * step;
     if (rows > 64) rows = 64;
-    const long long least = ceil_div(ceil_div(a.R, 65535), lpi) * lpi;
+    const long long least = ceil_div(ceil_div(a.R, 65535), step) * step;
     a.rows_per_wave = (int)(rows > least ? rows : least);
-    launch_mode<kResponse>(a, dim3((unsigned)tiles, (unsigned)ceil_div(a.R, a.rows_per_wave), (unsigned)hs), s);
+    launch_mode<kResponse>(a, dim3((unsigned)wgs, (unsigned)ceil_div(a.R, a.rows_per_wave), (unsigned)hs), s);
 }
 
 void launch_lr_grad(const LrArgs &a, bool loss, hipStream_t s) {
     if (a.chunks > 0) {
-        const dim3 grid((unsigned)ceil_div(a.M, items_per_wave(a)), (unsigned)a.chunks,
-                        (unsigned)ceil_div(a.H, sets_per_wave(a)));
+        const dim3 grid = wide(a) ? dim3((unsigned)ceil_div(a.M * ceil_div(a.H, 16), kWaves), (unsigned)a.chunks)
+                                  : dim3((unsigned)ceil_div(a.M, items_per_wave(a)), (unsigned)a.chunks,
+                                         (unsigned)ceil_div(a.H, sets_per_wave(a)));
         if (loss) launch_mode<kLoss>(a, grid, s);
         else launch_mode<kGrad>(a, grid, s);
     }

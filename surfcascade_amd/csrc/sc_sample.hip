@@ -13,11 +13,14 @@
 // no sort.  Weights are doubles and masses integers (sample_shift), so a sum
 // is the same in any order and a draw never depends on how the row was split.
 //
-// One workgroup per row.  The threshold comes from a radix descent of 11 bits
-// a pass over the row's own key range (bins hold counts for top_k, masses for
-// top_p), then each thread owns a contiguous part of the row, one block scan
-// gives every part's first cumulated mass, and a draw is a binary search over
-// the parts and a walk through one.
+// The threshold comes from a radix descent of 11 bits a pass over the row's own
+// key range: bins hold counts for top_k, masses for top_p, and the bin where
+// the sum from the top crosses is split again.  Cumulated masses then need one
+// pass in place order, and a draw is a search through them.
+//
+// Rows of up to kRowScores scores: one workgroup each, one launch; a thread
+// holds its keys and masses in registers through all passes.  Longer rows: many
+// workgroups, one launch per pass (below).
 #include <hip/hip_runtime.h>
 
 #include "sc_train.hpp"
@@ -28,7 +31,6 @@ namespace sc {
 namespace {
 
 typedef unsigned long long u64;
-constexpr int kThreads = 1024;
 constexpr int kBinBits = 11, kBins = 1 << kBinBits;
 
 // Order-preserving key of a score; 0: absent (-inf or NaN).
@@ -41,232 +43,859 @@ __device__ __forceinline__ float score_of(unsigned key) {
     return __uint_as_float((key & 0x80000000u) ? key ^ 0x80000000u : ~key);
 }
 
-__device__ __forceinline__ unsigned load_key(const SampleArgs &a, long long base, int i) {
-    if (a.dtype == SC_F32) return key_of(static_cast<const float *>(a.scores)[base + i]);
-    if (a.dtype == SC_F16) return key_of((float)static_cast<const _Float16 *>(a.scores)[base + i]);
-    return key_of(__uint_as_float((unsigned)static_cast<const unsigned short *>(a.scores)[base + i] << 16));
+// The keys of K places of a row of n scores (0 past its end): every load is
+// issued before the first is used.
+template <int K, class Place>
+__device__ __forceinline__ void load_keys(const SampleArgs &a, long long base, int n, unsigned (&key)[K], Place place) {
+    if (n == 0) {
+#pragma unroll
+        for (int j = 0; j < K; j++) key[j] = 0;
+        return;
+    }
+    float f[K];
+    if (a.dtype == SC_F32) {
+        const float *p = static_cast<const float *>(a.scores) + base;
+#pragma unroll
+        for (int j = 0; j < K; j++) f[j] = p[place(j) < n ? place(j) : n - 1];
+    } else {
+        const unsigned short *p = static_cast<const unsigned short *>(a.scores) + base;
+        unsigned short h[K];
+#pragma unroll
+        for (int j = 0; j < K; j++) h[j] = p[place(j) < n ? place(j) : n - 1];
+#pragma unroll
+        for (int j = 0; j < K; j++)
+            f[j] = a.dtype == SC_F16 ? (float)__builtin_bit_cast(_Float16, h[j]) : __uint_as_float((unsigned)h[j] << 16);
+    }
+#pragma unroll
+    for (int j = 0; j < K; j++) key[j] = place(j) < n ? key_of(f[j]) : 0;
+}
+
+// e^x for x <= 0 to 2^-51: x = n ln 2 + r with |r| <= ln 2 / 2, the Taylor
+// series of e^r to r^12 (remainder 0.35^13 / 13! = 2e-16), times 2^n.
+__device__ __forceinline__ double exp_neg(double x) {
+    x = x < -800.0 ? -800.0 : x;  // (2^-1154: 0)
+    const double n = rint(x * 1.44269504088896340736);
+    double r = __builtin_fma(n, -0.693147180559945286227, x);
+    r = __builtin_fma(n, -2.319046813846299558e-17, r);
+    double p = 1.0 / 479001600.0;
+    p = __builtin_fma(p, r, 1.0 / 39916800.0);
+    p = __builtin_fma(p, r, 1.0 / 3628800.0);
+    p = __builtin_fma(p, r, 1.0 / 362880.0);
+    p = __builtin_fma(p, r, 1.0 / 40320.0);
+    p = __builtin_fma(p, r, 1.0 / 5040.0);
+    p = __builtin_fma(p, r, 1.0 / 720.0);
+    p = __builtin_fma(p, r, 1.0 / 120.0);
+    p = __builtin_fma(p, r, 1.0 / 24.0);
+    p = __builtin_fma(p, r, 1.0 / 6.0);
+    p = __builtin_fma(p, r, 0.5);
+    p = __builtin_fma(p, r, 1.0);
+    p = __builtin_fma(p, r, 1.0);
+    return ldexp(p, (int)n);
 }
 
 struct Weigh {
     float top;
-    double rate;  // 1 / temperature
+    double rate;  // 1 / temperature (0: infinite, every weight but the best's is 0)
     double unit;  // 2^shift
     __device__ __forceinline__ double weight(unsigned key) const {
         const float s = score_of(key);
-        return s == top ? 1.0 : exp(((double)s - (double)top) * rate);  // (also +inf against +inf)
+        return s == top ? 1.0 : exp_neg(((double)s - (double)top) * rate);  // (also +inf against +inf)
     }
     __device__ __forceinline__ u64 mass(double w) const { return (u64)rint(w * unit); }
 };
 
-template <class V>
-__device__ __forceinline__ V wave_scan(V x, int lane) {  // inclusive
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const V o = __shfl_up(x, d, 64);
-        if (lane >= d) x += o;
+// Inclusive sum over the lanes of a wave: DPP shifts by 1, 2, 4 and 8 inside
+// the rows of 16, then the last lanes of rows broadcast into the rows behind
+// (a shuffle through LDS takes several times as long a step).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned dpp_or_0(unsigned v) {
+    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS, class V>
+__device__ __forceinline__ V scan_step(V x) {
+    if constexpr (sizeof(V) == 8) {
+        const unsigned lo = dpp_or_0<CTRL, ROWS>((unsigned)x), hi = dpp_or_0<CTRL, ROWS>((unsigned)(x >> 32));
+        return x + (((u64)hi << 32) | lo);
+    } else {
+        return x + dpp_or_0<CTRL, ROWS>(x);
     }
-    return x;
+}
+template <class V>
+__device__ __forceinline__ V wave_scan(V x) {
+    x = scan_step<0x111, 0xf>(x);
+    x = scan_step<0x112, 0xf>(x);
+    x = scan_step<0x114, 0xf>(x);
+    x = scan_step<0x118, 0xf>(x);
+    x = scan_step<0x142, 0xa>(x);
+    return scan_step<0x143, 0xc>(x);
+}
+__device__ __forceinline__ unsigned lane_of(unsigned v, int lane) {
+    return (unsigned)__builtin_amdgcn_readlane((int)v, lane);
+}
+__device__ __forceinline__ u64 lane_of(u64 v, int lane) {
+    return ((u64)lane_of((unsigned)(v >> 32), lane) << 32) | lane_of((unsigned)v, lane);
+}
+template <class V>
+__device__ __forceinline__ V wave_sum(V x) {
+    return lane_of(wave_scan(x), 63);
 }
 
-// inclusive block scan; total in every thread
-template <class V>
+// inclusive sum over the N threads of a workgroup; total in every thread
+template <int N, class V>
 __device__ __forceinline__ V block_scan(V x, V *s_wave, V &total) {
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-    x = wave_scan(x, lane);
+    const int wv = threadIdx.x >> 6;
+    x = wave_scan(x);
     __syncthreads();
-    if (lane == 63) s_wave[wv] = x;
+    if ((threadIdx.x & 63) == 63) s_wave[wv] = x;
     __syncthreads();
     V before = 0;
     total = 0;
-    for (int k = 0; k < kThreads / 64; k++) {
-        before += k < wv ? s_wave[k] : 0;
-        total += s_wave[k];
+#pragma unroll
+    for (int k = 0; k < N / 64; k++) {
+        const V v = s_wave[k];
+        before += k < wv ? v : 0;
+        total += v;
     }
     return before + x;
 }
 
-struct Found {
-    unsigned key;  // the key where the descending sum first reaches `need`
-    u64 left;      // what is still needed from the places with that key
+// smallest and largest key and the count over a workgroup of N threads
+template <int N>
+__device__ __forceinline__ void block_extent(unsigned &lo, unsigned &hi, unsigned &c, unsigned *s_x) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+        const unsigned l = __shfl_xor(lo, d, 64), h = __shfl_xor(hi, d, 64);
+        lo = l < lo ? l : lo;
+        hi = h > hi ? h : hi;
+    }
+    c = wave_sum(c);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+        s_x[3 * (threadIdx.x >> 6)] = lo;
+        s_x[3 * (threadIdx.x >> 6) + 1] = hi;
+        s_x[3 * (threadIdx.x >> 6) + 2] = c;
+    }
+    __syncthreads();
+    c = 0;
+#pragma unroll
+    for (int k = 0; k < N / 64; k++) {
+        lo = s_x[3 * k] < lo ? s_x[3 * k] : lo;
+        hi = s_x[3 * k + 1] > hi ? s_x[3 * k + 1] : hi;
+        c += s_x[3 * k + 2];
+    }
+}
+
+// floor(u * mass) for u clamped to [0, 1): below the mass
+__device__ __forceinline__ u64 target_of(double u, u64 mass) {
+    const u64 r = u > 0.0 ? (u < 1.0 ? (u64)(u * 18446744073709551616.0) : ~0ull) : 0;
+    return __umul64hi(r, mass);
+}
+
+__device__ __forceinline__ u64 need_of(double share, u64 total) {  // at least 1, at most all
+    const u64 need = (u64)ceil(share * (double)total);
+    return need < 1 ? 1 : need > total ? total : need;
+}
+
+// ---- rows for one workgroup -----------------------------------------------------
+
+template <int N>
+struct RowShared {
+    u64 bins[kBins];     // (later: cumulated masses of the threads' places)
+    unsigned ties[N];    // ties before each thread's places
+    u64 wave[N / 64];
+    unsigned x[3 * (N / 64)];
+    unsigned key;        // what a descent found
+    u64 left;
 };
 
-// Radix descent: the largest key whose descending sum over the pool's bins
-// reaches `need`.  fill(lo, shift, bins) adds every pool member whose key lies
-// in [lo, lo + (bins << shift)) to s_bin[(key - lo) >> shift]: the whole pool
-// first, then the one bin where the sum crosses.
-template <class Fill, class Need>
-__device__ Found descend(unsigned kmin, unsigned kmax, u64 *s_bin, u64 *s_wave, Found *s_found, Fill fill, Need need_of) {
+// Radix descent: the largest key at which the pool's sum from the top reaches
+// need (need = 0: share of the whole), and what its ties still have to bring.
+// fill(lo, shift, bins) adds what every pool member with a key in
+// [lo, lo + (bins << shift)) counts for to bins[(key - lo) >> shift]: the whole
+// pool first, then the one bin where the sum crosses.
+template <int N, class Fill>
+__device__ void descend(RowShared<N> &s, unsigned kmin, unsigned kmax, u64 need, double share, Fill fill,
+                        unsigned &key, u64 &left) {
+    constexpr int kPer = kBins / N;
     int shift = 0;
     while (((kmax - kmin) >> shift) >= kBins) shift++;
     unsigned lo = kmin, bins = kBins;
-    u64 need = 0;
-    for (bool first = true;; first = false) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < kBins; i += kThreads) s_bin[i] = 0;
+    for (;;) {
+        for (int i = threadIdx.x; i < kBins; i += N) s.bins[i] = 0;
         __syncthreads();
         fill(lo, shift, bins);
         __syncthreads();
-        // bins from the top: thread t has bins kBins-1-2t and kBins-2-2t
-        const int hi_bin = kBins - 1 - 2 * (int)threadIdx.x;
-        const u64 v1 = s_bin[hi_bin], v0 = s_bin[hi_bin - 1];
-        u64 total;
-        const u64 upto = block_scan<u64>(v1 + v0, s_wave, total);
-        if (first) need = need_of(total);
-        const u64 before = upto - v1 - v0;
-        if (before < need && need <= upto) {
-            const bool in_hi = need <= before + v1;
-            s_found->key = lo + ((unsigned)(in_hi ? hi_bin : hi_bin - 1) << shift);
-            s_found->left = need - before - (in_hi ? 0 : v1);
+        const int top = kBins - 1 - kPer * (int)threadIdx.x;  // this thread: bins top, top-1, ...
+        u64 v[kPer], sum = 0, total;
+#pragma unroll
+        for (int j = 0; j < kPer; j++) sum += v[j] = s.bins[top - j];
+        u64 before = block_scan<N, u64>(sum, s.wave, total) - sum;
+        if (need == 0) need = need_of(share, total);
+        if (before < need && need <= before + sum) {
+#pragma unroll
+            for (int j = 0; j < kPer; j++) {
+                if (before < need && need <= before + v[j]) {
+                    s.key = lo + ((unsigned)(top - j) << shift);
+                    s.left = need - before;
+                }
+                before += v[j];
+            }
         }
         __syncthreads();
-        const Found f = *s_found;
-        if (shift == 0) return f;
-        lo = f.key;
-        need = f.left;
+        key = s.key;
+        left = s.left;
+        if (shift == 0) return;
+        lo = key;
+        need = left;
         bins = shift > kBinBits ? kBins : 1u << shift;
         shift = shift > kBinBits ? shift - kBinBits : 0;
     }
 }
 
-__global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a) {
-    __shared__ u64 s_bin[kBins];  // (later: the parts' cumulated masses)
-    __shared__ u64 s_wave[kThreads / 64];
-    __shared__ unsigned s_min, s_max, s_count;
-    __shared__ Found s_found;
+// N threads, each with K neighbouring places: keys and masses in registers,
+// the keys in LDS too for the draws.
+template <int N, int K>
+__global__ __launch_bounds__(N) void sample_row_kernel(SampleArgs a) {
+    __shared__ RowShared<N> s;
+    __shared__ unsigned s_key[N * K];
     const int row = blockIdx.x, tid = threadIdx.x;
     int n = a.lens ? a.lens[row] : a.V;
     n = n < 0 ? 0 : n > a.V ? a.V : n;
     const long long base = row * a.ld;
     int *index = a.index + row * a.index_ld;
-
-    if (tid == 0) {
-        s_min = 0xffffffffu;
-        s_max = 0;
-        s_count = 0;
-    }
-    __syncthreads();
+    // neighbouring lanes load neighbouring places; the keys change owners in LDS
     {
-        unsigned lo = 0xffffffffu, hi = 0, c = 0;
-        for (int i = tid; i < n; i += kThreads) {
-            const unsigned k = load_key(a, base, i);
-            if (!k) continue;
-            lo = k < lo ? k : lo;
-            hi = k > hi ? k : hi;
-            c++;
-        }
-        if (c) {
-            atomicMin(&s_min, lo);
-            atomicMax(&s_max, hi);
-            atomicAdd(&s_count, c);
-        }
+        unsigned k[K];
+        load_keys<K>(a, base, n, k, [&](int j) { return j * N + tid; });
+#pragma unroll
+        for (int j = 0; j < K; j++) s_key[j * N + tid] = k[j];
     }
     __syncthreads();
-    const unsigned kmin = s_min, kmax = s_max, count = s_count;
+    unsigned key[K];
+    unsigned kmin = 0xffffffffu, kmax = 0, count = 0;
+#pragma unroll
+    for (int j = 0; j < K; j++) {
+        key[j] = s_key[tid * K + j];
+        if (key[j]) {
+            kmin = key[j] < kmin ? key[j] : kmin;
+            kmax = key[j] > kmax ? key[j] : kmax;
+            count++;
+        }
+    }
+    block_extent<N>(kmin, kmax, count, s.x);
     if (count == 0) {  // nothing to draw from
-        for (int j = tid; j < a.S; j += kThreads) index[j] = -1;
+        for (int j = tid; j < a.S; j += N) index[j] = -1;
         if (a.kept && tid == 0) a.kept[row] = 0;
         return;
     }
-    const int top_k = a.temperature == 0.0 ? 1 : a.top_k;  // temperature 0: the best place
-    const Weigh wg{score_of(kmax), a.temperature == 0.0 ? 0.0 : 1.0 / a.temperature, ldexp(1.0, a.shift)};
-
-    unsigned thr = 0;         // places with a larger key are kept,
-    u64 quota = ~0ull;        // and this many of those with this key
-    if (top_k > 0 && (unsigned)top_k < count) {
-        const Found f = descend(kmin, kmax, s_bin, s_wave, &s_found,
-            [&](unsigned lo, int shift, unsigned bins) {
-                for (int i = tid; i < n; i += kThreads) {
-                    const unsigned k = load_key(a, base, i);
-                    if (k && k >= lo && ((k - lo) >> shift) < bins) atomicAdd(&s_bin[(k - lo) >> shift], 1ull);
-                }
-            },
-            [&](u64) { return (u64)top_k; });
-        thr = f.key;
-        quota = f.left;
+    const Weigh wg{score_of(kmax), 1.0 / a.temperature, ldexp(1.0, a.shift)};
+    u64 mass[K];
+    unsigned low = 0;  // places under min_p
+#pragma unroll
+    for (int j = 0; j < K; j++) {
+        const double w = key[j] ? wg.weight(key[j]) : 0.0;
+        mass[j] = wg.mass(w);
+        low |= (unsigned)(w < a.min_p) << j;
     }
+
+    const int top_k = a.temperature == 0.0 ? 1 : a.top_k;  // temperature 0: the best place
+    unsigned thr = 0;   // places with a larger key are kept,
+    u64 quota = ~0ull;  // and this many of those with this key
+    if (top_k > 0 && (unsigned)top_k < count)
+        descend<N>(s, kmin, kmax, (u64)top_k, 0.0,
+            [&](unsigned lo, int shift, unsigned bins) {
+#pragma unroll
+                for (int j = 0; j < K; j++)
+                    if (key[j] && key[j] >= lo && ((key[j] - lo) >> shift) < bins)
+                        atomicAdd(&s.bins[(key[j] - lo) >> shift], 1ull);
+            },
+            thr, quota);
     if (a.top_p < 1.0) {
         const unsigned thr_k = thr;
         const u64 quota_k = quota;
-        const Found f = descend(kmin, kmax, s_bin, s_wave, &s_found,
+        u64 left;
+        descend<N>(s, kmin, kmax, 0, a.top_p,
             [&](unsigned lo, int shift, unsigned bins) {
-                for (int i = tid; i < n; i += kThreads) {
-                    const unsigned k = load_key(a, base, i);
-                    if (k > thr_k && k >= lo && ((k - lo) >> shift) < bins)
-                        atomicAdd(&s_bin[(k - lo) >> shift], wg.mass(wg.weight(k)));
-                }
+#pragma unroll
+                for (int j = 0; j < K; j++)
+                    if (key[j] > thr_k && key[j] >= lo && ((key[j] - lo) >> shift) < bins)
+                        atomicAdd(&s.bins[(key[j] - lo) >> shift], mass[j]);
                 if (tid == 0 && thr_k && thr_k >= lo && ((thr_k - lo) >> shift) < bins)  // the ties top_k keeps
-                    atomicAdd(&s_bin[(thr_k - lo) >> shift], quota_k * wg.mass(wg.weight(thr_k)));
+                    atomicAdd(&s.bins[(thr_k - lo) >> shift], quota_k * wg.mass(wg.weight(thr_k)));
             },
-            [&](u64 total) {
-                const u64 need = (u64)ceil(a.top_p * (double)total);
-                return need < 1 ? 1 : need > total ? total : need;
-            });
-        const u64 each = wg.mass(wg.weight(f.key));
-        thr = f.key;
-        quota = (f.left + each - 1) / each;
+            thr, left);
+        const u64 each = wg.mass(wg.weight(thr));
+        quota = (left + each - 1) / (each ? each : 1);
     }
 
-    // each thread owns places [i0, i1): ties in place order, then masses
-    const int per = (n + kThreads - 1) / kThreads;
-    const long long first = (long long)tid * per;
-    const int i0 = (int)(first < n ? first : n), i1 = (int)(first + per < n ? first + per : n);
-    u64 ties = 0;
-    if (thr)
-        for (int i = i0; i < i1; i++) ties += load_key(a, base, i) == thr;
-    u64 total;
-    const u64 ties_before = block_scan<u64>(ties, s_wave, total) - ties;
-    auto walk = [&](u64 tie, int from, int to, auto visit) {
-        for (int i = from; i < to; i++) {
-            const unsigned k = load_key(a, base, i);
-            if (!k || k < thr || (k == thr && tie++ >= quota)) continue;
-            const double w = wg.weight(k);
-            if (w < a.min_p) continue;
-            if (visit(i, wg.mass(w))) return;
-        }
-    };
-    u64 mass = 0, kept = 0;
-    walk(ties_before, i0, i1, [&](int, u64 q) {
-        mass += q;
-        kept++;
-        return false;
-    });
-    u64 kept_all, mass_all;
-    block_scan<u64>(kept, s_wave, kept_all);
-    const u64 upto = block_scan<u64>(mass, s_wave, mass_all);
+    // what is kept, in place order
+    unsigned ties = 0;
+    if (thr) {
+#pragma unroll
+        for (int j = 0; j < K; j++) ties += key[j] == thr;
+        unsigned every;
+        ties = block_scan<N, unsigned>(ties, reinterpret_cast<unsigned *>(s.wave), every) - ties;
+    }
+    const unsigned ties_before = ties;
+    u64 sum = 0;
+    unsigned kept = 0;
+#pragma unroll
+    for (int j = 0; j < K; j++) {
+        const bool tie = key[j] == thr;
+        const bool in = key[j] && key[j] >= thr && !(tie && ties >= quota) && !(low >> j & 1);
+        ties += tie;
+        kept += in;
+        sum += in ? mass[j] : 0;
+    }
+    unsigned kept_all;
+    u64 all;
     __syncthreads();
-    s_bin[tid] = upto;
-    s_bin[kThreads + tid] = ties_before;
+    block_scan<N, unsigned>(kept, s.x, kept_all);
+    const u64 upto = block_scan<N, u64>(sum, s.wave, all);
+    s.bins[tid] = upto;
+    s.ties[tid] = ties_before;
     __syncthreads();
     if (a.kept && tid == 0) a.kept[row] = (int)kept_all;
-    for (int j = tid; j < a.S; j += kThreads) {
-        const double u = a.u[row * a.u_ld + j];
-        const u64 r = u > 0.0 ? (u < 1.0 ? (u64)(u * 18446744073709551616.0) : ~0ull) : 0;
-        const u64 target = __umul64hi(r, mass_all);  // floor(u * mass), below the mass
-        int lo = 0, hi = kThreads - 1;  // the first part whose cumulated mass passes the target
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (s_bin[mid] > target) hi = mid;
-            else lo = mid + 1;
-        }
-        u64 sum = lo ? s_bin[lo - 1] : 0;
-        const long long b = (long long)lo * per;
+    for (int j = tid; j < a.S; j += N) {
+        const u64 target = target_of(a.u[row * a.u_ld + j], all);
+        int at = 0;  // the first thread whose cumulated mass passes the target
+#pragma unroll
+        for (int d = N / 2; d; d >>= 1) at += s.bins[at + d - 1] > target ? 0 : d;
+        u64 c = at ? s.bins[at - 1] : 0;
+        unsigned tie = s.ties[at];
         int found = -1;
-        walk(s_bin[kThreads + lo], (int)(b < n ? b : n), (int)(b + per < n ? b + per : n), [&](int i, u64 q) {
-            sum += q;
-            found = i;
-            return sum > target;
-        });
+#pragma unroll
+        for (int i = 0; i < K; i++) {
+            const unsigned k = s_key[at * K + i];
+            if (found >= 0 || !k || k < thr || (k == thr && tie++ >= quota)) continue;
+            const double w = wg.weight(k);
+            if (w < a.min_p) continue;
+            c += wg.mass(w);
+            if (c > target) found = at * K + i;
+        }
         index[j] = found;
     }
 }
 
+// ---- long rows: many workgroups per row ------------------------------------
+//
+// A row is cut into parts of 64 x 64 x f places, one workgroup each, and the
+// same steps run as one launch each; what a step finds is read by the next:
+//   extent  : each part's smallest and largest key and its count
+//   level 1 : bins over the row's key range: counts (top_k), masses (top_p)
+//   level 2, 3 of top_k, level 2, 3 of top_p : bins over the one bin the
+//             descent is in; every workgroup finds that bin itself from the
+//             bins of the launch before
+//   sums    : mass, places and ties above the threshold, per part and per
+//             group of 64 f places
+//   draw    : one wave per draw: part, group and place by three searches
+// Bins are shared by atomics on integers, so their order does not matter.
+
+constexpr int kPartThreads = 256;
+constexpr int kGroups = 64;         // groups of 64 f places per part
+constexpr int kMostParts = 1024;    // (a draw's workgroup holds their sums in LDS)
+
+enum BinArray { kC1, kM1, kC2, kK2, kC3, kK3, kM2, kM3, kBinArrays };  // K: masses of top_k's levels
+
+// where a descent is: its window of keys [lo, lo + (bins << shift))
+struct Descent {
+    unsigned lo, bins;
+    int shift;
+    int on;     // 0: this trim is off
+    int done;   // lo is the threshold's key, need what its ties bring
+    u64 need;   // still needed from the window
+    u64 above;  // mass of the keys above the window (top_k's descent)
+};
+
+struct RowState {
+    unsigned kmin, kmax, count;
+    unsigned thr;  // set by the sums, as quota
+    u64 quota;
+    Descent k, p;
+};
+
+// (member by member: a copy of the whole struct would go through scratch memory)
+__device__ __forceinline__ void copy(Descent &to, const Descent &from) {
+    to.lo = from.lo;
+    to.bins = from.bins;
+    to.shift = from.shift;
+    to.on = from.on;
+    to.done = from.done;
+    to.need = from.need;
+    to.above = from.above;
+}
+__device__ __forceinline__ void copy(RowState &to, const RowState &from) {
+    to.kmin = from.kmin;
+    to.kmax = from.kmax;
+    to.count = from.count;
+    to.thr = from.thr;
+    to.quota = from.quota;
+    copy(to.k, from.k);
+    copy(to.p, from.p);
+}
+
+struct Split {  // workspace of one row
+    int parts, f;
+    RowState *state;  // one per launch step
+    unsigned *extent;  // [parts][3]
+    u64 *bins;         // [kBinArrays][kBins]
+    u64 *group_mass;   // [parts][kGroups], places above the threshold
+    unsigned *group_ties;
+    u64 *part_mass;
+    unsigned *part_kept, *part_ties;
+};
+
+enum Step { kExtent, kLevel1, kK2Step, kK3Step, kP2Step, kP3Step, kSums, kSteps };
+
+__host__ __device__ inline int split_f(int V) {
+    const int per = kGroups * 64;
+    return (V + per * kMostParts - 1) / (per * kMostParts);
+}
+__host__ __device__ inline int split_parts(int V) { return (V + kGroups * 64 * split_f(V) - 1) / (kGroups * 64 * split_f(V)); }
+
+__host__ __device__ inline size_t split_row_bytes(int parts) {
+    size_t n = kSteps * sizeof(RowState) + (size_t)kBinArrays * kBins * 8 + (size_t)parts * (kGroups * 12 + 8 + 20);
+    return (n + 255) & ~(size_t)255;
+}
+
+__host__ __device__ inline Split split_of(void *ws, int V, int row) {
+    Split w;
+    w.f = split_f(V);
+    w.parts = split_parts(V);
+    char *p = static_cast<char *>(ws) + split_row_bytes(w.parts) * row;
+    w.bins = reinterpret_cast<u64 *>(p);
+    p += (size_t)kBinArrays * kBins * 8;
+    w.state = reinterpret_cast<RowState *>(p);
+    p += kSteps * sizeof(RowState);
+    w.group_mass = reinterpret_cast<u64 *>(p);
+    p += (size_t)w.parts * kGroups * 8;
+    w.part_mass = reinterpret_cast<u64 *>(p);
+    p += (size_t)w.parts * 8;
+    w.group_ties = reinterpret_cast<unsigned *>(p);
+    p += (size_t)w.parts * kGroups * 4;
+    w.part_kept = reinterpret_cast<unsigned *>(p);
+    p += (size_t)w.parts * 4;
+    w.part_ties = reinterpret_cast<unsigned *>(p);
+    p += (size_t)w.parts * 4;
+    w.extent = reinterpret_cast<unsigned *>(p);
+    return w;
+}
+
+struct SplitShared {
+    u64 bins[2 * kBins];
+    u64 wave[kPartThreads / 64];
+    u64 found_before, found_in;
+    int found_bin;
+};
+
+// The bin, from the top, where the running sum of `bin` reaches need (of the
+// whole sum when need is 0 and share >= 0: share of it): *at, and the sum
+// before it.  `other`'s sum before that bin too (NULL: not wanted).
+__device__ void find_bin(SplitShared &s, const u64 *bin, const u64 *other, u64 need, double share,
+                         int &at, u64 &need_out, u64 &before_out, u64 &other_before) {
+    constexpr int kPer = kBins / kPartThreads;
+    u64 v[kPer], o[kPer], sum = 0, osum = 0;
+    const int top = kBins - 1 - (int)threadIdx.x * kPer;  // this thread: bins top, top-1, ... (unused ones are 0)
+#pragma unroll
+    for (int j = 0; j < kPer; j++) {
+        v[j] = bin[top - j];
+        o[j] = other ? other[top - j] : 0;
+        sum += v[j];
+        osum += o[j];
+    }
+    u64 total, ototal = 0;
+    u64 before = block_scan<kPartThreads, u64>(sum, s.wave, total) - sum;
+    u64 obefore = other ? block_scan<kPartThreads, u64>(osum, s.wave, ototal) - osum : 0;
+    if (share >= 0.0) {
+        need = need_of(share, total);
+    }
+    if (before < need && need <= before + sum) {
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+            if (before < need && need <= before + v[j]) {
+                s.found_bin = top - j;
+                s.found_before = before;
+                s.found_in = obefore;
+            }
+            before += v[j];
+            obefore += o[j];
+        }
+    }
+    __syncthreads();
+    at = s.found_bin;
+    before_out = s.found_before;
+    other_before = s.found_in;
+    need_out = need;
+    __syncthreads();
+}
+
+// one level down, into bin `at`
+__device__ __forceinline__ void into_bin(Descent &d, int at, u64 before, u64 above) {
+    d.lo += (unsigned)at << d.shift;
+    d.need -= before;
+    d.above += above;
+    d.done = d.shift == 0;
+    d.bins = d.shift > kBinBits ? kBins : 1u << d.shift;
+    d.shift = d.shift > kBinBits ? d.shift - kBinBits : 0;
+}
+
+// A thread's places of a part: wave w has the groups w, w + 4, ... (64 f places
+// each), one place of 64 neighbouring ones per lane.  All loads of a round are
+// issued before the first is used.
+constexpr int kPartKeys = kGroups * 64 / kPartThreads;
+struct PartKeys {
+    const SampleArgs &a;
+    long long base;
+    int i0, n, f;
+    unsigned key[kPartKeys];
+    __device__ __forceinline__ int place(int j, int jj) const {
+        return i0 + ((j * (kPartThreads / 64) + ((int)threadIdx.x >> 6)) * f + jj) * 64 + ((int)threadIdx.x & 63);
+    }
+    __device__ __forceinline__ void load(int jj) {
+        load_keys<kPartKeys>(a, base, n, key, [&](int j) { return place(j, jj); });
+    }
+};
+
+// The part's keys inside a descent's window -> the row's bins, through LDS:
+// counts and / or masses.
+__device__ __forceinline__ void fill_bins(SplitShared &s, PartKeys &keys, int f, const Weigh &wg, unsigned lo,
+                                          int shift, unsigned bins, u64 *counts, u64 *masses) {
+    u64 *s_c = s.bins, *s_m = s.bins + kBins;
+    for (int i = threadIdx.x; i < (int)bins; i += kPartThreads) s_c[i] = s_m[i] = 0;
+    __syncthreads();
+    for (int jj = 0; jj < f; jj++) {
+        if (jj) keys.load(jj);
+#pragma unroll
+        for (int j = 0; j < kPartKeys; j++) {
+            const unsigned k = keys.key[j];
+            if (!k || k < lo || ((k - lo) >> shift) >= bins) continue;
+            const unsigned b = (k - lo) >> shift;
+            if (counts) atomicAdd(&s_c[b], 1ull);
+            if (masses) atomicAdd(&s_m[b], wg.mass(wg.weight(k)));
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < (int)bins; i += kPartThreads) {
+        if (counts && s_c[i]) atomicAdd(&counts[i], s_c[i]);
+        if (masses && s_m[i]) atomicAdd(&masses[i], s_m[i]);
+    }
+}
+
+template <int STEP>
+__global__ __launch_bounds__(kPartThreads) void sample_step_kernel(SampleArgs a) {
+    __shared__ SplitShared s;
+    const int all = split_parts(a.V);
+    const int row = blockIdx.x / all, part = blockIdx.x - row * all, tid = threadIdx.x;
+    const Split w = split_of(a.ws, a.V, row);
+    int n = a.lens ? a.lens[row] : a.V;
+    n = n < 0 ? 0 : n > a.V ? a.V : n;
+    const int size = kGroups * 64 * w.f;
+    const long long base = row * a.ld;
+    const bool use_k = a.top_k > 0 || a.temperature == 0.0, use_p = a.top_p < 1.0;  // (the launches that run)
+    PartKeys keys{a, base, part * size, n, w.f, {}};
+    keys.load(0);
+
+    if constexpr (STEP == kExtent) {
+        const int words = kBinArrays * kBins;
+        if (use_k || use_p)
+            for (int i = part * kPartThreads + tid; i < words; i += w.parts * kPartThreads) w.bins[i] = 0;
+        unsigned lo = 0xffffffffu, hi = 0, c = 0;
+        for (int jj = 0; jj < w.f; jj++) {
+            if (jj) keys.load(jj);
+#pragma unroll
+            for (int j = 0; j < kPartKeys; j++) {
+                const unsigned k = keys.key[j];
+                if (!k) continue;
+                lo = k < lo ? k : lo;
+                hi = k > hi ? k : hi;
+                c++;
+            }
+        }
+        block_extent<kPartThreads>(lo, hi, c, reinterpret_cast<unsigned *>(s.bins));
+        if (tid == 0) {
+            w.extent[part * 3] = lo;
+            w.extent[part * 3 + 1] = hi;
+            w.extent[part * 3 + 2] = c;
+        }
+        return;
+    }
+
+    RowState st;
+    const int before_sums = use_p ? kP3Step : use_k ? kK3Step : kLevel1;
+    if (STEP == kLevel1 || (STEP == kSums && before_sums == kLevel1)) {  // no trim: the sums are the second step
+        unsigned lo = 0xffffffffu, hi = 0, c = 0;
+        for (int k = tid; k < w.parts; k += kPartThreads) {
+            const unsigned l = w.extent[k * 3], h = w.extent[k * 3 + 1];
+            lo = l < lo ? l : lo;
+            hi = h > hi ? h : hi;
+            c += w.extent[k * 3 + 2];
+        }
+        block_extent<kPartThreads>(lo, hi, c, reinterpret_cast<unsigned *>(s.bins));
+        __syncthreads();
+        st.thr = 0;
+        st.quota = 0;
+        st.k.done = st.p.done = 0;
+        st.k.above = st.p.above = st.p.need = 0;
+        st.kmin = lo;
+        st.kmax = hi;
+        st.count = c;
+        const int top_k = a.temperature == 0.0 ? 1 : a.top_k;
+        st.k.on = use_k && (unsigned)top_k < c;
+        st.k.need = top_k;
+        st.p.on = use_p && c > 0;
+        int shift = 0;
+        while (c && ((hi - lo) >> shift) >= kBins) shift++;
+        st.k.lo = st.p.lo = lo;
+        st.k.bins = st.p.bins = kBins;
+        st.k.shift = st.p.shift = shift;
+    } else {
+        constexpr int kBefore = STEP == kK2Step ? kLevel1 : STEP == kK3Step ? kK2Step : STEP == kP3Step ? kP2Step : -1;
+        copy(st, w.state[STEP == kP2Step ? (use_k ? kK3Step : kLevel1) : STEP == kSums ? before_sums : kBefore]);
+    }
+    const Weigh wg{score_of(st.kmax), 1.0 / a.temperature, ldexp(1.0, a.shift)};
+    u64 *C1 = w.bins + kC1 * kBins, *M1 = w.bins + kM1 * kBins, *C2 = w.bins + kC2 * kBins, *K2 = w.bins + kK2 * kBins;
+    u64 *C3 = w.bins + kC3 * kBins, *K3 = w.bins + kK3 * kBins, *M2 = w.bins + kM2 * kBins, *M3 = w.bins + kM3 * kBins;
+    auto down = [&](Descent &d, const u64 *bin, const u64 *mass, double share) {
+        int at;
+        u64 need, before, above;
+        find_bin(s, bin, mass, d.need, share, at, need, before, above);
+        d.need = need;
+        into_bin(d, at, before, above);
+    };
+    u64 *counts = nullptr, *masses = nullptr;  // of the window of st.k (of st.p: P2 and P3)
+    if (STEP == kLevel1) {
+        counts = st.k.on ? C1 : nullptr;
+        masses = st.p.on ? M1 : nullptr;
+    }
+    if (STEP == kK2Step && st.k.on) {
+        down(st.k, C1, st.p.on ? M1 : nullptr, -1.0);
+        counts = C2;
+        masses = st.p.on ? K2 : nullptr;
+    }
+    if (STEP == kK3Step && st.k.on && !st.k.done) {
+        down(st.k, C2, st.p.on ? K2 : nullptr, -1.0);
+        counts = C3;
+        masses = st.p.on ? K3 : nullptr;
+    }
+    if ((STEP == kP2Step || (STEP == kSums && !use_p)) && st.k.on && !st.k.done)
+        down(st.k, C3, st.p.on ? K3 : nullptr, -1.0);
+    if (STEP == kP2Step && st.p.on) {
+        double share = a.top_p;
+        if (st.k.on) {  // of what top_k keeps: every key above its threshold, and its share of the ties
+            const u64 total = st.k.above + st.k.need * wg.mass(wg.weight(st.k.lo));
+            st.p.need = need_of(a.top_p, total);
+            share = -1.0;
+        }
+        down(st.p, M1, nullptr, share);
+        masses = M2;
+    }
+    if (STEP == kP3Step && st.p.on && !st.p.done) {
+        down(st.p, M2, nullptr, -1.0);
+        masses = M3;
+    }
+    if (STEP == kSums && st.p.on && !st.p.done) down(st.p, M3, nullptr, -1.0);
+    if constexpr (STEP != kSums) {
+        if (part == 0 && tid == 0) copy(w.state[STEP], st);
+        constexpr bool kOfP = STEP == kP2Step || STEP == kP3Step;
+        if ((counts || masses) && !(kOfP ? st.p.done : st.k.done))
+            fill_bins(s, keys, w.f, wg, kOfP ? st.p.lo : st.k.lo, kOfP ? st.p.shift : st.k.shift,
+                      kOfP ? st.p.bins : st.k.bins, counts, masses);
+    } else {
+        st.thr = 0;
+        st.quota = ~0ull;
+        u64 each = 0;
+        if (st.p.on || st.k.on) {
+            st.thr = st.p.on ? st.p.lo : st.k.lo;
+            const double wt = wg.weight(st.thr);
+            each = wg.mass(wt);
+            st.quota = st.p.on ? (st.p.need + each - 1) / (each ? each : 1) : st.k.need;
+            if (wt < a.min_p) st.quota = 0;
+        }
+        if (part == 0 && tid == 0) copy(w.state[STEP], st);
+        const int lane = tid & 63, wave = tid >> 6;
+        u64 mass[kPartKeys], part_mass = 0;
+        unsigned ties[kPartKeys], part_kept = 0, part_ties = 0;
+#pragma unroll
+        for (int j = 0; j < kPartKeys; j++) mass[j] = ties[j] = 0;
+        for (int jj = 0; jj < w.f; jj++) {
+            if (jj) keys.load(jj);
+#pragma unroll
+            for (int j = 0; j < kPartKeys; j++) {
+                const unsigned k = keys.key[j];
+                ties[j] += __popcll(__ballot(k && k == st.thr));
+                const double wt = wg.weight(k);
+                const bool in = k > st.thr && wt >= a.min_p;
+                mass[j] += in ? wg.mass(wt) : 0;
+                part_kept += __popcll(__ballot(in));
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kPartKeys; j++) {
+            const u64 m = wave_sum(mass[j]);
+            if (lane == 0) {
+                w.group_mass[part * kGroups + j * (kPartThreads / 64) + wave] = m;
+                w.group_ties[part * kGroups + j * (kPartThreads / 64) + wave] = ties[j];
+            }
+            part_mass += m;
+            part_ties += ties[j];
+        }
+        unsigned *x = reinterpret_cast<unsigned *>(s.bins);
+        if (lane == 0) {
+            s.wave[wave] = part_mass;
+            x[wave] = part_kept;
+            x[4 + wave] = part_ties;
+        }
+        __syncthreads();
+        if (tid == 0) {
+            w.part_mass[part] = s.wave[0] + s.wave[1] + s.wave[2] + s.wave[3];
+            w.part_kept[part] = x[0] + x[1] + x[2] + x[3];
+            w.part_ties[part] = x[4] + x[5] + x[6] + x[7];
+        }
+    }
+}
+
+__global__ __launch_bounds__(kPartThreads) void sample_draw_kernel(SampleArgs a, int chunks, int draws) {
+    __shared__ u64 s_mass[kMostParts];       // cumulated kept mass, by part
+    __shared__ unsigned s_ties[kMostParts];  // ties before each part
+    __shared__ u64 s_wave[kPartThreads / 64];
+    const int row = blockIdx.x / chunks, chunk = blockIdx.x - row * chunks, tid = threadIdx.x;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Split w = split_of(a.ws, a.V, row);
+    const RowState &st = w.state[kSums];
+    const unsigned thr = st.thr, count = st.count;
+    const u64 quota = st.quota;
+    const Weigh wg{score_of(st.kmax), 1.0 / a.temperature, ldexp(1.0, a.shift)};
+    const u64 each = thr ? wg.mass(wg.weight(thr)) : 0;
+    int n = a.lens ? a.lens[row] : a.V;
+    n = n < 0 ? 0 : n > a.V ? a.V : n;
+    auto kept_ties = [&](u64 before, u64 ties) {
+        const u64 left = before < quota ? quota - before : 0;
+        return left < ties ? left : ties;
+    };
+    u64 total = 0;
+    {
+        constexpr int kPer = kMostParts / kPartThreads;  // parts tid*kPer ..
+        u64 ties[kPer], kept = 0, all_ties = 0, sum = 0;
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+            const int p = tid * kPer + j;
+            ties[j] = p < w.parts ? w.part_ties[p] : 0;
+            kept += p < w.parts ? w.part_kept[p] : 0;
+            all_ties += ties[j];
+        }
+        u64 every, every_kept;
+        u64 before = block_scan<kPartThreads, u64>(all_ties, s_wave, every) - all_ties;
+        block_scan<kPartThreads, u64>(kept, s_wave, every_kept);
+        u64 cum[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+            const int p = tid * kPer + j;
+            s_ties[p] = (unsigned)before;
+            sum += (p < w.parts ? w.part_mass[p] : 0) + kept_ties(before, ties[j]) * each;
+            cum[j] = sum;
+            before += ties[j];
+        }
+        const u64 upto = block_scan<kPartThreads, u64>(sum, s_wave, total) - sum;
+#pragma unroll
+        for (int j = 0; j < kPer; j++) s_mass[tid * kPer + j] = upto + cum[j];
+        if (a.kept && chunk == 0 && tid == 0)
+            a.kept[row] = (int)(every_kept + kept_ties(0, every));
+    }
+    __syncthreads();
+    const long long base = row * a.ld;
+    const int size = kGroups * 64 * w.f;
+    for (int d = 0; d < draws; d++) {
+        const long long j = ((long long)chunk * draws + d) * (kPartThreads / 64) + wave;
+        if (j >= a.S) break;
+        int found = -1;
+        if (count) {
+            const double u = a.u[row * a.u_ld + j];
+            const u64 target = target_of(u, total);
+            // part: 16 of them per lane, then one of those
+            const int l16 = __ffsll((long long)__ballot(s_mass[lane * 16 + 15] > target)) - 1;
+            const int part = l16 * 16 + __ffsll((long long)__ballot(lane < 16 && s_mass[l16 * 16 + (lane & 15)] > target)) - 1;
+            u64 sum = part ? s_mass[part - 1] : 0;
+            // group
+            const u64 ties = w.group_ties[part * kGroups + lane];
+            u64 before = s_ties[part] + wave_scan(ties) - ties;
+            const u64 upto = sum + wave_scan(w.group_mass[part * kGroups + lane] + kept_ties(before, ties) * each);
+            const int g = __builtin_amdgcn_readfirstlane(__ffsll((long long)__ballot(upto > target)) - 1);
+            if (g > 0) sum = lane_of(upto, g - 1);
+            before = lane_of(before, g);
+            // place
+            for (int f = 0; f < w.f && found < 0; f++) {
+                const int i = part * size + (g * w.f + f) * 64 + lane;
+                unsigned key[1];
+                load_keys<1>(a, base, n, key, [&](int) { return i; });
+                const unsigned k = key[0];
+                const bool tie = k && k == thr;
+                const u64 tied = __ballot(tie);
+                u64 q = 0;
+                if (k > thr || (tie && before + __popcll(tied & ((1ull << lane) - 1)) < quota)) {
+                    const double wt = wg.weight(k);
+                    if (wt >= a.min_p) q = wg.mass(wt);
+                }
+                before += __popcll(tied);
+                const u64 c = sum + wave_scan(q);
+                const u64 hit = __ballot(c > target);
+                if (hit) found = part * size + (g * w.f + f) * 64 + __ffsll((long long)hit) - 1;
+                sum = lane_of(c, 63);
+            }
+        }
+        if (lane == 0) a.index[row * a.index_ld + j] = found;
+    }
+}
+
+template <int STEP>
+void launch_step(const SampleArgs &a, hipStream_t s) {
+    hipLaunchKernelGGL((sample_step_kernel<STEP>), dim3((unsigned)a.B * split_parts(a.V)), dim3(kPartThreads), 0, s, a);
+}
+
 }  // namespace
 
-SamplePlan sample_plan(const SampleArgs &) { return SamplePlan{0}; }
+// Rows of up to kRowScores scores have one workgroup, whose registers hold
+// them; longer ones are cut over many.
+constexpr int kRowScores = 16384;
+
+SamplePlan sample_plan(const SampleArgs &a) {
+    SamplePlan p{0};
+    if (a.V > kRowScores) p.ws_bytes = split_row_bytes(split_parts(a.V)) * a.B;
+    return p;
+}
+
+template <int N, int K>
+static void launch_row(const SampleArgs &a, hipStream_t s) {
+    hipLaunchKernelGGL((sample_row_kernel<N, K>), dim3((unsigned)a.B), dim3(N), 0, s, a);
+}
 
 void launch_sample(const SampleArgs &a, hipStream_t s) {
     if (a.B == 0) return;
-    hipLaunchKernelGGL(sample_row_kernel, dim3((unsigned)a.B), dim3(kThreads), 0, s, a);
+    if (a.V <= kRowScores) {
+        if (a.V <= 256) launch_row<256, 1>(a, s);
+        else if (a.V <= 1024) launch_row<256, 4>(a, s);
+        else if (a.V <= 4096) launch_row<1024, 4>(a, s);
+        else if (a.V <= 8192) launch_row<1024, 8>(a, s);
+        else launch_row<1024, 16>(a, s);
+        return;
+    }
+    const bool use_k = a.top_k > 0 || a.temperature == 0.0, use_p = a.top_p < 1.0;
+    launch_step<kExtent>(a, s);
+    if (use_k || use_p) launch_step<kLevel1>(a, s);
+    if (use_k) {
+        launch_step<kK2Step>(a, s);
+        launch_step<kK3Step>(a, s);
+    }
+    if (use_p) {
+        launch_step<kP2Step>(a, s);
+        launch_step<kP3Step>(a, s);
+    }
+    launch_step<kSums>(a, s);
+    // draws per wave: one until the chip's 8192 waves are taken, 16 at most
+    const long long waves = (long long)a.B * a.S;
+    const int draws = waves <= 8192 ? 1 : waves >= 16 * 8192 ? 16 : (int)((waves + 8191) / 8192);
+    const int per = draws * kPartThreads / 64, chunks = a.S > per ? (a.S + per - 1) / per : 1;
+    hipLaunchKernelGGL(sample_draw_kernel, dim3((unsigned)((long long)a.B * chunks)), dim3(kPartThreads), 0, s, a,
+                       chunks, draws);
 }
 
 }  // namespace sc

@@ -128,12 +128,17 @@ sc::LrArgs lr_args(const sc_samples *x, const sc_weak_bank *k) {
     a.b = k->b;
     a.alpha = 1.0f;
     a.beta = 1.0f;
+    if (a.n == 0) {  // every row is absent: what is read in their place lies in the weights
+        a.x = a.w;
+        a.ld = 0;
+        a.n_patches = 0;
+    }
     return a;
 }
 
 void lr_pointers(const sc_trainer *t, const sc::LrArgs &a) {
     if (a.M == 0 || a.H == 0) return;
-    if (a.R > 0 && a.n > 0) {
+    if (a.R > 0) {
         need_ptr(t, a.x, "samples");
         need_aligned(a.x, elem_size(a.dtype), "samples");
     }

@@ -174,6 +174,37 @@ def test_large_pool(tr):
         _check(tr, scores, u, **trim)
 
 
+def test_larger_pools_and_many_rows(tr):
+    """Past 2^22 scores a part's groups grow; past 128 rows each row has one
+    workgroup again, however long it is."""
+    scores, u = _inputs(1, 5000011, 300, 14, "bf16")
+    for trim in (dict(top_p=0.9), dict(top_k=3000000, top_p=0.9, min_p=1e-4), dict(top_k=2)):
+        _check(tr, scores, u, **trim)
+    scores, u = _inputs(150, 9001, 5, 15)
+    lens = torch.randint(0, 9002, (150,), generator=torch.Generator().manual_seed(1), dtype=torch.int32)
+    _check(tr, scores, u, lens=lens, top_k=2000, top_p=0.9)
+    _check(tr, scores[:128].contiguous(), u[:128].contiguous(), lens=lens[:128], top_k=2000, top_p=0.9)
+
+
+@pytest.mark.parametrize("trim", TRIMS, ids=str)
+def test_masked_places_in_long_rows(tr, trim):
+    inf, low = float("inf"), torch.finfo(torch.float32).min
+    v = 40001
+    g = torch.Generator().manual_seed(7)
+    scores = torch.randn(8, v, generator=g)
+    scores[0] = -inf
+    scores[1] = float("nan")
+    scores[2] = -inf
+    scores[2, 31234] = -3.0
+    scores[3, :30000] = -inf
+    scores[4, ::3] = float("nan")
+    scores[5] = low
+    scores[6, 5:] = low
+    scores[7, 100] = scores[7, 39000] = inf
+    u = torch.rand(8, 70, generator=g, dtype=torch.float64)
+    _check(tr, scores, u, **trim)
+
+
 def test_strides(tr):
     """Rows of wider buffers, and offsets past 32 bits."""
     scores, u = _inputs(3, 700, 11, 10)
