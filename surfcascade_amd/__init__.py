@@ -104,6 +104,25 @@ class ScanParams(ctypes.Structure):
         return cls(**d)
 
 
+class _Samples(ctypes.Structure):
+    """sc_samples"""
+    _fields_ = [("data", ctypes.c_void_p), ("dtype", ctypes.c_int32), ("n_patches", ctypes.c_int32),
+                ("n", ctypes.c_int64), ("ld", ctypes.c_int64), ("rows", ctypes.c_void_p),
+                ("n_rows", ctypes.c_int64)]
+
+
+class _WeakBank(ctypes.Structure):
+    """sc_weak_bank"""
+    _fields_ = [("m", ctypes.c_int32), ("h", ctypes.c_int32), ("patch", ctypes.c_void_p),
+                ("w", ctypes.c_void_p), ("b", ctypes.c_void_p)]
+
+
+class _SampleParams(ctypes.Structure):
+    """sc_sample_params"""
+    _fields_ = [("temperature", ctypes.c_double), ("top_k", ctypes.c_int32),
+                ("top_p", ctypes.c_double), ("min_p", ctypes.c_double)]
+
+
 def library_path():
     return os.environ.get("SURFCASCADE_LIB", os.path.join(HERE, "lib", "libsurfcascade.so"))
 
@@ -175,7 +194,7 @@ def load_library():
     L.sc_fast_nms.argtypes = [vp, i32, ctypes.c_double, vp, i32, P(i32)]
     L.sc_decode_jpeg_gray.argtypes = [vp, sz, vp, sz, P(i32), P(i32)]
     L.sc_imread_gray.argtypes = [ctypes.c_char_p, vp, sz, P(i32), P(i32)]
-    f32 = ctypes.c_float
+    f32, xs, ks = ctypes.c_float, P(_Samples), P(_WeakBank)
     L.sc_trainer_create.argtypes = [i32, P(vp)]
     L.sc_trainer_destroy.argtypes = [vp]
     L.sc_trainer_destroy.restype = None
@@ -185,14 +204,14 @@ def load_library():
     L.sc_stream_wait_trainer.argtypes = [vp, vp]
     L.sc_trainer_set_stream.argtypes = [vp, vp, i32]
     L.sc_trainer_synchronize.argtypes = [vp]
-    L.sc_lr_response.argtypes = [vp, vp, vp, i32, f32, vp, i32, i64, f32, vp, i64]
-    L.sc_lr_workspace.argtypes = [vp, vp, P(sz)]
-    L.sc_lr_response_grad.argtypes = [vp, vp, vp, i32, f32, vp, i64, vp, vp, i32, f32, vp, i64, vp, sz]
-    L.sc_lr_loss.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, sz]
-    L.sc_sample_params_default.argtypes = [vp]
+    L.sc_lr_response.argtypes = [vp, xs, ks, i32, f32, vp, i32, i64, f32, vp, i64]
+    L.sc_lr_workspace.argtypes = [xs, ks, P(sz)]
+    L.sc_lr_response_grad.argtypes = [vp, xs, ks, i32, f32, vp, i64, vp, vp, i32, f32, vp, i64, vp, sz]
+    L.sc_lr_loss.argtypes = [vp, xs, ks, vp, vp, vp, vp, vp, vp, sz]
+    L.sc_sample_params_default.argtypes = [P(_SampleParams)]
     L.sc_sample_params_default.restype = None
     L.sc_sample_workspace.argtypes = [i32, i32, i32, P(sz)]
-    L.sc_sample.argtypes = [vp, vp, i32, i32, i32, i64, vp, vp, vp, i32, i64, vp, i64, vp, vp, sz]
+    L.sc_sample.argtypes = [vp, vp, i32, i32, i32, i64, vp, P(_SampleParams), vp, i32, i64, vp, i64, vp, vp, sz]
     L.sc_selftest_rn.argtypes = [i32, i32, ctypes.c_uint32, ctypes.c_uint32, P(ctypes.c_uint64)]
     L.sc_normalize_operand_range.argtypes = [i32, i32, P(ctypes.c_double), P(ctypes.c_double)]
     L.sc_normalize_operand_range.restype = None

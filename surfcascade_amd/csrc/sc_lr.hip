@@ -20,6 +20,8 @@
 // dot, so the sigmoid runs once per result on full lanes.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "sc_train.hpp"
 #include "surfcascade.h"
 
@@ -28,6 +30,7 @@ namespace sc {
 namespace {
 
 constexpr int kWaves = 4;  // waves per workgroup
+constexpr int kWideWaves = 4;   // ... of the wide form
 constexpr int kNarrowSets = 4;  // parameter sets per learner up to which the narrow form runs
 
 struct F32 {
@@ -132,7 +135,9 @@ __device__ __forceinline__ float sum_lanes(float v) {
     return v;
 }
 
-__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+// (the hardware's reciprocal, good to one unit in the last place: the IEEE
+// division is ten instructions)
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
 
 enum Mode { kResponse = 0, kGrad = 1, kLoss = 2 };
 
@@ -159,7 +164,7 @@ __device__ __forceinline__ float log1p_over(float e) {
 // NaN e, and stays one.
 template <int MODE>
 __device__ __forceinline__ float grad_of(int act, float z, float pos, float neg, float &loss) {
-    const float e = __expf(-fabsf(z)), d = __fdividef(1.0f, 1.0f + e);
+    const float e = __expf(-fabsf(z)), d = __builtin_amdgcn_rcpf(1.0f + e);
     if constexpr (MODE == kLoss) {
         const bool up = z >= 0.0f;
         const float near = up ? pos : -neg, far = up ? -neg : pos;
@@ -272,9 +277,15 @@ __global__ __launch_bounds__(64 * kWaves) void lr_kernel(LrArgs a) {
 #pragma unroll
             for (int h = 0; h < H; h++) {
                 float g = 0.0f;
+                if constexpr (MODE == kGrad) {
+                    if (learner && rq < r1 && h0 + h < a.H) {
+                        const long long col = (long long)m * a.H + h0 + h;
+                        const float dy = a.dy[(long long)rq * a.dy_ld + col];
+                        pos = a.alpha * dy;
+                        if (a.res_kind == SC_RES_FULL) a.dres[(long long)rq * a.dres_ld + col] = a.beta * dy;
+                    }
+                }
                 if (idx >= 0 && present && h0 + h < a.H) {
-                    if constexpr (MODE == kGrad)
-                        pos = a.alpha * a.dy[(long long)rq * a.dy_ld + (long long)m * a.H + h0 + h];
                     g = grad_of<MODE>(a.act, z[h], pos, neg, sum_l[h]);
                 }
                 sum_g[h] += g;
@@ -321,38 +332,35 @@ __global__ __launch_bounds__(64 * kWaves) void lr_kernel(LrArgs a) {
 }
 
 // Wide form, for many parameter sets: a wave owns one learner and 16 of its
-// sets and multiplies 16 rows at a time on the matrix cores (16x16x4, f32 in
-// and out, so nothing is rounded that the narrow form does not round).
+// sets and multiplies 16 rows at a time on the matrix cores.  Neighbouring
+// waves have the sets of a learner, then the next learner, whose descriptors
+// lie in the same lines.
 //   z = X W^T : lane (i = lane % 16, q = lane / 16) holds 8 values of row i's
-//               descriptor, the same 8 places of set i's weights; any order of
-//               the places will do, so each lane keeps what one 16-B load
-//               brings.  Result: set i, rows 4q .. 4q+3.
-//   dW = G^T X: that result is already the operand layout of the second
+//               descriptor and the same 8 places of set i's weights; any order
+//               of the places will do, so each lane keeps what one 16-B load
+//               brings.
+//   dW = G^T X: z's result is already the operand layout of the second
 //               product; X is read again with lane i = descriptor place (its
 //               lines are in the vector L1 from the first read).
 template <class T>
-struct WideRow;  // the 8 values of a lane's row and which places they are
+struct WideRow {  // the 8 values of a lane's row: places 8q..8q+7
+    uint4_v a;
+    __device__ __forceinline__ void load(const char *p) { a = load16<T>(p); }
+    __device__ __forceinline__ void values(float *f) const { unpack<T>(a, f); }
+    static __device__ __forceinline__ int place(int q, int k) { return q * 8 + k; }
+};
 template <>
 struct WideRow<F32> {  // places 4q..4q+3 and 16+4q..: each load covers half a line of 16 rows
     uint4_v a, b;
-    __device__ __forceinline__ void load(const char *p, int q) {
-        a = load16<F32>(p + q * 16);
-        b = load16<F32>(p + 64 + q * 16);
+    __device__ __forceinline__ void load(const char *p) {
+        a = load16<F32>(p);
+        b = load16<F32>(p + 64);
     }
-    __device__ __forceinline__ void clear() { a = b = uint4_v{0, 0, 0, 0}; }
     __device__ __forceinline__ void values(float *f) const {
         unpack<F32>(a, f);
         unpack<F32>(b, f + 4);
     }
     static __device__ __forceinline__ int place(int q, int k) { return (k & 4) * 4 + q * 4 + (k & 3); }
-};
-template <class T>
-struct WideRow {  // places 8q..8q+7
-    uint4_v a;
-    __device__ __forceinline__ void load(const char *p, int q) { a = load16<T>(p + q * 16); }
-    __device__ __forceinline__ void clear() { a = uint4_v{0, 0, 0, 0}; }
-    __device__ __forceinline__ void values(float *f) const { unpack<T>(a, f); }
-    static __device__ __forceinline__ int place(int q, int k) { return q * 8 + k; }
 };
 
 template <class T>
@@ -363,170 +371,421 @@ __device__ __forceinline__ float load_one(const char *p) {
 }
 
 typedef float float4_v __attribute__((ext_vector_type(4)));
+typedef float float4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 
-template <class T, int MODE>
-__global__ __launch_bounds__(64 * kWaves) void lr_wide_kernel(LrArgs a) {
+// what a wave of the wide form works on
+struct WideUnit {
+    int m, h0, r0, r1;  // learner, first set, rows
+    bool present;       // its patch exists
+    const char *x;      // that patch of sample 0 (patch 0 in an absent one's place)
+    long long step;     // bytes from sample to sample
+    // samples in order, 16 of them within 2^31 bytes: one base per tile and
+    // per-lane offsets that stay the same
+    bool in_order;
+};
+
+template <class T>
+__device__ __forceinline__ bool wide_unit(const LrArgs &a, int wave, WideUnit &u) {
+    const int sets = (a.H + 15) / 16, unit = blockIdx.x * (blockDim.x >> 6) + wave;
+    u.m = unit / sets;
+    u.h0 = (unit - u.m * sets) * 16;
+    if (u.m >= a.M) return false;
+    const int p = a.patch ? a.patch[u.m] : u.m;
+    u.present = (unsigned)p < (unsigned)a.n_patches;
+    u.x = static_cast<const char *>(a.x) + (long long)(u.present ? p : 0) * kDesc * T::kSize;
+    u.step = a.ld * T::kSize;
+    u.in_order = !a.rows && u.step < (1 << 26);
+    const long long lo = (long long)blockIdx.y * a.rows_per_wave;
+    u.r0 = (int)(lo < a.R ? lo : a.R);
+    u.r1 = (int)(lo + a.rows_per_wave < a.R ? lo + a.rows_per_wave : a.R);
+    return true;
+}
+
+// Responses: z^T = W X^T, so that lane i has row i and four neighbouring sets
+// (one 16-B store).
+template <class T>
+__global__ __launch_bounds__(64 * kWideWaves) void lr_wide_response_kernel(LrArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, q = lane >> 4;
-    const int sets = (a.H + 15) / 16;
-    // neighbouring waves: the sets of a learner, then the next learner (whose
-    // descriptors lie in the same lines)
-    const int unit = blockIdx.x * kWaves + wave;
-    const int m = unit / sets, h = (unit - m * sets) * 16 + i;
-    if (m >= a.M) return;
-    int p = a.patch ? a.patch[m] : m;
-    const bool present = (unsigned)p < (unsigned)a.n_patches;
-    if (!present) p = 0;
-    const bool on = h < a.H;
-    const long long mh = (long long)m * a.H + h;
+    WideUnit u;
+    if (!wide_unit<T>(a, wave, u)) return;
     float w[8];
+    float4_v bias = {0, 0, 0, 0};
+    const long long first = (long long)u.m * a.H + u.h0;  // column of the first set
+    const int left = a.H - u.h0 - 4 * q;                  // sets from this lane's first on
 #pragma unroll
-    for (int k = 0; k < 8; k++) w[k] = on ? a.w[mh * kDesc + WideRow<T>::place(q, k)] : 0.0f;
-    const float bias = on && a.b ? a.b[mh] : 0.0f;
-    const long long r_lo = (long long)blockIdx.y * a.rows_per_wave;
-    const int r0 = (int)(r_lo < a.R ? r_lo : a.R);
-    const int r1 = (int)(r_lo + a.rows_per_wave < a.R ? r_lo + a.rows_per_wave : a.R);
-    const char *x = static_cast<const char *>(a.x) + (long long)p * kDesc * T::kSize;
-    const long long step = a.ld * T::kSize;
-    float4_v acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-    float sum_g = 0.0f, sum_l = 0.0f;
-    // Two stages ahead of the products: the rows' numbers (and weights), then
-    // their descriptors, so a wave always has one tile of loads in flight.
-    // Absent rows load sample 0 instead and are cleared where they are used:
-    // a tile without any (every tile but the last, mostly) has no branches.
-    struct Meta {
+    for (int k = 0; k < 8; k++)
+        w[k] = u.h0 + i < a.H ? a.w[(first + i) * kDesc + WideRow<T>::place(q, k)] : 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+        if (a.b && k < left) bias[k] = a.b[first + 4 * q + k];
+    struct Tile {
+        WideRow<T> x;
+        float4_v res;
         int idx;
-        float pos, neg;
     };
-    auto load_meta = [&](int r) {
-        Meta u{-1, 0.0f, 0.0f};
-        if (r + i < r1) {
-            u.idx = a.rows ? a.rows[r + i] : r + i;
-            if ((unsigned)u.idx >= (unsigned)a.n) u.idx = -1;
+    auto row_of = [&](int r) {  // the sample row r + i reads; -1: absent, or past the end
+        int idx = -1;
+        if (r + i < u.r1) {
+            idx = a.rows ? a.rows[r + i] : r + i;
+            if ((unsigned)idx >= (unsigned)a.n) idx = -1;
         }
-        if constexpr (MODE == kLoss) {
-            if (u.idx >= 0) {
-                const float c = a.weight ? a.weight[u.idx] : 1.0f, t = a.target[u.idx];
-                u.pos = c * (1.0f - t);
-                u.neg = c * t;
-                if (c == 0.0f) u.idx = -1;  // a row without weight is not looked at, whatever it holds
+        return idx;
+    };
+    const unsigned lane_off = (unsigned)(i * u.step) + q * 16;
+    auto load = [&](int r, int idx) {
+        Tile t;
+        t.idx = idx;
+        if (u.in_order && r + 16 <= u.r1) t.x.load(u.x + r * u.step + lane_off);
+        else t.x.load(u.x + (idx < 0 ? 0 : idx) * u.step + q * 16);
+        t.res = float4_v{0, 0, 0, 0};
+        const int row = r + i;
+        if (row < u.r1) {
+            if (a.res_kind == SC_RES_ROW) {
+                const float v = a.res[(long long)row * a.res_ld];
+                t.res = float4_v{v, v, v, v};
+            } else if (a.res_kind == SC_RES_FULL) {
+                const float *p = a.res + (long long)row * a.res_ld + first + 4 * q;
+                if (left >= 4) {
+                    t.res = *reinterpret_cast<const float4_a4 *>(p);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 3; k++)
+                        if (k < left) t.res[k] = p[k];
+                }
             }
         }
-        return u;
+        return t;
     };
-    struct Tile {
-        Meta u;
-        WideRow<T> xr;
-        float xc[2][4];  // rows 4q .. 4q+3 (those of this lane's results), places i and 16+i
-        float d[4];      // dy or residual of those results
-        bool whole;      // no row of it is absent
-    };
-    const long long col = on ? mh : (long long)m * a.H;  // (lanes past the sets read the first one's)
-    auto load_tile = [&](int r, Meta u) {
-        Tile v;
-        v.u = u;
-        v.whole = present && __ballot(u.idx < 0) == 0;
-        const int j = u.idx < 0 ? 0 : u.idx;
-        v.xr.load(x + j * step, q);
+    auto finish = [&](int r, const Tile &t) {
+        float f[8];
+        t.x.values(f);
+        float4_v z = bias;
+#pragma unroll
+        for (int k = 0; k < 8; k++) z = __builtin_amdgcn_mfma_f32_16x16x4f32(w[k], f[k], z, 0, 0, 0);
+        float4_v y;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const int row = r + q * 4 + k < r1 ? r + q * 4 + k : r0;
-            if constexpr (MODE == kResponse) {
-                if (a.res_kind != SC_RES_NONE)
-                    v.d[k] = a.res[(long long)row * a.res_ld + (a.res_kind == SC_RES_FULL ? col : 0)];
+            y[k] = a.alpha * (a.act == SC_ACT_SIGMOID ? sigmoid(z[k]) : z[k]);
+            if (t.idx < 0 || !u.present) y[k] = 0.0f;  // an absent row or patch has no response
+            if (a.res_kind != SC_RES_NONE) y[k] += a.beta * t.res[k];
+        }
+        const int row = r + i;
+        if (row < u.r1) {
+            float *p = a.y + (long long)row * a.y_ld + first + 4 * q;
+            if (left >= 4) {
+                *reinterpret_cast<float4_a4 *>(p) = y;
             } else {
-                if constexpr (MODE == kGrad) v.d[k] = a.dy[(long long)row * a.dy_ld + col];
-                const char *at = x + __shfl(j, q * 4 + k, 64) * step + i * T::kSize;
-                v.xc[0][k] = load_one<T>(at);
-                v.xc[1][k] = load_one<T>(at + 16 * T::kSize);
+#pragma unroll
+                for (int k = 0; k < 3; k++)
+                    if (k < left) p[k] = y[k];
             }
         }
-        return v;
     };
-    auto products = [&](int r, Tile &v) {
-        float f[8];
-        v.xr.values(f);
+    // two tiles in turn: the next one's loads are issued before a tile's
+    // products, its rows' numbers a tile earlier still
+    int ahead = row_of(u.r0 + 16);
+    Tile one = load(u.r0, row_of(u.r0)), two;
+    for (int r = u.r0; r < u.r1; r += 32) {
+        two = load(r + 16, ahead);
+        ahead = row_of(r + 32);
+        finish(r, one);
+        if (r + 16 >= u.r1) break;
+        one = load(r + 32, ahead);
+        ahead = row_of(r + 48);
+        finish(r + 16, two);
+    }
+}
+
+// What the gradient kernels of the wide form know of a lane's row r + i ...
+struct WideMeta {
+    int idx;         // its sample; -1: absent, or past the end
+    float pos, neg;  // (loss)
+};
+template <int MODE>
+__device__ __forceinline__ WideMeta wide_meta(const LrArgs &a, const WideUnit &u, int r, int i) {
+    WideMeta v{-1, 0.0f, 0.0f};
+    if (r + i < u.r1) {
+        v.idx = a.rows ? a.rows[r + i] : r + i;
+        if ((unsigned)v.idx >= (unsigned)a.n) v.idx = -1;
+    }
+    if constexpr (MODE == kLoss) {
+        if (v.idx >= 0) {
+            const float c = a.weight ? a.weight[v.idx] : 1.0f, t = a.target[v.idx];
+            v.pos = c * (1.0f - t);
+            v.neg = c * t;
+            if (c == 0.0f) v.idx = -1;  // a row without weight is not looked at, whatever it holds
+        }
+    }
+    return v;
+}
+
+// two neighbouring values as they are loaded
+typedef float float2_a4 __attribute__((ext_vector_type(2), aligned(4)));
+typedef unsigned uint_a2 __attribute__((aligned(2)));
+template <class T>
+using PlacePair = std::conditional_t<T::kSize == 4, float __attribute__((ext_vector_type(2))), unsigned>;
+template <class T>
+__device__ __forceinline__ PlacePair<T> load_pair(const char *p) {
+    if constexpr (T::kSize == 4) return *reinterpret_cast<const float2_a4 *>(p);
+    else return *reinterpret_cast<const uint_a2 *>(p);
+}
+
+// ... and what they load of 16 rows.  Absent rows load some sample's values
+// instead, which are cleared where they are used: a tile without any (every
+// tile but the last, mostly) has no branches.
+template <class T>
+struct WideTile {
+    WideMeta v;
+    WideRow<T> x;                                        // row i
+    PlacePair<T> xc[4];  // rows 4q .. 4q+3, places 2i and 2i+1
+    float dy[4];                                         // of those rows, set i
+    bool whole;                                          // no row of it is absent
+};
+struct WideOffsets {
+    unsigned row, place[4];
+};
+template <class T>
+__device__ __forceinline__ WideOffsets wide_offsets(const WideUnit &u, int i, int q) {
+    WideOffsets o;
+    o.row = (unsigned)(i * u.step) + q * 16;
+#pragma unroll
+    for (int k = 0; k < 4; k++) o.place[k] = (unsigned)((4 * q + k) * u.step) + 2 * i * T::kSize;
+    return o;
+}
+template <class T, int MODE>
+__device__ __forceinline__ void wide_load(const LrArgs &a, const WideUnit &u, const WideOffsets &o, int r, WideMeta v,
+                                          int i, int q, long long col, WideTile<T> &t) {
+    t.v = v;
+    t.whole = u.present && __ballot(v.idx < 0) == 0;
+    if (u.in_order && r + 16 <= u.r1) {
+        const char *base = u.x + r * u.step;
+        t.x.load(base + o.row);
+#pragma unroll
+        for (int k = 0; k < 4; k++) t.xc[k] = load_pair<T>(base + o.place[k]);
+    } else {
+        const int j = v.idx < 0 ? 0 : v.idx;
+        t.x.load(u.x + j * u.step + q * 16);
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            t.xc[k] = load_pair<T>(u.x + __shfl(j, q * 4 + k, 64) * u.step + 2 * i * T::kSize);
+    }
+    if constexpr (MODE == kGrad) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int row = r + q * 4 + k < u.r1 ? r + q * 4 + k : u.r0;
+            t.dy[k] = a.dy[(long long)row * a.dy_ld + col];
+        }
+    }
+}
+
+// g of this lane's four results; clears what an absent row loaded
+template <class T, int MODE>
+__device__ __forceinline__ void wide_grad(const LrArgs &a, const WideUnit &u, WideTile<T> &t, float4_v z, int r, int q,
+                                          bool on, long long col, float (&g)[4], float &sum_g, float &sum_l) {
+    float pos[4], neg[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        if constexpr (MODE == kLoss) {
+            pos[k] = __shfl(t.v.pos, q * 4 + k, 64);
+            neg[k] = __shfl(t.v.neg, q * 4 + k, 64);
+        } else {
+            pos[k] = a.alpha * t.dy[k];
+            neg[k] = 0.0f;
+            const int row = r + q * 4 + k;
+            if (a.res_kind == SC_RES_FULL && on && row < u.r1)
+                a.dres[(long long)row * a.dres_ld + col] = a.beta * t.dy[k];
+        }
+    }
+    if (t.whole) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) g[k] = grad_of<MODE>(a.act, z[k], pos[k], neg[k], sum_l);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const bool there = u.present && __shfl(t.v.idx, q * 4 + k, 64) >= 0;
+            float l = 0.0f;
+            const float gk = grad_of<MODE>(a.act, z[k], pos[k], neg[k], l);
+            g[k] = there ? gk : 0.0f;
+            sum_l += there ? l : 0.0f;
+            if (!there) t.xc[k] = PlacePair<T>{};
+        }
+    }
+    sum_g += (g[0] + g[1]) + (g[2] + g[3]);
+}
+
+// a wave's sums -> the partial sums of its chunk, or the results
+template <int MODE>
+__device__ __forceinline__ void wide_store(const LrArgs &a, const WideUnit &u, const float4_v *acc, float sum_g,
+                                           float sum_l, int i, int q) {
+    sum_g += __shfl_xor(sum_g, 16, 64);
+    sum_g += __shfl_xor(sum_g, 32, 64);
+    sum_l += __shfl_xor(sum_l, 16, 64);
+    sum_l += __shfl_xor(sum_l, 32, 64);
+    const long long first = (long long)u.m * a.H + u.h0;
+    float *part = a.part ? a.part + (long long)blockIdx.y * a.M * a.H * kPartWords : nullptr;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {  // set 4q+k, places 2i and 2i+1
+        if (u.h0 + q * 4 + k >= a.H) continue;
+        const long long mh = first + q * 4 + k;
+        float *to = part ? part + mh * kPartWords : a.dw + mh * kDesc;
+        to[2 * i] = acc[0][k];
+        to[2 * i + 1] = acc[1][k];
+    }
+    if (u.h0 + i < a.H && q == 0) {
+        if (part) {
+            part[(first + i) * kPartWords + kDesc] = sum_g;
+            part[(first + i) * kPartWords + kDesc + 1] = sum_l;
+        } else {
+            a.db[first + i] = sum_g;
+            if (MODE == kLoss) a.loss[first + i] = sum_l;
+        }
+    }
+}
+
+template <class T>
+__device__ __forceinline__ float place_value(const WideTile<T> &t, int half, int k) {
+    if constexpr (__is_same(T, F32)) return t.xc[k][half];
+    else if constexpr (__is_same(T, F16)) return (float)__builtin_bit_cast(half2_v, t.xc[k])[half];
+    else return __uint_as_float(half ? t.xc[k] & 0xffff0000u : t.xc[k] << 16);
+}
+
+// Gradient and loss, f32 products (16x16x4: nothing is rounded that the narrow
+// form does not round).
+template <class T, int MODE>
+__global__ __launch_bounds__(64 * kWideWaves, 4) void lr_wide_kernel(LrArgs a) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int i = lane & 15, q = lane >> 4;
+    WideUnit u;
+    if (!wide_unit<T>(a, wave, u)) return;
+    const bool on = u.h0 + i < a.H;
+    const long long col = (long long)u.m * a.H + (on ? u.h0 + i : 0);  // (lanes past the sets read the first one's)
+    float w[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) w[k] = on ? a.w[col * kDesc + WideRow<T>::place(q, k)] : 0.0f;
+    const float bias = on && a.b ? a.b[col] : 0.0f;
+    const WideOffsets o = wide_offsets<T>(u, i, q);
+    float4_v acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    float sum_g = 0.0f, sum_l = 0.0f;
+    auto products = [&](int r, WideTile<T> &t) {
+        float f[8], g[4];
+        t.x.values(f);
         float4_v z = {bias, bias, bias, bias};
 #pragma unroll
         for (int k = 0; k < 8; k++) z = __builtin_amdgcn_mfma_f32_16x16x4f32(f[k], w[k], z, 0, 0, 0);
-        if constexpr (MODE == kResponse) {
+        wide_grad<T, MODE>(a, u, t, z, r, q, on, col, g, sum_g, sum_l);
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const int row = r + q * 4 + k;
-                float y = a.alpha * (a.act == SC_ACT_SIGMOID ? sigmoid(z[k]) : z[k]);
-                if (!v.whole && (!present || __shfl(v.u.idx, q * 4 + k, 64) < 0)) y = 0.0f;  // absent: no response
-                if (a.res_kind != SC_RES_NONE) y += a.beta * v.d[k];
-                if (on && row < r1) a.y[(long long)row * a.y_ld + mh] = y;
-            }
-        } else {
-            float g[4], l = 0.0f;
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                float pos, neg = 0.0f;
-                if constexpr (MODE == kLoss) {
-                    pos = __shfl(v.u.pos, q * 4 + k, 64);
-                    neg = __shfl(v.u.neg, q * 4 + k, 64);
-                } else {
-                    pos = a.alpha * v.d[k];
-                }
-                if (v.whole) {
-                    g[k] = grad_of<MODE>(a.act, z[k], pos, neg, l);
-                } else {
-                    const bool there = present && __shfl(v.u.idx, q * 4 + k, 64) >= 0;
-                    float lk = 0.0f;
-                    const float gk = grad_of<MODE>(a.act, z[k], pos, neg, lk);
-                    g[k] = there ? gk : 0.0f;
-                    l += there ? lk : 0.0f;
-                    v.xc[0][k] = there ? v.xc[0][k] : 0.0f;
-                    v.xc[1][k] = there ? v.xc[1][k] : 0.0f;
-                }
-                sum_g += g[k];
-            }
-            sum_l += l;
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                acc[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(g[k], v.xc[0][k], acc[0], 0, 0, 0);
-                acc[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(g[k], v.xc[1][k], acc[1], 0, 0, 0);
-            }
+        for (int k = 0; k < 4; k++) {
+            acc[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(g[k], place_value<T>(t, 0, k), acc[0], 0, 0, 0);
+            acc[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(g[k], place_value<T>(t, 1, k), acc[1], 0, 0, 0);
         }
     };
-    Meta meta = load_meta(r0 + 16);
-    Tile one = load_tile(r0, load_meta(r0)), two;
-    for (int r = r0; r < r1; r += 32) {
-        two = load_tile(r + 16, meta);
-        meta = load_meta(r + 32);
+    WideMeta ahead = wide_meta<MODE>(a, u, u.r0 + 16, i);
+    WideTile<T> one, two;
+    wide_load<T, MODE>(a, u, o, u.r0, wide_meta<MODE>(a, u, u.r0, i), i, q, col, one);
+    for (int r = u.r0; r < u.r1; r += 32) {
+        wide_load<T, MODE>(a, u, o, r + 16, ahead, i, q, col, two);
+        ahead = wide_meta<MODE>(a, u, r + 32, i);
         products(r, one);
-        if (r + 16 >= r1) break;
-        one = load_tile(r + 32, meta);
-        meta = load_meta(r + 48);
+        if (r + 16 >= u.r1) break;
+        wide_load<T, MODE>(a, u, o, r + 32, ahead, i, q, col, one);
+        ahead = wide_meta<MODE>(a, u, r + 48, i);
         products(r + 16, two);
     }
-    if constexpr (MODE != kResponse) {
-        sum_g += __shfl_xor(sum_g, 16, 64);
-        sum_g += __shfl_xor(sum_g, 32, 64);
-        sum_l += __shfl_xor(sum_l, 16, 64);
-        sum_l += __shfl_xor(sum_l, 32, 64);
-        const int h0 = (unit - m * sets) * 16;
+    wide_store<MODE>(a, u, acc, sum_g, sum_l, i, q);
+}
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// v = a + b + c, each a bfloat16 (8 + 8 + 8 bits of 24): the high halves
+__device__ __forceinline__ void split3(float v, unsigned &a, unsigned &b, unsigned &c) {
+    a = __float_as_uint(v) & 0xffff0000u;
+    const float r = v - __uint_as_float(a);
+    b = __float_as_uint(r) & 0xffff0000u;
+    c = __float_as_uint(r - __uint_as_float(b)) & 0xffff0000u;
+}
+// two high halves -> one register, `lo` first
+__device__ __forceinline__ unsigned pack(unsigned lo, unsigned hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
+
+// Gradient and loss of bfloat16 samples on the bfloat16 matrix cores (16x16x32,
+// a fifth of the f32 ones' time for these products): the samples are exact
+// there, and the weights and g go in as sums of three bfloat16 each, their 24
+// bits whole, so every product is exact and the sums are f32 as before.
+template <int MODE>
+__global__ __launch_bounds__(64 * kWideWaves) void lr_wide_bf16_kernel(LrArgs a) {
+    using T = BF16;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int i = lane & 15, q = lane >> 4;
+    WideUnit u;
+    if (!wide_unit<T>(a, wave, u)) return;
+    const bool on = u.h0 + i < a.H;
+    const long long col = (long long)u.m * a.H + (on ? u.h0 + i : 0);
+    uint4_v w[3];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {  // set 4q+k, places i and 16+i
-            const int hk = h0 + q * 4 + k;
-            if (hk >= a.H) continue;
-            const long long at = (long long)m * a.H + hk;
-            float *to = a.part ? a.part + ((long long)blockIdx.y * a.M * a.H + at) * kPartWords : a.dw + at * kDesc;
-            to[i] = acc[0][k];
-            to[16 + i] = acc[1][k];
-        }
-        if (on && q == 0) {
-            if (a.part) {
-                float *to = a.part + ((long long)blockIdx.y * a.M * a.H + mh) * kPartWords;
-                to[kDesc] = sum_g;
-                to[kDesc + 1] = sum_l;
-            } else {
-                a.db[mh] = sum_g;
-                if (MODE == kLoss) a.loss[mh] = sum_l;
-            }
-        }
+    for (int k = 0; k < 4; k++) {
+        unsigned lo[3], hi[3];
+        split3(on ? a.w[col * kDesc + 8 * q + 2 * k] : 0.0f, lo[0], lo[1], lo[2]);
+        split3(on ? a.w[col * kDesc + 8 * q + 2 * k + 1] : 0.0f, hi[0], hi[1], hi[2]);
+#pragma unroll
+        for (int e = 0; e < 3; e++) w[e][k] = pack(lo[e], hi[e]);
     }
+    const float bias = on && a.b ? a.b[col] : 0.0f;
+    const WideOffsets o = wide_offsets<T>(u, i, q);
+    float4_v acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    float sum_g = 0.0f, sum_l = 0.0f;
+    auto dot = [&](const WideTile<T> &t) {
+        const bf16x8 x = __builtin_bit_cast(bf16x8, t.x.a);
+        float4_v z = {bias, bias, bias, bias};
+#pragma unroll
+        for (int e = 2; e >= 0; e--)
+            z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(bf16x8, w[e]), z, 0, 0, 0);
+        return z;
+    };
+    // the 32 rows of two tiles: k of the second product = (tile, row 4q + k)
+    auto products = [&](int r, WideTile<T> &one, WideTile<T> &two) {
+        const float4_v z1 = dot(one), z2 = dot(two);
+        float g[2][4];
+        wide_grad<T, MODE>(a, u, one, z1, r, q, on, col, g[0], sum_g, sum_l);
+        wide_grad<T, MODE>(a, u, two, z2, r + 16, q, on, col, g[1], sum_g, sum_l);
+        uint4_v gs[3], xs[2];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int tile = k >> 1, e = 2 * (k & 1);
+            unsigned lo[3], hi[3];
+            split3(g[tile][e], lo[0], lo[1], lo[2]);
+            split3(g[tile][e + 1], hi[0], hi[1], hi[2]);
+#pragma unroll
+            for (int p = 0; p < 3; p++) gs[p][k] = pack(lo[p], hi[p]);
+            const WideTile<T> &t = tile ? two : one;
+            xs[0][k] = __builtin_amdgcn_perm(t.xc[e + 1], t.xc[e], 0x05040100u);  // the low halves
+            xs[1][k] = pack(t.xc[e], t.xc[e + 1]);
+        }
+#pragma unroll
+        for (int p = 2; p >= 0; p--)
+#pragma unroll
+            for (int half = 0; half < 2; half++)
+                acc[half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, gs[p]),
+                                                                    __builtin_bit_cast(bf16x8, xs[half]), acc[half], 0, 0, 0);
+    };
+    WideTile<T> t[4];
+    auto load = [&](int r, int k, const WideMeta &m0, const WideMeta &m1) {
+        wide_load<T, MODE>(a, u, o, r, m0, i, q, col, t[k]);
+        wide_load<T, MODE>(a, u, o, r + 16, m1, i, q, col, t[k + 1]);
+    };
+    WideMeta m0 = wide_meta<MODE>(a, u, u.r0 + 32, i), m1 = wide_meta<MODE>(a, u, u.r0 + 48, i);
+    load(u.r0, 0, wide_meta<MODE>(a, u, u.r0, i), wide_meta<MODE>(a, u, u.r0 + 16, i));
+    for (int r = u.r0; r < u.r1; r += 64) {
+        load(r + 32, 2, m0, m1);
+        m0 = wide_meta<MODE>(a, u, r + 64, i);
+        m1 = wide_meta<MODE>(a, u, r + 80, i);
+        products(r, t[0], t[1]);
+        if (r + 32 >= u.r1) break;
+        load(r + 64, 0, m0, m1);
+        m0 = wide_meta<MODE>(a, u, r + 96, i);
+        m1 = wide_meta<MODE>(a, u, r + 112, i);
+        products(r + 32, t[2], t[3]);
+    }
+    wide_store<MODE>(a, u, acc, sum_g, sum_l, i, q);
 }
 
 // Joins the row chunks' partial sums: 32 neighbouring words per workgroup, its
@@ -551,14 +810,7 @@ __global__ __launch_bounds__(256) void lr_join_kernel(LrArgs a, int loss) {
     else if (loss) a.loss[mh] = (float)s;
 }
 
-// gradient of a residual: beta * dy, or its sum over a row's results
-__global__ __launch_bounds__(256) void res_full_kernel(LrArgs a) {
-    const long long cols = (long long)a.M * a.H;
-    for (long long r = blockIdx.y; r < a.R; r += gridDim.y)
-        for (long long c = (long long)blockIdx.x * 256 + threadIdx.x; c < cols; c += (long long)gridDim.x * 256)
-            a.dres[r * a.dres_ld + c] = a.beta * a.dy[r * a.dy_ld + c];
-}
-
+// gradient of a residual of one value per row: beta * the sum of the row's dy
 __global__ __launch_bounds__(256) void res_row_kernel(LrArgs a) {
     __shared__ double s_sum[4];
     const long long cols = (long long)a.M * a.H;
@@ -586,7 +838,10 @@ bool wide(const LrArgs &a) { return a.H > kNarrowSets; }
 template <class T, int MODE>
 void launch_form(const LrArgs &a, dim3 grid, hipStream_t s) {
     if (wide(a)) {
-        hipLaunchKernelGGL((lr_wide_kernel<T, MODE>), grid, dim3(64 * kWaves), 0, s, a);
+        constexpr dim3 block(64 * kWideWaves);
+        if constexpr (MODE == kResponse) hipLaunchKernelGGL((lr_wide_response_kernel<T>), grid, block, 0, s, a);
+        else if constexpr (__is_same(T, BF16)) hipLaunchKernelGGL((lr_wide_bf16_kernel<MODE>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((lr_wide_kernel<T, MODE>), grid, block, 0, s, a);
         return;
     }
     switch (sets_per_wave(a)) {
@@ -607,18 +862,27 @@ void launch_mode(const LrArgs &a, dim3 grid, hipStream_t s) {
 
 }  // namespace
 
-// Gradient and loss: rows are cut into chunks until the grid has a few waves
-// per SIMD of the 256 CUs; a chunk is one range of rows per wave of a
-// workgroup (narrow form), or one for all of them (wide form).
+// Gradient and loss: rows are cut into chunks, of one range of rows per wave of
+// a workgroup (narrow form) or one for all of them (wide form).  The grid runs
+// in rounds of as many waves as the registers of 256 CUs hold, so the time is
+// about rounds x (rows per wave + what a wave's start and end cost, some 48
+// rows' time): the number of chunks with the least of that.
 LrPlan lr_plan(const LrArgs &a) {
     LrPlan p{0, 0, 0};
     if (a.R == 0) return p;
     const int step = wide(a) ? 16 : lanes_per_item(a), ranges = wide(a) ? 1 : kWaves;
     const long long waves = wide(a) ? a.M * ceil_div(a.H, 16)
                                     : ceil_div(a.M, items_per_wave(a)) * ceil_div(a.H, sets_per_wave(a)) * kWaves;
-    long long chunks = ceil_div(4096, waves);
-    if (chunks > ceil_div(a.R, (long long)ranges * step)) chunks = ceil_div(a.R, (long long)ranges * step);
-    p.rows_per_wave = (int)(ceil_div(ceil_div(a.R, chunks * ranges), step) * step);
+    const long long room = 1024 * (wide(a) || a.H == 2 ? 4 : a.H == 1 ? 6 : 3);
+    const long long most = ceil_div(a.R, (long long)ranges * step);
+    long long best = -1;
+    for (long long chunks = 1; chunks <= most && (chunks == 1 || waves * (chunks - 1) < 4 * room); chunks++) {
+        const long long rows = ceil_div(ceil_div(a.R, chunks * ranges), step) * step;
+        const long long cost = ceil_div(waves * chunks, room) * (rows + 48);
+        if (best >= 0 && cost >= best) continue;
+        best = cost;
+        p.rows_per_wave = (int)rows;
+    }
     p.chunks = (int)ceil_div(a.R, (long long)p.rows_per_wave * ranges);
     if (p.chunks > 1) p.part_bytes = (size_t)p.chunks * a.M * a.H * kPartWords * sizeof(float);
     return p;
@@ -628,9 +892,10 @@ void launch_lr_response(const LrArgs &a0, hipStream_t s) {
     LrArgs a = a0;
     const int step = wide(a) ? 16 : lanes_per_item(a);
     const long long units = wide(a) ? a.M * ceil_div(a.H, 16) : ceil_div(a.M, items_per_wave(a));
-    const long long wgs = ceil_div(units, kWaves), hs = wide(a) ? 1 : ceil_div(a.H, sets_per_wave(a));
+    const int wg = wide(a) ? kWideWaves : kWaves;
+    const long long wgs = ceil_div(units, wg), hs = wide(a) ? 1 : ceil_div(a.H, sets_per_wave(a));
     // rows per wave: enough waves for the chip, at most 64 rows, at most 65535 chunks
-    long long rows = ceil_div(ceil_div(a.R, ceil_div(8192, wgs * hs * kWaves)), step) * step;
+    long long rows = ceil_div(ceil_div(a.R, ceil_div(8192, wgs * hs * wg)), step) * step;
     if (rows > 64) rows = 64;
     const long long least = ceil_div(ceil_div(a.R, 65535), step) * step;
     a.rows_per_wave = (int)(rows > least ? rows : least);
@@ -639,7 +904,7 @@ void launch_lr_response(const LrArgs &a0, hipStream_t s) {
 
 void launch_lr_grad(const LrArgs &a, bool loss, hipStream_t s) {
     if (a.chunks > 0) {
-        const dim3 grid = wide(a) ? dim3((unsigned)ceil_div(a.M * ceil_div(a.H, 16), kWaves), (unsigned)a.chunks)
+        const dim3 grid = wide(a) ? dim3((unsigned)ceil_div(a.M * ceil_div(a.H, 16), kWideWaves), (unsigned)a.chunks)
                                   : dim3((unsigned)ceil_div(a.M, items_per_wave(a)), (unsigned)a.chunks,
                                          (unsigned)ceil_div(a.H, sets_per_wave(a)));
         if (loss) launch_mode<kLoss>(a, grid, s);
@@ -651,16 +916,9 @@ void launch_lr_grad(const LrArgs &a, bool loss, hipStream_t s) {
     }
 }
 
-void launch_lr_res_grad(const LrArgs &a, hipStream_t s) {
-    if (a.R == 0) return;
-    if (a.res_kind == SC_RES_ROW) {
+void launch_lr_res_row(const LrArgs &a, hipStream_t s) {
+    if (a.R > 0)
         hipLaunchKernelGGL(res_row_kernel, dim3((unsigned)(a.R < 8192 ? a.R : 8192)), dim3(256), 0, s, a);
-    } else {
-        const long long cols = (long long)a.M * a.H;
-        const long long bx = ceil_div(cols, 256);
-        hipLaunchKernelGGL(res_full_kernel, dim3((unsigned)(bx < 64 ? bx : 64), (unsigned)(a.R < 4096 ? a.R : 4096)),
-                           dim3(256), 0, s, a);
-    }
 }
 
 }  // namespace sc

@@ -55,7 +55,7 @@ LrPlan lr_plan(const LrArgs &a);
 
 void launch_lr_response(const LrArgs &a, hipStream_t s);
 void launch_lr_grad(const LrArgs &a, bool loss, hipStream_t s);  // + the join of its chunks
-void launch_lr_res_grad(const LrArgs &a, hipStream_t s);
+void launch_lr_res_row(const LrArgs &a, hipStream_t s);  // dres of SC_RES_ROW (SC_RES_FULL's: launch_lr_grad)
 
 struct SampleArgs {
     const void *scores;

@@ -12,33 +12,18 @@ from __future__ import annotations
 
 import ctypes
 
-from . import SurfCascadeError, _check, load_library  # noqa: F401
+from . import _check, _SampleParams, _Samples, _WeakBank, load_library
 
 _ACT = {"none": 0, "sigmoid": 1}
 _RES = {None: 0, "none": 0, "row": 1, "full": 2}
 
 
-class _Samples(ctypes.Structure):
-    _fields_ = [("data", ctypes.c_void_p), ("dtype", ctypes.c_int32), ("n_patches", ctypes.c_int32),
-                ("n", ctypes.c_int64), ("ld", ctypes.c_int64), ("rows", ctypes.c_void_p),
-                ("n_rows", ctypes.c_int64)]
-
-
-class _WeakBank(ctypes.Structure):
-    _fields_ = [("m", ctypes.c_int32), ("h", ctypes.c_int32), ("patch", ctypes.c_void_p),
-                ("w", ctypes.c_void_p), ("b", ctypes.c_void_p)]
-
-
-class _SampleParams(ctypes.Structure):
-    _fields_ = [("temperature", ctypes.c_double), ("top_k", ctypes.c_int32),
-                ("top_p", ctypes.c_double), ("min_p", ctypes.c_double)]
-
-
 class Trainer:
     """Launches the training kernels of one GPU (sc_trainer).  Calls are
     asynchronous and ordered like torch operations: they run on torch's current
-    stream of the trainer's device, allocate their results and workspaces from
-    torch, and can be captured into a graph.  Tensors live on the trainer's
+    stream of the trainer's device, allocate their results from torch, and can be
+    captured into a graph (workspaces: the trainer's own, a captured call's the
+    graph's).  Tensors live on the trainer's
     device; a layout the C ABI does not take is refused, not copied.  One
     trainer is not thread-safe.
 
@@ -55,6 +40,8 @@ class Trainer:
         self._L = load_library()
         self.device = int(device)
         self._dev = torch.device("cuda", self.device)
+        self._f32, self._f64, self._i32 = torch.float32, torch.float64, torch.int32
+        self._ws = None
         h = ctypes.c_void_p()
         _check(self._L.sc_trainer_create(self.device, ctypes.byref(h)))
         self._h = h.value
@@ -76,20 +63,21 @@ class Trainer:
     def _follow(self):
         """Launch on torch's current stream of this device (a trainer that
         changes streams waits for its earlier work, sc_trainer_set_stream)."""
-        if self._h is None:
-            raise ValueError("the trainer is closed")
         s = self._raw(self.device) if self._raw is not None \
             else self._torch.cuda.current_stream(self.device).cuda_stream
         if s != self._on:
+            if self._h is None:
+                raise ValueError("the trainer is closed")
             _check(self._L.sc_trainer_set_stream(self._h, s or None, 0))
             self._on = s
 
     def _need(self, t, dtype, shape, what):
-        """A contiguous tensor of this type and shape on this device."""
-        if t.dtype != dtype or t.get_device() != self.device:
+        """The address of a contiguous tensor of this type and shape on this
+        device (an empty one: any device address)."""
+        if t.dtype is not dtype or t.get_device() != self.device:
             raise ValueError("%s must be a %s tensor on cuda:%d (got %s on %s)"
                              % (what, dtype, self.device, t.dtype, t.device))
-        if tuple(t.shape) != shape or not t.is_contiguous():
+        if t.shape != shape or not t.is_contiguous():
             raise ValueError("%s must be contiguous, of shape %s (got %s, strides %s)"
                              % (what, shape, tuple(t.shape), t.stride()))
         return t.data_ptr()
@@ -97,59 +85,69 @@ class Trainer:
     def _rowwise(self, t, dtype, r, cols, what):
         """[r, cols] (or [r, m, h], cols = m*h) values, each row contiguous ->
         (pointer, stride between rows)."""
-        if t.dtype != dtype or t.get_device() != self.device:
+        if t.dtype is not dtype or t.get_device() != self.device:
             raise ValueError("%s must be a %s tensor on cuda:%d (got %s on %s)"
                              % (what, dtype, self.device, t.dtype, t.device))
-        n, step = 1, 1
-        for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
-            if size != 1 and stride != step:
-                raise ValueError("each row of %s must be contiguous (strides %s)" % (what, t.stride()))
-            step *= size
-            n *= size
-        if t.dim() < 2 or t.shape[0] != r or n != cols:
-            raise ValueError("%s must have %d rows of %d values (got %s)" % (what, r, cols, tuple(t.shape)))
-        ld = t.stride(0)
-        if r > 1 and cols > 0 and ld < cols:
-            raise ValueError("rows of %s overlap (strides %s)" % (what, t.stride()))
-        return t.data_ptr(), max(ld, cols)
+        shape = t.shape
+        if len(shape) < 2 or shape[0] != r or t.numel() != r * cols:
+            raise ValueError("%s must have %d rows of %d values (got %s)" % (what, r, cols, tuple(shape)))
+        if t.is_contiguous():
+            return t.data_ptr(), cols
+        stride, step = t.stride(), 1
+        for k in range(len(shape) - 1, 0, -1):
+            if shape[k] != 1 and stride[k] != step:
+                raise ValueError("each row of %s must be contiguous (strides %s)" % (what, stride))
+            step *= shape[k]
+        if r > 1 and stride[0] < cols:
+            raise ValueError("rows of %s overlap (strides %s)" % (what, stride))
+        return t.data_ptr(), max(stride[0], cols)
 
     def _operands(self, samples, w, b, patch, rows):
-        torch = self._torch
-        if samples.dtype not in self._dtypes or samples.get_device() != self.device:
+        f32, i32 = self._f32, self._i32
+        dtype = self._dtypes.get(samples.dtype)
+        if dtype is None or samples.get_device() != self.device:
             raise ValueError("samples must be float32, float16 or bfloat16 on cuda:%d (got %s on %s)"
                              % (self.device, samples.dtype, samples.device))
-        if samples.dim() != 3 or samples.shape[2] != 32:
-            raise ValueError("samples must be [n, n_patches, 32] (got %s)" % (tuple(samples.shape),))
-        n, p, _ = samples.shape
-        s0, s1, s2 = samples.stride()
-        if s2 != 1 or (p > 1 and s1 != 32) or (n > 1 and s0 < 32 * p):
-            raise ValueError("each sample's descriptors must be contiguous (strides %s)" % (samples.stride(),))
-        if w.dim() not in (2, 3) or w.shape[-1] != 32:
+        shape, sets = samples.shape, w.shape[:-1]  # sets: (m,) or (m, h)
+        if len(shape) != 3 or shape[2] != 32:
+            raise ValueError("samples must be [n, n_patches, 32] (got %s)" % (tuple(shape),))
+        if not 1 <= len(sets) <= 2 or w.shape[-1] != 32:
             raise ValueError("w must be [m, 32] or [m, h, 32] (got %s)" % (tuple(w.shape),))
-        sets = tuple(w.shape[:-1])  # (m,) or (m, h)
-        m, h = sets[0], (sets[1] if len(sets) == 2 else 1)
-        x = _Samples(samples.data_ptr(), self._dtypes[samples.dtype], p, n, max(s0, 32 * p), None, 0)
-        r = n
+        n, p, _ = shape
+        ld = 32 * p
+        if not samples.is_contiguous():
+            s0, s1, s2 = samples.stride()
+            if s2 != 1 or (p > 1 and s1 != 32) or (n > 1 and s0 < ld):
+                raise ValueError("each sample's descriptors must be contiguous (strides %s)" % (samples.stride(),))
+            ld = max(s0, ld)
+        m, h = sets if len(sets) == 2 else (sets[0], 1)
+        r, at = n, None
         if rows is not None:
             r = rows.numel()
-            x.rows = self._need(rows, torch.int32, (r,), "rows") or 1  # (an empty tensor has no address)
-            x.n_rows = r
-        k = _WeakBank(m, h, None if patch is None else self._need(patch, torch.int32, (m,), "patch") or None,
-                      self._need(w, torch.float32, sets + (32,), "w"),
-                      None if b is None else self._need(b, torch.float32, sets, "b") or None)
-        if patch is None and m > p:
+            at = self._need(rows, i32, (r,), "rows") or 1  # (an empty tensor has no address)
+        if patch is not None:
+            patch = self._need(patch, i32, (m,), "patch") or None
+        elif m > p:
             raise ValueError("%d weak learners, %d patches and no patch numbers" % (m, p))
+        x = _Samples(samples.data_ptr(), dtype, p, n, ld, at, r)
+        k = _WeakBank(m, h, patch, self._need(w, f32, sets + (32,), "w"),
+                      None if b is None else self._need(b, f32, sets, "b") or None)
         return x, k, r, sets, m * h
 
-    def _empty(self, shape, dtype=None):
-        return self._torch.empty(shape, dtype=dtype or self._torch.float32, device=self._dev)
-
-    def _workspace(self, bytes_):
-        return self._torch.empty(bytes_, dtype=self._torch.uint8, device=self._dev) if bytes_ else None
-
-    @staticmethod
-    def _ptr(t):
-        return None if t is None else t.data_ptr()
+    def _workspace(self, rc, bytes_):
+        """After a call that brought no workspace: True when it has to be made
+        again with the one now in self._ws, of bytes_() bytes.  A captured call
+        needs memory of its graph's own (the trainer's own is shared by its
+        other calls), which torch's allocator hands out under a capture."""
+        if rc == 0:
+            return False
+        if rc == -1 and self._torch.cuda.is_current_stream_capturing():
+            n = bytes_()
+            if n:
+                self._ws = self._torch.empty(n, dtype=self._torch.uint8, device=self._dev)
+                return True
+        _check(rc)
+        return False
 
     # -- weak learners -------------------------------------------------------
     def response(self, samples, w, b=None, patch=None, rows=None, activation="sigmoid", alpha=1.0,
@@ -160,22 +158,24 @@ class Trainer:
         self._follow()
         x, k, r, sets, cols = self._operands(samples, w, b, patch, rows)
         res, kind, res_ld = None, 0, 0
-        if residual is not None and residual.dim() == 1:
-            kind, res_ld = 1, 1
-            if residual.shape[0] != r or residual.dtype != self._torch.float32 \
-                    or residual.get_device() != self.device or (r > 1 and residual.stride(0) < 1):
-                raise ValueError("residual must be float32 [%d] on cuda:%d" % (r, self.device))
-            res, res_ld = residual.data_ptr(), max(residual.stride(0), 1)
-        elif residual is not None:
-            kind = 2
-            res, res_ld = self._rowwise(residual, self._torch.float32, r, cols, "residual")
+        if residual is not None:
+            if residual.dim() == 1:
+                kind, res_ld = 1, residual.stride(0)
+                if residual.shape[0] != r or residual.dtype is not self._f32 \
+                        or residual.get_device() != self.device or (r > 1 and res_ld < 1):
+                    raise ValueError("residual must be float32 [%d] on cuda:%d" % (r, self.device))
+                res, res_ld = residual.data_ptr(), max(res_ld, 1)
+            else:
+                kind = 2
+                res, res_ld = self._rowwise(residual, self._f32, r, cols, "residual")
         if out is None:
-            out = self._empty((r,) + sets)
+            out = w.new_empty((r,) + sets)
             y, y_ld = out.data_ptr(), cols
         else:
-            y, y_ld = self._rowwise(out, self._torch.float32, r, cols, "out")
-        _check(self._L.sc_lr_response(self._h, ctypes.byref(x), ctypes.byref(k), _ACT[activation], alpha,
-                                      res, kind, res_ld, beta, y, y_ld))
+            y, y_ld = self._rowwise(out, self._f32, r, cols, "out")
+        rc = self._L.sc_lr_response(self._h, x, k, _ACT[activation], alpha, res, kind, res_ld, beta, y, y_ld)
+        if rc:
+            _check(rc)
         return out
 
     def response_grad(self, samples, w, grad_out, b=None, patch=None, rows=None, activation="sigmoid",
@@ -185,14 +185,20 @@ class Trainer:
         residual: None or "none", "row" or "full", the residual's kind."""
         self._follow()
         x, k, r, sets, cols = self._operands(samples, w, b, patch, rows)
-        dy, dy_ld = self._rowwise(grad_out, self._torch.float32, r, cols, "grad_out")
+        dy, dy_ld = self._rowwise(grad_out, self._f32, r, cols, "grad_out")
         kind = _RES[residual]
-        dw, db = self._empty(sets + (32,)), self._empty(sets)
-        dres = self._empty((r,) if kind == 1 else (r,) + sets) if kind else None
-        ws, ws_bytes = self._lr_workspace(x, k)
-        _check(self._L.sc_lr_response_grad(self._h, ctypes.byref(x), ctypes.byref(k), _ACT[activation], alpha,
-                                           dy, dy_ld, dw.data_ptr(), db.data_ptr(), kind, beta,
-                                           self._ptr(dres), 1 if kind == 1 else cols, self._ptr(ws), ws_bytes))
+        dw, db, dres, dr = w.new_empty(w.shape), w.new_empty(sets), None, None
+        if kind:
+            dres = w.new_empty((r,) if kind == 1 else (r,) + sets)
+            dr = dres.data_ptr()
+
+        def call(ws, ws_bytes):
+            return self._L.sc_lr_response_grad(self._h, x, k, _ACT[activation], alpha, dy, dy_ld, dw.data_ptr(),
+                                               db.data_ptr(), kind, beta, dr, 1 if kind == 1 else cols, ws, ws_bytes)
+
+        if self._workspace(call(None, 0), lambda: self._lr_bytes(x, k)):
+            _check(call(self._ws.data_ptr(), self._ws.numel()))
+            self._ws = None
         return dw, db, dres
 
     def loss(self, samples, w, target, b=None, weight=None, patch=None, rows=None):
@@ -202,18 +208,22 @@ class Trainer:
         self._follow()
         x, k, r, sets, cols = self._operands(samples, w, b, patch, rows)
         n = samples.shape[0]
-        t = self._need(target, self._torch.float32, (n,), "target")
-        c = None if weight is None else self._need(weight, self._torch.float32, (n,), "weight") or None
-        loss, dw, db = self._empty(sets), self._empty(sets + (32,)), self._empty(sets)
-        ws, ws_bytes = self._lr_workspace(x, k)
-        _check(self._L.sc_lr_loss(self._h, ctypes.byref(x), ctypes.byref(k), t, c, loss.data_ptr(),
-                                  dw.data_ptr(), db.data_ptr(), self._ptr(ws), ws_bytes))
+        t = self._need(target, self._f32, (n,), "target")
+        c = None if weight is None else self._need(weight, self._f32, (n,), "weight") or None
+        loss, dw, db = w.new_empty(sets), w.new_empty(w.shape), w.new_empty(sets)
+
+        def call(ws, ws_bytes):
+            return self._L.sc_lr_loss(self._h, x, k, t, c, loss.data_ptr(), dw.data_ptr(), db.data_ptr(), ws, ws_bytes)
+
+        if self._workspace(call(None, 0), lambda: self._lr_bytes(x, k)):
+            _check(call(self._ws.data_ptr(), self._ws.numel()))
+            self._ws = None
         return loss, dw, db
 
-    def _lr_workspace(self, x, k):
+    def _lr_bytes(self, x, k):
         size = ctypes.c_size_t()
-        _check(self._L.sc_lr_workspace(ctypes.byref(x), ctypes.byref(k), ctypes.byref(size)))
-        return self._workspace(size.value), size.value
+        _check(self._L.sc_lr_workspace(x, k, size))
+        return size.value
 
     # -- draws ---------------------------------------------------------------
     def sample(self, scores, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, lens=None):
@@ -221,29 +231,39 @@ class Trainer:
         float32, float16 or bfloat16) by the random numbers u (float64 [s] or
         [b, s], in [0, 1)) -> (index int32 like u, kept int32 [b])
         (sc_sample).  lens: int32 [b], the length of each row."""
-        torch = self._torch
         self._follow()
-        if scores.dtype not in self._dtypes or scores.get_device() != self.device:
+        dtype, dim = self._dtypes.get(scores.dtype), scores.dim()
+        if dtype is None or scores.get_device() != self.device:
             raise ValueError("scores must be float32, float16 or bfloat16 on cuda:%d (got %s on %s)"
                              % (self.device, scores.dtype, scores.device))
-        if scores.dim() not in (1, 2) or u.dim() != scores.dim():
+        if not 1 <= dim <= 2 or u.dim() != dim:
             raise ValueError("scores [v] with u [s], or scores [b, v] with u [b, s] (got %s and %s)"
                              % (tuple(scores.shape), tuple(u.shape)))
-        s2 = scores if scores.dim() == 2 else scores[None]
-        u2 = u if u.dim() == 2 else u[None]
-        b, v = s2.shape
-        s = u2.shape[1]
-        sc, ld = self._rowwise(s2, scores.dtype, b, v, "scores")
-        up, u_ld = self._rowwise(u2, torch.float64, b, s, "u")
-        ln = None if lens is None else self._need(lens, torch.int32, (b,), "lens") or None
-        index, kept = self._empty(tuple(u.shape), torch.int32), self._empty((b,), torch.int32)
+        shape = u.shape
+        if dim == 1:
+            scores, u = scores[None], u[None]
+        b, v = scores.shape
+        s = u.shape[1]
+        sc, ld = self._rowwise(scores, scores.dtype, b, v, "scores")
+        up, u_ld = self._rowwise(u, self._f64, b, s, "u")
+        ln = None if lens is None else self._need(lens, self._i32, (b,), "lens") or None
+        index = u.new_empty(shape, dtype=self._i32)
+        kept = index.new_empty((b,))
         prm = _SampleParams(temperature, top_k, top_p, min_p)
-        size = ctypes.c_size_t()
-        _check(self._L.sc_sample_workspace(b, v, s, ctypes.byref(size)))
-        ws = self._workspace(size.value)
-        _check(self._L.sc_sample(self._h, sc, self._dtypes[scores.dtype], b, v, ld, ln, ctypes.byref(prm), up, s,
-                                 u_ld, index.data_ptr(), s, kept.data_ptr(), self._ptr(ws), size.value))
+
+        def call(ws, ws_bytes):
+            return self._L.sc_sample(self._h, sc, dtype, b, v, ld, ln, prm, up, s, u_ld, index.data_ptr(), s,
+                                     kept.data_ptr(), ws, ws_bytes)
+
+        if self._workspace(call(None, 0), lambda: self._sample_bytes(b, v, s)):
+            _check(call(self._ws.data_ptr(), self._ws.numel()))
+            self._ws = None
         return index, kept
+
+    def _sample_bytes(self, b, v, s):
+        size = ctypes.c_size_t()
+        _check(self._L.sc_sample_workspace(b, v, s, size))
+        return size.value
 
     # -- models --------------------------------------------------------------
     def bank(self, weak_classifiers):
