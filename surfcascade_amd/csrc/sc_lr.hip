@@ -30,7 +30,7 @@ namespace sc {
 namespace {
 
 constexpr int kWaves = 4;  // waves per workgroup
-constexpr int kWideWaves = 4;   // ... of the wide form
+constexpr int kWideWaves = 8;   // ... of the wide form (4: 20 % slower on 16 sets of 608 patches)
 constexpr int kNarrowSets = 4;  // parameter sets per learner up to which the narrow form runs
 
 struct F32 {
@@ -49,6 +49,16 @@ typedef unsigned uint4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned uint4_a2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef unsigned uint4_v __attribute__((ext_vector_type(4)));
 typedef _Float16 half2_v __attribute__((ext_vector_type(2)));
+
+typedef float float4_v __attribute__((ext_vector_type(4)));
+typedef float float4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+
+__device__ __forceinline__ void load4(const float *p, bool on, float *to) {  // (0 where not on)
+    float4_v v = {0, 0, 0, 0};
+    if (on) v = *reinterpret_cast<const float4_a4 *>(p);
+#pragma unroll
+    for (int k = 0; k < 4; k++) to[k] = v[k];
+}
 
 template <class T>
 __device__ __forceinline__ uint4_v load16(const char *p) {
@@ -204,7 +214,7 @@ __global__ __launch_bounds__(64 * kWaves) void lr_kernel(LrArgs a) {
         const bool on = learner && h0 + h < a.H;
         const long long mh = (long long)m * a.H + h0 + h;
 #pragma unroll
-        for (int e = 0; e < EPL; e++) w[h][e] = on ? a.w[mh * kDesc + q * EPL + e] : 0.0f;
+        for (int e = 0; e < EPL; e += 4) load4(a.w + mh * kDesc + q * EPL + e, on, w[h] + e);
         bias[h] = on && a.b ? a.b[mh] : 0.0f;
     }
     float acc[H][EPL], sum_g[H], sum_l[H];
@@ -347,7 +357,7 @@ struct WideRow {  // the 8 values of a lane's row: places 8q..8q+7
     uint4_v a;
     __device__ __forceinline__ void load(const char *p) { a = load16<T>(p); }
     __device__ __forceinline__ void values(float *f) const { unpack<T>(a, f); }
-    static __device__ __forceinline__ int place(int q, int k) { return q * 8 + k; }
+    static __device__ __forceinline__ int place(int q, int four) { return q * 8 + four * 4; }  // the first of four
 };
 template <>
 struct WideRow<F32> {  // places 4q..4q+3 and 16+4q..: each load covers half a line of 16 rows
@@ -360,7 +370,7 @@ struct WideRow<F32> {  // places 4q..4q+3 and 16+4q..: each load covers half a l
         unpack<F32>(a, f);
         unpack<F32>(b, f + 4);
     }
-    static __device__ __forceinline__ int place(int q, int k) { return (k & 4) * 4 + q * 4 + (k & 3); }
+    static __device__ __forceinline__ int place(int q, int four) { return four * 16 + q * 4; }
 };
 
 template <class T>
@@ -369,9 +379,6 @@ __device__ __forceinline__ float load_one(const char *p) {
     else if constexpr (__is_same(T, F16)) return (float)*reinterpret_cast<const _Float16 *>(p);
     else return __uint_as_float((unsigned)*reinterpret_cast<const unsigned short *>(p) << 16);
 }
-
-typedef float float4_v __attribute__((ext_vector_type(4)));
-typedef float float4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 
 // what a wave of the wide form works on
 struct WideUnit {
@@ -382,6 +389,7 @@ struct WideUnit {
     // samples in order, 16 of them within 2^31 bytes: one base per tile and
     // per-lane offsets that stay the same
     bool in_order;
+    bool dense;  // ... of dy and dres within 2^31 elements
 };
 
 template <class T>
@@ -395,6 +403,7 @@ __device__ __forceinline__ bool wide_unit(const LrArgs &a, int wave, WideUnit &u
     u.x = static_cast<const char *>(a.x) + (long long)(u.present ? p : 0) * kDesc * T::kSize;
     u.step = a.ld * T::kSize;
     u.in_order = !a.rows && u.step < (1 << 26);
+    u.dense = a.dy_ld < (1 << 26) && a.dres_ld < (1 << 26);
     const long long lo = (long long)blockIdx.y * a.rows_per_wave;
     u.r0 = (int)(lo < a.R ? lo : a.R);
     u.r1 = (int)(lo + a.rows_per_wave < a.R ? lo + a.rows_per_wave : a.R);
@@ -414,8 +423,8 @@ __global__ __launch_bounds__(64 * kWideWaves) void lr_wide_response_kernel(LrArg
     const long long first = (long long)u.m * a.H + u.h0;  // column of the first set
     const int left = a.H - u.h0 - 4 * q;                  // sets from this lane's first on
 #pragma unroll
-    for (int k = 0; k < 8; k++)
-        w[k] = u.h0 + i < a.H ? a.w[(first + i) * kDesc + WideRow<T>::place(q, k)] : 0.0f;
+    for (int k = 0; k < 2; k++)
+        load4(a.w + (first + i) * kDesc + WideRow<T>::place(q, k), u.h0 + i < a.H, w + 4 * k);
 #pragma unroll
     for (int k = 0; k < 4; k++)
         if (a.b && k < left) bias[k] = a.b[first + 4 * q + k];
@@ -542,15 +551,17 @@ struct WideTile {
     float dy[4];                                         // of those rows, set i
     bool whole;                                          // no row of it is absent
 };
+// (a lane's own offsets; everything else of an address is the same in a wave)
 struct WideOffsets {
-    unsigned row, place[4];
+    unsigned row, place, dy, dres;
 };
 template <class T>
-__device__ __forceinline__ WideOffsets wide_offsets(const WideUnit &u, int i, int q) {
+__device__ __forceinline__ WideOffsets wide_offsets(const LrArgs &a, const WideUnit &u, int i, int q, long long col) {
     WideOffsets o;
     o.row = (unsigned)(i * u.step) + q * 16;
-#pragma unroll
-    for (int k = 0; k < 4; k++) o.place[k] = (unsigned)((4 * q + k) * u.step) + 2 * i * T::kSize;
+    o.place = (unsigned)(4 * q * u.step) + 2 * i * T::kSize;
+    o.dy = (unsigned)(4 * q * a.dy_ld + col);
+    o.dres = (unsigned)(4 * q * a.dres_ld + col);
     return o;
 }
 template <class T, int MODE>
@@ -562,7 +573,7 @@ __device__ __forceinline__ void wide_load(const LrArgs &a, const WideUnit &u, co
         const char *base = u.x + r * u.step;
         t.x.load(base + o.row);
 #pragma unroll
-        for (int k = 0; k < 4; k++) t.xc[k] = load_pair<T>(base + o.place[k]);
+        for (int k = 0; k < 4; k++) t.xc[k] = load_pair<T>(base + k * u.step + o.place);
     } else {
         const int j = v.idx < 0 ? 0 : v.idx;
         t.x.load(u.x + j * u.step + q * 16);
@@ -571,18 +582,23 @@ __device__ __forceinline__ void wide_load(const LrArgs &a, const WideUnit &u, co
             t.xc[k] = load_pair<T>(u.x + __shfl(j, q * 4 + k, 64) * u.step + 2 * i * T::kSize);
     }
     if constexpr (MODE == kGrad) {
+        if (u.dense && r + 16 <= u.r1) {
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int row = r + q * 4 + k < u.r1 ? r + q * 4 + k : u.r0;
-            t.dy[k] = a.dy[(long long)row * a.dy_ld + col];
+            for (int k = 0; k < 4; k++) t.dy[k] = (a.dy + (long long)(r + k) * a.dy_ld)[o.dy];
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int row = r + q * 4 + k < u.r1 ? r + q * 4 + k : u.r0;
+                t.dy[k] = a.dy[(long long)row * a.dy_ld + col];
+            }
         }
     }
 }
 
 // g of this lane's four results; clears what an absent row loaded
 template <class T, int MODE>
-__device__ __forceinline__ void wide_grad(const LrArgs &a, const WideUnit &u, WideTile<T> &t, float4_v z, int r, int q,
-                                          bool on, long long col, float (&g)[4], float &sum_g, float &sum_l) {
+__device__ __forceinline__ void wide_grad(const LrArgs &a, const WideUnit &u, const WideOffsets &o, WideTile<T> &t, float4_v z,
+                                          int r, int q, bool on, long long col, float (&g)[4], float &sum_g, float &sum_l) {
     float pos[4], neg[4];
 #pragma unroll
     for (int k = 0; k < 4; k++) {
@@ -592,9 +608,16 @@ __device__ __forceinline__ void wide_grad(const LrArgs &a, const WideUnit &u, Wi
         } else {
             pos[k] = a.alpha * t.dy[k];
             neg[k] = 0.0f;
-            const int row = r + q * 4 + k;
-            if (a.res_kind == SC_RES_FULL && on && row < u.r1)
-                a.dres[(long long)row * a.dres_ld + col] = a.beta * t.dy[k];
+        }
+    }
+    if (MODE == kGrad && a.res_kind == SC_RES_FULL && on) {
+        if (u.dense && r + 16 <= u.r1) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) (a.dres + (long long)(r + k) * a.dres_ld)[o.dres] = a.beta * t.dy[k];
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (r + q * 4 + k < u.r1) a.dres[(long long)(r + q * 4 + k) * a.dres_ld + col] = a.beta * t.dy[k];
         }
     }
     if (t.whole) {
@@ -662,9 +685,9 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void lr_wide_kernel(LrArgs a) {
     const long long col = (long long)u.m * a.H + (on ? u.h0 + i : 0);  // (lanes past the sets read the first one's)
     float w[8];
 #pragma unroll
-    for (int k = 0; k < 8; k++) w[k] = on ? a.w[col * kDesc + WideRow<T>::place(q, k)] : 0.0f;
+    for (int k = 0; k < 2; k++) load4(a.w + col * kDesc + WideRow<T>::place(q, k), on, w + 4 * k);
     const float bias = on && a.b ? a.b[col] : 0.0f;
-    const WideOffsets o = wide_offsets<T>(u, i, q);
+    const WideOffsets o = wide_offsets<T>(a, u, i, q, col);
     float4_v acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
     float sum_g = 0.0f, sum_l = 0.0f;
     auto products = [&](int r, WideTile<T> &t) {
@@ -673,7 +696,7 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void lr_wide_kernel(LrArgs a) {
         float4_v z = {bias, bias, bias, bias};
 #pragma unroll
         for (int k = 0; k < 8; k++) z = __builtin_amdgcn_mfma_f32_16x16x4f32(f[k], w[k], z, 0, 0, 0);
-        wide_grad<T, MODE>(a, u, t, z, r, q, on, col, g, sum_g, sum_l);
+        wide_grad<T, MODE>(a, u, o, t, z, r, q, on, col, g, sum_g, sum_l);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             acc[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(g[k], place_value<T>(t, 0, k), acc[0], 0, 0, 0);
@@ -721,16 +744,19 @@ __global__ __launch_bounds__(64 * kWideWaves) void lr_wide_bf16_kernel(LrArgs a)
     const bool on = u.h0 + i < a.H;
     const long long col = (long long)u.m * a.H + (on ? u.h0 + i : 0);
     uint4_v w[3];
+    float wf[8];
+    load4(a.w + col * kDesc + 8 * q, on, wf);
+    load4(a.w + col * kDesc + 8 * q + 4, on, wf + 4);
 #pragma unroll
     for (int k = 0; k < 4; k++) {
         unsigned lo[3], hi[3];
-        split3(on ? a.w[col * kDesc + 8 * q + 2 * k] : 0.0f, lo[0], lo[1], lo[2]);
-        split3(on ? a.w[col * kDesc + 8 * q + 2 * k + 1] : 0.0f, hi[0], hi[1], hi[2]);
+        split3(wf[2 * k], lo[0], lo[1], lo[2]);
+        split3(wf[2 * k + 1], hi[0], hi[1], hi[2]);
 #pragma unroll
         for (int e = 0; e < 3; e++) w[e][k] = pack(lo[e], hi[e]);
     }
     const float bias = on && a.b ? a.b[col] : 0.0f;
-    const WideOffsets o = wide_offsets<T>(u, i, q);
+    const WideOffsets o = wide_offsets<T>(a, u, i, q, col);
     float4_v acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
     float sum_g = 0.0f, sum_l = 0.0f;
     auto dot = [&](const WideTile<T> &t) {
@@ -745,8 +771,8 @@ __global__ __launch_bounds__(64 * kWideWaves) void lr_wide_bf16_kernel(LrArgs a)
     auto products = [&](int r, WideTile<T> &one, WideTile<T> &two) {
         const float4_v z1 = dot(one), z2 = dot(two);
         float g[2][4];
-        wide_grad<T, MODE>(a, u, one, z1, r, q, on, col, g[0], sum_g, sum_l);
-        wide_grad<T, MODE>(a, u, two, z2, r + 16, q, on, col, g[1], sum_g, sum_l);
+        wide_grad<T, MODE>(a, u, o, one, z1, r, q, on, col, g[0], sum_g, sum_l);
+        wide_grad<T, MODE>(a, u, o, two, z2, r + 16, q, on, col, g[1], sum_g, sum_l);
         uint4_v gs[3], xs[2];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
@@ -788,21 +814,25 @@ __global__ __launch_bounds__(64 * kWideWaves) void lr_wide_bf16_kernel(LrArgs a)
     wide_store<MODE>(a, u, acc, sum_g, sum_l, i, q);
 }
 
-// Joins the row chunks' partial sums: 32 neighbouring words per workgroup, its
-// 8 lane rows each walk every eighth chunk, in 64 bits.  No chunk at all (no
-// rows): zeros.
-__global__ __launch_bounds__(256) void lr_join_kernel(LrArgs a, int loss) {
-    __shared__ double s_sum[8][32];
+// Joins the row chunks' partial sums: 32 neighbouring words per workgroup, each
+// of its SUBS lane rows walks every SUBS-th chunk, in 64 bits.  No chunk at all
+// (no rows): zeros.
+template <int SUBS>
+__global__ __launch_bounds__(32 * SUBS) void lr_join_kernel(LrArgs a, int loss) {
+    __shared__ double s_sum[SUBS][32];
     const long long words = (long long)a.M * a.H * kPartWords;
     const long long i = (long long)blockIdx.x * 32 + (threadIdx.x & 31);
     const int sub = threadIdx.x >> 5;
     double s = 0.0;
-    if (i < words)
-        for (int k = sub; k < a.chunks; k += 8) s += (double)a.part[k * words + i];
+    if (i < words) {
+#pragma unroll 4
+        for (int k = sub; k < a.chunks; k += SUBS) s += (double)a.part[k * words + i];
+    }
     s_sum[sub][threadIdx.x & 31] = s;
     __syncthreads();
     if (sub != 0 || i >= words) return;
-    for (int k = 1; k < 8; k++) s += s_sum[k][threadIdx.x];
+#pragma unroll
+    for (int k = 1; k < SUBS; k++) s += s_sum[k][threadIdx.x];
     const long long mh = i / kPartWords;
     const int word = (int)(i - mh * kPartWords);
     if (word < kDesc) a.dw[mh * kDesc + word] = (float)s;
@@ -862,27 +892,40 @@ void launch_mode(const LrArgs &a, dim3 grid, hipStream_t s) {
 
 }  // namespace
 
-// Gradient and loss: rows are cut into chunks, of one range of rows per wave of
-// a workgroup (narrow form) or one for all of them (wide form).  The grid runs
-// in rounds of as many waves as the registers of 256 CUs hold, so the time is
-// about rounds x (rows per wave + what a wave's start and end cost, some 48
-// rows' time): the number of chunks with the least of that.
+// Gradient and loss: rows are cut into chunks, of `ranges` waves' rows each.
+// The grid runs in rounds of as many waves as the registers of 256 CUs hold
+// (room), so the time is about rounds x (rows per wave + what a wave's start
+// and end cost, some 48 rows' time): the best of 1 to 4 full rounds.
+static int rows_per_wave(long long R, long long waves, int ranges, int step, long long room) {
+    const long long most = ceil_div(R, (long long)ranges * step);
+    long long best = -1;
+    int found = step;
+    for (int rounds = 1; rounds <= 4; rounds++) {
+        long long chunks = rounds * room / waves;
+        chunks = chunks < 1 ? 1 : chunks > most ? most : chunks;
+        const long long rows = ceil_div(ceil_div(R, chunks * ranges), step) * step;
+        const long long cost = ceil_div(waves * ceil_div(R, rows * ranges), room) * (rows + 48);
+        if (best >= 0 && cost >= best) continue;
+        best = cost;
+        found = (int)rows;
+    }
+    return found;
+}
+
+// waves of the narrow form over learners and sets
+static long long narrow_waves(const LrArgs &a) {
+    return ceil_div(a.M, items_per_wave(a)) * ceil_div(a.H, sets_per_wave(a));
+}
+static long long wide_waves(const LrArgs &a) { return a.M * ceil_div(a.H, 16); }
+
 LrPlan lr_plan(const LrArgs &a) {
     LrPlan p{0, 0, 0};
     if (a.R == 0) return p;
-    const int step = wide(a) ? 16 : lanes_per_item(a), ranges = wide(a) ? 1 : kWaves;
-    const long long waves = wide(a) ? a.M * ceil_div(a.H, 16)
-                                    : ceil_div(a.M, items_per_wave(a)) * ceil_div(a.H, sets_per_wave(a)) * kWaves;
-    const long long room = 1024 * (wide(a) || a.H == 2 ? 4 : a.H == 1 ? 6 : 3);
-    const long long most = ceil_div(a.R, (long long)ranges * step);
-    long long best = -1;
-    for (long long chunks = 1; chunks <= most && (chunks == 1 || waves * (chunks - 1) < 4 * room); chunks++) {
-        const long long rows = ceil_div(ceil_div(a.R, chunks * ranges), step) * step;
-        const long long cost = ceil_div(waves * chunks, room) * (rows + 48);
-        if (best >= 0 && cost >= best) continue;
-        best = cost;
-        p.rows_per_wave = (int)rows;
-    }
+    // (a chunk of the narrow form is one range of rows per wave of a workgroup)
+    const int ranges = wide(a) ? 1 : kWaves;
+    p.rows_per_wave = wide(a) ? rows_per_wave(a.R, wide_waves(a), 1, 16, 4096)
+                              : rows_per_wave(a.R, narrow_waves(a) * kWaves, kWaves, lanes_per_item(a),
+                                              1024 * (a.H == 1 ? 6 : a.H == 2 ? 4 : 3));
     p.chunks = (int)ceil_div(a.R, (long long)p.rows_per_wave * ranges);
     if (p.chunks > 1) p.part_bytes = (size_t)p.chunks * a.M * a.H * kPartWords * sizeof(float);
     return p;
@@ -890,16 +933,18 @@ LrPlan lr_plan(const LrArgs &a) {
 
 void launch_lr_response(const LrArgs &a0, hipStream_t s) {
     LrArgs a = a0;
-    const int step = wide(a) ? 16 : lanes_per_item(a);
-    const long long units = wide(a) ? a.M * ceil_div(a.H, 16) : ceil_div(a.M, items_per_wave(a));
-    const int wg = wide(a) ? kWideWaves : kWaves;
-    const long long wgs = ceil_div(units, wg), hs = wide(a) ? 1 : ceil_div(a.H, sets_per_wave(a));
-    // rows per wave: enough waves for the chip, at most 64 rows, at most 65535 chunks
-    long long rows = ceil_div(ceil_div(a.R, ceil_div(8192, wgs * hs * wg)), step) * step;
-    if (rows > 64) rows = 64;
-    const long long least = ceil_div(ceil_div(a.R, 65535), step) * step;
+    const long long waves = wide(a) ? wide_waves(a) : narrow_waves(a);
+    // As few rows as a wave can take: one pass, its loads issued at once (16384 x
+    // 608 f32: 222 us with 8 rows, 235 with 16, 259 with 64).  The wide form
+    // takes 32, for its prefetch, once there are waves enough (2001 x 608 x 16
+    // f16: 59.5 us with 32, 63 with 16, 61 with 160).
+    const long long rows = !wide(a) ? 8 : waves * ceil_div(a.R, 32) < 2048 ? 16 : 32;
+    const long long least = ceil_div(ceil_div(a.R, 65535), wide(a) ? 16 : 8) * (wide(a) ? 16 : 8);  // (grid y)
     a.rows_per_wave = (int)(rows > least ? rows : least);
-    launch_mode<kResponse>(a, dim3((unsigned)wgs, (unsigned)ceil_div(a.R, a.rows_per_wave), (unsigned)hs), s);
+    const dim3 grid = wide(a) ? dim3((unsigned)ceil_div(waves, kWideWaves), (unsigned)ceil_div(a.R, a.rows_per_wave))
+                              : dim3((unsigned)ceil_div(ceil_div(a.M, items_per_wave(a)), kWaves),
+                                     (unsigned)ceil_div(a.R, a.rows_per_wave), (unsigned)ceil_div(a.H, sets_per_wave(a)));
+    launch_mode<kResponse>(a, grid, s);
 }
 
 void launch_lr_grad(const LrArgs &a, bool loss, hipStream_t s) {
@@ -912,7 +957,9 @@ void launch_lr_grad(const LrArgs &a, bool loss, hipStream_t s) {
     }
     if (a.chunks != 1) {
         const long long words = (long long)a.M * a.H * kPartWords;
-        hipLaunchKernelGGL(lr_join_kernel, dim3((unsigned)ceil_div(words, 32)), dim3(256), 0, s, a, loss ? 1 : 0);
+        const dim3 grid((unsigned)ceil_div(words, 32));
+        if (a.chunks > 32) hipLaunchKernelGGL(lr_join_kernel<32>, grid, dim3(1024), 0, s, a, loss ? 1 : 0);
+        else hipLaunchKernelGGL(lr_join_kernel<8>, grid, dim3(256), 0, s, a, loss ? 1 : 0);
     }
 }
 
