@@ -814,11 +814,29 @@ __global__ __launch_bounds__(64 * kWideWaves) void lr_wide_bf16_kernel(LrArgs a)
     wide_store<MODE>(a, u, acc, sum_g, sum_l, i, q);
 }
 
-// Joins the row chunks' partial sums: 32 neighbouring words per workgroup, each
-// of its SUBS lane rows walks every SUBS-th chunk, in 64 bits.  No chunk at all
-// (no rows): zeros.
+// What follows the row chunks, in one launch.  The first `joins` workgroups join
+// their partial sums: 32 neighbouring words each, every lane row of SUBS walks
+// every SUBS-th chunk, in 64 bits (no chunk at all, no rows: zeros).  The others
+// write the gradient of a residual of one value per row, beta * the sum of the
+// row's dy: `lanes` of a wave a row, in 64 bits.
 template <int SUBS>
-__global__ __launch_bounds__(32 * SUBS) void lr_join_kernel(LrArgs a, int loss) {
+__global__ __launch_bounds__(32 * SUBS) void lr_tail_kernel(LrArgs a, int loss, int joins, int lanes) {
+    if ((int)blockIdx.x >= joins) {
+        const long long cols = (long long)a.M * a.H, rows = 32 * SUBS / lanes;
+        const int at = threadIdx.x & (lanes - 1);
+        const long long step = (gridDim.x - joins) * rows;
+        for (long long r0 = (blockIdx.x - joins) * rows; r0 < a.R; r0 += step) {
+            const long long r = r0 + threadIdx.x / lanes;
+            double s = 0.0;
+            if (r < a.R) {
+#pragma unroll 4
+                for (long long c = at; c < cols; c += lanes) s += (double)a.dy[r * a.dy_ld + c];
+            }
+            for (int d = lanes / 2; d; d >>= 1) s += __shfl_xor(s, d, 64);
+            if (r < a.R && at == 0) a.dres[r * a.dres_ld] = (float)((double)a.beta * s);
+        }
+        return;
+    }
     __shared__ double s_sum[SUBS][32];
     const long long words = (long long)a.M * a.H * kPartWords;
     const long long i = (long long)blockIdx.x * 32 + (threadIdx.x & 31);
@@ -838,23 +856,6 @@ __global__ __launch_bounds__(32 * SUBS) void lr_join_kernel(LrArgs a, int loss) 
     if (word < kDesc) a.dw[mh * kDesc + word] = (float)s;
     else if (word == kDesc) a.db[mh] = (float)s;
     else if (loss) a.loss[mh] = (float)s;
-}
-
-// gradient of a residual of one value per row: beta * the sum of the row's dy
-__global__ __launch_bounds__(256) void res_row_kernel(LrArgs a) {
-    __shared__ double s_sum[4];
-    const long long cols = (long long)a.M * a.H;
-    for (long long r = blockIdx.x; r < a.R; r += gridDim.x) {
-        double s = 0.0;
-        for (long long c = threadIdx.x; c < cols; c += 256) s += (double)a.dy[r * a.dy_ld + c];
-#pragma unroll
-        for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d, 64);
-        if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = s;
-        __syncthreads();
-        if (threadIdx.x == 0)
-            a.dres[r * a.dres_ld] = (float)((double)a.beta * (s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]));
-        __syncthreads();
-    }
 }
 
 int items_per_wave(const LrArgs &a) { return a.dtype == SC_F32 ? 8 : 16; }
@@ -897,6 +898,7 @@ void launch_mode(const LrArgs &a, dim3 grid, hipStream_t s) {
 // (room), so the time is about rounds x (rows per wave + what a wave's start
 // and end cost, some 48 rows' time): the best of 1 to 4 full rounds.
 static int rows_per_wave(long long R, long long waves, int ranges, int step, long long room) {
+    if (R <= 16 * ranges) return (int)(ceil_div(ceil_div(R, ranges), step) * step);  // one chunk: nothing to join
     const long long most = ceil_div(R, (long long)ranges * step);
     long long best = -1;
     int found = step;
@@ -920,7 +922,7 @@ static long long wide_waves(const LrArgs &a) { return a.M * ceil_div(a.H, 16); }
 
 LrPlan lr_plan(const LrArgs &a) {
     LrPlan p{0, 0, 0};
-    if (a.R == 0) return p;
+    if (a.R == 0 || a.M == 0 || a.H == 0) return p;
     // (a chunk of the narrow form is one range of rows per wave of a workgroup)
     const int ranges = wide(a) ? 1 : kWaves;
     p.rows_per_wave = wide(a) ? rows_per_wave(a.R, wide_waves(a), 1, 16, 4096)
@@ -955,17 +957,16 @@ void launch_lr_grad(const LrArgs &a, bool loss, hipStream_t s) {
         if (loss) launch_mode<kLoss>(a, grid, s);
         else launch_mode<kGrad>(a, grid, s);
     }
-    if (a.chunks != 1) {
-        const long long words = (long long)a.M * a.H * kPartWords;
-        const dim3 grid((unsigned)ceil_div(words, 32));
-        if (a.chunks > 32) hipLaunchKernelGGL(lr_join_kernel<32>, grid, dim3(1024), 0, s, a, loss ? 1 : 0);
-        else hipLaunchKernelGGL(lr_join_kernel<8>, grid, dim3(256), 0, s, a, loss ? 1 : 0);
-    }
-}
-
-void launch_lr_res_row(const LrArgs &a, hipStream_t s) {
-    if (a.R > 0)
-        hipLaunchKernelGGL(res_row_kernel, dim3((unsigned)(a.R < 8192 ? a.R : 8192)), dim3(256), 0, s, a);
+    const long long words = (long long)a.M * a.H * kPartWords;
+    const int joins = a.chunks == 1 ? 0 : (int)ceil_div(words, 32);
+    // a wave per row, or 16 lanes where rows are short
+    const int lanes = (long long)a.M * a.H > 64 ? 64 : 16, block = a.chunks > 32 ? 1024 : 256;
+    long long sums = !loss && a.res_kind == SC_RES_ROW ? ceil_div(a.R, block / lanes) : 0;
+    if (sums > 4096) sums = 4096;
+    if (joins + sums == 0) return;
+    const dim3 grid((unsigned)(joins + sums));
+    if (block == 1024) hipLaunchKernelGGL(lr_tail_kernel<32>, grid, dim3(block), 0, s, a, loss ? 1 : 0, joins, lanes);
+    else hipLaunchKernelGGL(lr_tail_kernel<8>, grid, dim3(block), 0, s, a, loss ? 1 : 0, joins, lanes);
 }
 
 }  // namespace sc

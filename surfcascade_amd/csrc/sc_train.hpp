@@ -54,8 +54,8 @@ struct LrPlan {
 LrPlan lr_plan(const LrArgs &a);
 
 void launch_lr_response(const LrArgs &a, hipStream_t s);
-void launch_lr_grad(const LrArgs &a, bool loss, hipStream_t s);  // + the join of its chunks
-void launch_lr_res_row(const LrArgs &a, hipStream_t s);  // dres of SC_RES_ROW (SC_RES_FULL's: launch_lr_grad)
+// sums per chunk, their join, and dres
+void launch_lr_grad(const LrArgs &a, bool loss, hipStream_t s);
 
 struct SampleArgs {
     const void *scores;

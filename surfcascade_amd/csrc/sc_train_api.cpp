@@ -318,11 +318,8 @@ int sc_lr_response_grad(sc_trainer *t, const sc_samples *x, const sc_weak_bank *
         a.res_kind = res_kind;
         a.dres = dres;
         a.dres_ld = dres_ld;
-        if (cols > 0) lr_grad(t, a, false, ws, ws_bytes);
-        if (res_kind == SC_RES_ROW) {
-            sc::launch_lr_res_row(a, t->stream);
-            HIPCHK(hipGetLastError());
-        }
+        if (cols == 0 && res_kind != SC_RES_ROW) return SC_OK;
+        lr_grad(t, a, false, ws, ws_bytes);
         return SC_OK;
     });
 }
