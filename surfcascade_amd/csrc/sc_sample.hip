@@ -18,9 +18,9 @@
 // the sum from the top crosses is split again.  Cumulated masses then need one
 // pass in place order, and a draw is a search through them.
 //
-// Rows of up to kRowScores scores: one workgroup each, one launch; a thread
-// holds its keys and masses in registers through all passes.  Longer rows: many
-// workgroups, one launch per pass (below).
+// Short rows: one workgroup each, one launch; a thread holds its keys and masses
+// in registers through all passes.  Long rows: many workgroups, one launch per
+// pass.
 #include <hip/hip_runtime.h>
 
 #include "sc_train.hpp"
@@ -43,52 +43,60 @@ __device__ __forceinline__ float score_of(unsigned key) {
     return __uint_as_float((key & 0x80000000u) ? key ^ 0x80000000u : ~key);
 }
 
-// The keys of K places of a row of n scores (0 past its end): every load is
-// issued before the first is used.
+// The scores of K places of a row of n scores as they lie: only loads, so that
+// other loads can be issued behind them before the first is waited for.
 template <int K, class Place>
-__device__ __forceinline__ void load_keys(const SampleArgs &a, long long base, int n, unsigned (&key)[K], Place place) {
-    if (n == 0) {
+__device__ __forceinline__ void load_raw(const SampleArgs &a, long long base, int n, unsigned (&raw)[K], Place place) {
+    if (n <= 0) {  // nothing to read (there may be no buffer at all)
 #pragma unroll
-        for (int j = 0; j < K; j++) key[j] = 0;
+        for (int j = 0; j < K; j++) raw[j] = 0;
         return;
     }
-    float f[K];
+    const int last = n - 1;
     if (a.dtype == SC_F32) {
-        const float *p = static_cast<const float *>(a.scores) + base;
+        const unsigned *p = static_cast<const unsigned *>(a.scores) + base;
 #pragma unroll
-        for (int j = 0; j < K; j++) f[j] = p[place(j) < n ? place(j) : n - 1];
+        for (int j = 0; j < K; j++) raw[j] = p[place(j) < n ? place(j) : last];
     } else {
         const unsigned short *p = static_cast<const unsigned short *>(a.scores) + base;
-        unsigned short h[K];
 #pragma unroll
-        for (int j = 0; j < K; j++) h[j] = p[place(j) < n ? place(j) : n - 1];
-#pragma unroll
-        for (int j = 0; j < K; j++)
-            f[j] = a.dtype == SC_F16 ? (float)__builtin_bit_cast(_Float16, h[j]) : __uint_as_float((unsigned)h[j] << 16);
+        for (int j = 0; j < K; j++) raw[j] = p[place(j) < n ? place(j) : last];
     }
+}
+// ... and their keys (0 past the row's end)
+template <int K, class Place>
+__device__ __forceinline__ void to_keys(const SampleArgs &a, int n, unsigned (&raw)[K], Place place) {
 #pragma unroll
-    for (int j = 0; j < K; j++) key[j] = place(j) < n ? key_of(f[j]) : 0;
+    for (int j = 0; j < K; j++) {
+        const float f = a.dtype == SC_F32   ? __uint_as_float(raw[j])
+                        : a.dtype == SC_F16 ? (float)__builtin_bit_cast(_Float16, (unsigned short)raw[j])
+                                            : __uint_as_float(raw[j] << 16);
+        raw[j] = place(j) < n ? key_of(f) : 0;
+    }
+}
+template <int K, class Place>
+__device__ __forceinline__ void load_keys(const SampleArgs &a, long long base, int n, unsigned (&key)[K], Place place) {
+    load_raw<K>(a, base, n, key, place);
+    to_keys<K>(a, n, key, place);
 }
 
-// e^x for x <= 0 to 2^-51: x = n ln 2 + r with |r| <= ln 2 / 2, the Taylor
-// series of e^r to r^12 (remainder 0.35^13 / 13! = 2e-16), times 2^n.
+// e^x for x <= 0 to 7e-16: x = n ln 2 + r with |r| <= ln 2 / 2, e^r by its
+// Chebyshev interpolation of degree 10 there (5.9e-16), times 2^n.
 __device__ __forceinline__ double exp_neg(double x) {
     x = x < -800.0 ? -800.0 : x;  // (2^-1154: 0)
     const double n = rint(x * 1.44269504088896340736);
     double r = __builtin_fma(n, -0.693147180559945286227, x);
     r = __builtin_fma(n, -2.319046813846299558e-17, r);
-    double p = 1.0 / 479001600.0;
-    p = __builtin_fma(p, r, 1.0 / 39916800.0);
-    p = __builtin_fma(p, r, 1.0 / 3628800.0);
-    p = __builtin_fma(p, r, 1.0 / 362880.0);
-    p = __builtin_fma(p, r, 1.0 / 40320.0);
-    p = __builtin_fma(p, r, 1.0 / 5040.0);
-    p = __builtin_fma(p, r, 1.0 / 720.0);
-    p = __builtin_fma(p, r, 1.0 / 120.0);
-    p = __builtin_fma(p, r, 1.0 / 24.0);
-    p = __builtin_fma(p, r, 1.0 / 6.0);
-    p = __builtin_fma(p, r, 0.5);
-    p = __builtin_fma(p, r, 1.0);
+    double p = 2.7519707534693554e-07;
+    p = __builtin_fma(p, r, 2.7642139218631665e-06);
+    p = __builtin_fma(p, r, 2.4801790688999252e-05);
+    p = __builtin_fma(p, r, 0.00019841165565505855);
+    p = __builtin_fma(p, r, 0.00138888886671899);
+    p = __builtin_fma(p, r, 0.008333333389376566);
+    p = __builtin_fma(p, r, 0.04166666666755826);
+    p = __builtin_fma(p, r, 0.166666666665438);
+    p = __builtin_fma(p, r, 0.49999999999998807);
+    p = __builtin_fma(p, r, 1.0000000000000075);
     p = __builtin_fma(p, r, 1.0);
     return ldexp(p, (int)n);
 }
@@ -101,7 +109,10 @@ struct Weigh {
         const float s = score_of(key);
         return s == top ? 1.0 : exp_neg(((double)s - (double)top) * rate);  // (also +inf against +inf)
     }
-    __device__ __forceinline__ u64 mass(double w) const { return (u64)rint(w * unit); }
+    // rint(w * unit), at most 2^51: the mantissa of its sum with 2^52
+    __device__ __forceinline__ u64 mass(double w) const {
+        return (u64)__double_as_longlong(__builtin_fma(w, unit, 4503599627370496.0)) & 0xfffffffffffffull;
+    }
 };
 
 // Inclusive sum over the lanes of a wave: DPP shifts by 1, 2, 4 and 8 inside
@@ -157,6 +168,35 @@ __device__ __forceinline__ V block_scan(V x, V *s_wave, V &total) {
         total += v;
     }
     return before + x;
+}
+
+// two of them at once
+template <int N, class V, class W>
+__device__ __forceinline__ void block_scan2(V &x, W &y, V *s_x, W *s_y, V &total_x, W &total_y) {
+    const int wv = threadIdx.x >> 6;
+    x = wave_scan(x);
+    y = wave_scan(y);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) {
+        s_x[wv] = x;
+        s_y[wv] = y;
+    }
+    __syncthreads();
+    V bx = 0;
+    W by = 0;
+    total_x = 0;
+    total_y = 0;
+#pragma unroll
+    for (int k = 0; k < N / 64; k++) {
+        const V vx = s_x[k];
+        const W vy = s_y[k];
+        bx += k < wv ? vx : 0;
+        by += k < wv ? vy : 0;
+        total_x += vx;
+        total_y += vy;
+    }
+    x += bx;
+    y += by;
 }
 
 // smallest and largest key and the count over a workgroup of N threads
@@ -391,7 +431,8 @@ __global__ __launch_bounds__(N) void sample_row_kernel(SampleArgs a) {
 //   draw    : one wave per draw: part, group and place by three searches
 // Bins are shared by atomics on integers, so their order does not matter.
 
-constexpr int kPartThreads = 256;
+constexpr int kPartThreads = 512;  // (256: 10 to 30 % slower to 200 parts; 1024: 50 % slower from 2000)
+constexpr int kDrawThreads = 256;
 constexpr int kGroups = 64;         // groups of 64 f places per part
 constexpr int kMostParts = 1024;    // (a draw's workgroup holds their sums in LDS)
 
@@ -483,50 +524,56 @@ __host__ __device__ inline Split split_of(void *ws, int V, int row) {
 
 struct SplitShared {
     u64 bins[2 * kBins];
-    u64 wave[kPartThreads / 64];
-    u64 found_before, found_in;
+    u64 wave[2][kPartThreads / 64];
+    u64 found_before, found_other;
     int found_bin;
 };
 
-// The bin, from the top, where the running sum of `bin` reaches need (of the
-// whole sum when need is 0 and share >= 0: share of it): *at, and the sum
-// before it.  `other`'s sum before that bin too (NULL: not wanted).
-__device__ void find_bin(SplitShared &s, const u64 *bin, const u64 *other, u64 need, double share,
-                         int &at, u64 &need_out, u64 &before_out, u64 &other_before) {
-    constexpr int kPer = kBins / kPartThreads;
-    u64 v[kPer], o[kPer], sum = 0, osum = 0;
-    const int top = kBins - 1 - (int)threadIdx.x * kPer;  // this thread: bins top, top-1, ... (unused ones are 0)
-#pragma unroll
-    for (int j = 0; j < kPer; j++) {
-        v[j] = bin[top - j];
-        o[j] = other ? other[top - j] : 0;
-        sum += v[j];
-        osum += o[j];
-    }
-    u64 total, ototal = 0;
-    u64 before = block_scan<kPartThreads, u64>(sum, s.wave, total) - sum;
-    u64 obefore = other ? block_scan<kPartThreads, u64>(osum, s.wave, ototal) - osum : 0;
-    if (share >= 0.0) {
-        need = need_of(share, total);
-    }
-    if (before < need && need <= before + sum) {
+// A thread's share of the bins of a level, loaded before the row's state is
+// known: counts or masses `v`, and the masses `o` beside top_k's counts.
+constexpr int kPer = kBins / kPartThreads;
+struct Bins {
+    u64 v[kPer], o[kPer];
+    __device__ __forceinline__ void load(const u64 *bin, const u64 *other) {
+        const int top = kBins - 1 - (int)threadIdx.x * kPer;  // bins top, top-1, ... (unused ones are 0)
 #pragma unroll
         for (int j = 0; j < kPer; j++) {
-            if (before < need && need <= before + v[j]) {
-                s.found_bin = top - j;
+            v[j] = bin[top - j];
+            o[j] = other ? other[top - j] : 0;
+        }
+    }
+};
+
+// The bin, from the top, where the running sum of b.v reaches need (share >= 0:
+// that share of the whole sum), and the sums of b.v and b.o before it.
+__device__ __forceinline__ void find_bin(SplitShared &s, const Bins &b, double share, int &at, u64 &need, u64 &before_out,
+                                         u64 &other_before) {
+    u64 sum = 0, osum = 0;
+#pragma unroll
+    for (int j = 0; j < kPer; j++) {
+        sum += b.v[j];
+        osum += b.o[j];
+    }
+    u64 upto = sum, oupto = osum, total, ototal;
+    block_scan2<kPartThreads, u64, u64>(upto, oupto, s.wave[0], s.wave[1], total, ototal);
+    u64 before = upto - sum, obefore = oupto - osum;
+    if (share >= 0.0) need = need_of(share, total);
+    if (before < need && need <= upto) {
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+            if (before < need && need <= before + b.v[j]) {
+                s.found_bin = kBins - 1 - (int)threadIdx.x * kPer - j;
                 s.found_before = before;
-                s.found_in = obefore;
+                s.found_other = obefore;
             }
-            before += v[j];
-            obefore += o[j];
+            before += b.v[j];
+            obefore += b.o[j];
         }
     }
     __syncthreads();
     at = s.found_bin;
     before_out = s.found_before;
-    other_before = s.found_in;
-    need_out = need;
-    __syncthreads();
+    other_before = s.found_other;
 }
 
 // one level down, into bin `at`
@@ -539,8 +586,8 @@ __device__ __forceinline__ void into_bin(Descent &d, int at, u64 before, u64 abo
     d.shift = d.shift > kBinBits ? d.shift - kBinBits : 0;
 }
 
-// A thread's places of a part: wave w has the groups w, w + 4, ... (64 f places
-// each), one place of 64 neighbouring ones per lane.  All loads of a round are
+// A thread's places of a part: wave w has the groups w, w + 8, ... (64 f
+// places each), one place of 64 neighbouring ones per lane.  All loads of a round are
 // issued before the first is used.
 constexpr int kPartKeys = kGroups * 64 / kPartThreads;
 struct PartKeys {
@@ -551,8 +598,15 @@ struct PartKeys {
     __device__ __forceinline__ int place(int j, int jj) const {
         return i0 + ((j * (kPartThreads / 64) + ((int)threadIdx.x >> 6)) * f + jj) * 64 + ((int)threadIdx.x & 63);
     }
-    __device__ __forceinline__ void load(int jj) {
-        load_keys<kPartKeys>(a, base, n, key, [&](int j) { return place(j, jj); });
+    __device__ __forceinline__ void start(int jj) {
+        load_raw<kPartKeys>(a, base, n, key, [&](int j) { return place(j, jj); });
+    }
+    __device__ __forceinline__ void finish(int jj) {
+        to_keys<kPartKeys>(a, n, key, [&](int j) { return place(j, jj); });
+    }
+    __device__ __forceinline__ void load(int jj) {  // every round after the first
+        start(jj);
+        finish(jj);
     }
 };
 
@@ -593,9 +647,10 @@ __global__ __launch_bounds__(kPartThreads) void sample_step_kernel(SampleArgs a)
     const long long base = row * a.ld;
     const bool use_k = a.top_k > 0 || a.temperature == 0.0, use_p = a.top_p < 1.0;  // (the launches that run)
     PartKeys keys{a, base, part * size, n, w.f, {}};
-    keys.load(0);
+    keys.start(0);
 
     if constexpr (STEP == kExtent) {
+        keys.finish(0);
         const int words = kBinArrays * kBins;
         if (use_k || use_p)
             for (int i = part * kPartThreads + tid; i < words; i += w.parts * kPartThreads) w.bins[i] = 0;
@@ -620,6 +675,15 @@ __global__ __launch_bounds__(kPartThreads) void sample_step_kernel(SampleArgs a)
         return;
     }
 
+    u64 *C1 = w.bins + kC1 * kBins, *M1 = w.bins + kM1 * kBins, *C2 = w.bins + kC2 * kBins, *K2 = w.bins + kK2 * kBins;
+    u64 *C3 = w.bins + kC3 * kBins, *K3 = w.bins + kK3 * kBins, *M2 = w.bins + kM2 * kBins, *M3 = w.bins + kM3 * kBins;
+    Bins bins, bins3;  // of the level before; top_k's last one
+    if (STEP == kK2Step) bins.load(C1, use_p ? M1 : nullptr);
+    if (STEP == kK3Step) bins.load(C2, use_p ? K2 : nullptr);
+    if (STEP == kP2Step) bins.load(M1, nullptr);
+    if (STEP == kP3Step) bins.load(M2, nullptr);
+    if (STEP == kSums && use_p) bins.load(M3, nullptr);
+    if ((STEP == kP2Step || (STEP == kSums && !use_p)) && use_k) bins3.load(C3, use_p ? K3 : nullptr);
     RowState st;
     const int before_sums = use_p ? kP3Step : use_k ? kK3Step : kLevel1;
     if (STEP == kLevel1 || (STEP == kSums && before_sums == kLevel1)) {  // no trim: the sums are the second step
@@ -653,13 +717,10 @@ __global__ __launch_bounds__(kPartThreads) void sample_step_kernel(SampleArgs a)
         copy(st, w.state[STEP == kP2Step ? (use_k ? kK3Step : kLevel1) : STEP == kSums ? before_sums : kBefore]);
     }
     const Weigh wg{score_of(st.kmax), 1.0 / a.temperature, ldexp(1.0, a.shift)};
-    u64 *C1 = w.bins + kC1 * kBins, *M1 = w.bins + kM1 * kBins, *C2 = w.bins + kC2 * kBins, *K2 = w.bins + kK2 * kBins;
-    u64 *C3 = w.bins + kC3 * kBins, *K3 = w.bins + kK3 * kBins, *M2 = w.bins + kM2 * kBins, *M3 = w.bins + kM3 * kBins;
-    auto down = [&](Descent &d, const u64 *bin, const u64 *mass, double share) {
+    auto down = [&](Descent &d, const Bins &b, double share) {
         int at;
-        u64 need, before, above;
-        find_bin(s, bin, mass, d.need, share, at, need, before, above);
-        d.need = need;
+        u64 before, above;
+        find_bin(s, b, share, at, d.need, before, above);
         into_bin(d, at, before, above);
     };
     u64 *counts = nullptr, *masses = nullptr;  // of the window of st.k (of st.p: P2 and P3)
@@ -668,17 +729,17 @@ __global__ __launch_bounds__(kPartThreads) void sample_step_kernel(SampleArgs a)
         masses = st.p.on ? M1 : nullptr;
     }
     if (STEP == kK2Step && st.k.on) {
-        down(st.k, C1, st.p.on ? M1 : nullptr, -1.0);
+        down(st.k, bins, -1.0);
         counts = C2;
         masses = st.p.on ? K2 : nullptr;
     }
     if (STEP == kK3Step && st.k.on && !st.k.done) {
-        down(st.k, C2, st.p.on ? K2 : nullptr, -1.0);
+        down(st.k, bins, -1.0);
         counts = C3;
         masses = st.p.on ? K3 : nullptr;
     }
     if ((STEP == kP2Step || (STEP == kSums && !use_p)) && st.k.on && !st.k.done)
-        down(st.k, C3, st.p.on ? K3 : nullptr, -1.0);
+        down(st.k, bins3, -1.0);
     if (STEP == kP2Step && st.p.on) {
         double share = a.top_p;
         if (st.k.on) {  // of what top_k keeps: every key above its threshold, and its share of the ties
@@ -686,14 +747,15 @@ __global__ __launch_bounds__(kPartThreads) void sample_step_kernel(SampleArgs a)
             st.p.need = need_of(a.top_p, total);
             share = -1.0;
         }
-        down(st.p, M1, nullptr, share);
+        down(st.p, bins, share);
         masses = M2;
     }
     if (STEP == kP3Step && st.p.on && !st.p.done) {
-        down(st.p, M2, nullptr, -1.0);
+        down(st.p, bins, -1.0);
         masses = M3;
     }
-    if (STEP == kSums && st.p.on && !st.p.done) down(st.p, M3, nullptr, -1.0);
+    if (STEP == kSums && st.p.on && !st.p.done) down(st.p, bins, -1.0);
+    keys.finish(0);
     if constexpr (STEP != kSums) {
         if (part == 0 && tid == 0) copy(w.state[STEP], st);
         constexpr bool kOfP = STEP == kP2Step || STEP == kP3Step;
@@ -740,24 +802,49 @@ __global__ __launch_bounds__(kPartThreads) void sample_step_kernel(SampleArgs a)
             part_ties += ties[j];
         }
         unsigned *x = reinterpret_cast<unsigned *>(s.bins);
+        constexpr int kWaves = kPartThreads / 64;
         if (lane == 0) {
-            s.wave[wave] = part_mass;
+            s.wave[0][wave] = part_mass;
             x[wave] = part_kept;
-            x[4 + wave] = part_ties;
+            x[kWaves + wave] = part_ties;
         }
         __syncthreads();
         if (tid == 0) {
-            w.part_mass[part] = s.wave[0] + s.wave[1] + s.wave[2] + s.wave[3];
-            w.part_kept[part] = x[0] + x[1] + x[2] + x[3];
-            w.part_ties[part] = x[4] + x[5] + x[6] + x[7];
+            for (int k = 1; k < kWaves; k++) {
+                part_mass += s.wave[0][k];
+                part_kept += x[k];
+                part_ties += x[kWaves + k];
+            }
+            w.part_mass[part] = part_mass;
+            w.part_kept[part] = part_kept;
+            w.part_ties[part] = part_ties;
         }
     }
 }
 
-__global__ __launch_bounds__(kPartThreads) void sample_draw_kernel(SampleArgs a, int chunks, int draws) {
+// One wave's draw inside a group: its lane's key, the ties and the mass before
+// the group -> the lane of the place, -1 if the target lies behind; `sum` and
+// `before` move past the group.
+__device__ __forceinline__ int draw_lane(unsigned k, unsigned thr, u64 quota, const Weigh &wg, double min_p, u64 target,
+                                         u64 &sum, u64 &before) {
+    const bool tie = k && k == thr;
+    const u64 tied = __ballot(tie);
+    u64 q = 0;
+    if (k > thr || (tie && before + __popcll(tied & ((1ull << (threadIdx.x & 63)) - 1)) < quota)) {
+        const double w = wg.weight(k);
+        if (w >= min_p) q = wg.mass(w);
+    }
+    before += __popcll(tied);
+    const u64 c = sum + wave_scan(q);
+    const u64 hit = __ballot(c > target);
+    sum = lane_of(c, 63);
+    return __ffsll((long long)hit) - 1;
+}
+
+__global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a, int chunks, int draws) {
     __shared__ u64 s_mass[kMostParts];       // cumulated kept mass, by part
     __shared__ unsigned s_ties[kMostParts];  // ties before each part
-    __shared__ u64 s_wave[kPartThreads / 64];
+    __shared__ u64 s_wave[2][kDrawThreads / 64];
     const int row = blockIdx.x / chunks, chunk = blockIdx.x - row * chunks, tid = threadIdx.x;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Split w = split_of(a.ws, a.V, row);
@@ -768,44 +855,42 @@ __global__ __launch_bounds__(kPartThreads) void sample_draw_kernel(SampleArgs a,
     const u64 each = thr ? wg.mass(wg.weight(thr)) : 0;
     int n = a.lens ? a.lens[row] : a.V;
     n = n < 0 ? 0 : n > a.V ? a.V : n;
-    auto kept_ties = [&](u64 before, u64 ties) {
-        const u64 left = before < quota ? quota - before : 0;
-        return left < ties ? left : ties;
-    };
-    u64 total = 0;
+    // cumulated by part: mass above the threshold, and ties, of which the first
+    // `quota` are kept
+    u64 total;
     {
-        constexpr int kPer = kMostParts / kPartThreads;  // parts tid*kPer ..
-        u64 ties[kPer], kept = 0, all_ties = 0, sum = 0;
+        constexpr int kPer = kMostParts / kDrawThreads;  // parts tid*kPer ..
+        u64 mass[kPer], sum = 0, counts = 0;
+        unsigned ties[kPer];
 #pragma unroll
         for (int j = 0; j < kPer; j++) {
             const int p = tid * kPer + j;
-            ties[j] = p < w.parts ? w.part_ties[p] : 0;
-            kept += p < w.parts ? w.part_kept[p] : 0;
-            all_ties += ties[j];
+            const bool in = p < w.parts;
+            mass[j] = in ? w.part_mass[p] : 0;
+            ties[j] = in ? w.part_ties[p] : 0;
+            sum += mass[j];
+            counts += ((u64)ties[j] << 32) + (in ? w.part_kept[p] : 0);  // (both below 2^27)
         }
-        u64 every, every_kept;
-        u64 before = block_scan<kPartThreads, u64>(all_ties, s_wave, every) - all_ties;
-        block_scan<kPartThreads, u64>(kept, s_wave, every_kept);
-        u64 cum[kPer];
+        u64 upto = sum, cupto = counts, every;
+        block_scan2<kDrawThreads, u64, u64>(upto, cupto, s_wave[0], s_wave[1], total, every);
+        upto -= sum;
+        u64 before = (cupto - counts) >> 32;
 #pragma unroll
         for (int j = 0; j < kPer; j++) {
-            const int p = tid * kPer + j;
-            s_ties[p] = (unsigned)before;
-            sum += (p < w.parts ? w.part_mass[p] : 0) + kept_ties(before, ties[j]) * each;
-            cum[j] = sum;
+            s_ties[tid * kPer + j] = (unsigned)before;
+            upto += mass[j];
             before += ties[j];
+            s_mass[tid * kPer + j] = upto + (before < quota ? before : quota) * each;
         }
-        const u64 upto = block_scan<kPartThreads, u64>(sum, s_wave, total) - sum;
-#pragma unroll
-        for (int j = 0; j < kPer; j++) s_mass[tid * kPer + j] = upto + cum[j];
-        if (a.kept && chunk == 0 && tid == 0)
-            a.kept[row] = (int)(every_kept + kept_ties(0, every));
+        const u64 kept = (every >> 32) < quota ? every >> 32 : quota;
+        total += kept * each;
+        if (a.kept && chunk == 0 && tid == 0) a.kept[row] = (int)((every & 0xffffffffu) + kept);
     }
     __syncthreads();
     const long long base = row * a.ld;
     const int size = kGroups * 64 * w.f;
     for (int d = 0; d < draws; d++) {
-        const long long j = ((long long)chunk * draws + d) * (kPartThreads / 64) + wave;
+        const long long j = ((long long)chunk * draws + d) * (kDrawThreads / 64) + wave;
         if (j >= a.S) break;
         int found = -1;
         if (count) {
@@ -816,30 +901,20 @@ __global__ __launch_bounds__(kPartThreads) void sample_draw_kernel(SampleArgs a,
             const int part = l16 * 16 + __ffsll((long long)__ballot(lane < 16 && s_mass[l16 * 16 + (lane & 15)] > target)) - 1;
             u64 sum = part ? s_mass[part - 1] : 0;
             // group
-            const u64 ties = w.group_ties[part * kGroups + lane];
-            u64 before = s_ties[part] + wave_scan(ties) - ties;
-            const u64 upto = sum + wave_scan(w.group_mass[part * kGroups + lane] + kept_ties(before, ties) * each);
+            const unsigned ties = w.group_ties[part * kGroups + lane], ties0 = s_ties[part];
+            const u64 mass = wave_scan(w.group_mass[part * kGroups + lane]), past = ties0 + wave_scan(ties);
+            const u64 upto = sum + mass + ((past < quota ? past : quota) - (ties0 < quota ? ties0 : quota)) * each;
             const int g = __builtin_amdgcn_readfirstlane(__ffsll((long long)__ballot(upto > target)) - 1);
             if (g > 0) sum = lane_of(upto, g - 1);
-            before = lane_of(before, g);
+            u64 before = lane_of(past - ties, g);
             // place
             for (int f = 0; f < w.f && found < 0; f++) {
                 const int i = part * size + (g * w.f + f) * 64 + lane;
                 unsigned key[1];
                 load_keys<1>(a, base, n, key, [&](int) { return i; });
                 const unsigned k = key[0];
-                const bool tie = k && k == thr;
-                const u64 tied = __ballot(tie);
-                u64 q = 0;
-                if (k > thr || (tie && before + __popcll(tied & ((1ull << lane) - 1)) < quota)) {
-                    const double wt = wg.weight(k);
-                    if (wt >= a.min_p) q = wg.mass(wt);
-                }
-                before += __popcll(tied);
-                const u64 c = sum + wave_scan(q);
-                const u64 hit = __ballot(c > target);
-                if (hit) found = part * size + (g * w.f + f) * 64 + __ffsll((long long)hit) - 1;
-                sum = lane_of(c, 63);
+                const int at = draw_lane(k, thr, quota, wg, a.min_p, target, sum, before);
+                if (at >= 0) found = part * size + (g * w.f + f) * 64 + at;
             }
         }
         if (lane == 0) a.index[row * a.index_ld + j] = found;
@@ -853,13 +928,16 @@ void launch_step(const SampleArgs &a, hipStream_t s) {
 
 }  // namespace
 
-// Rows of up to kRowScores scores have one workgroup, whose registers hold
-// them; longer ones are cut over many.
-constexpr int kRowScores = 16384;
+// Rows of up to kRowScores scores have one workgroup, whose registers hold them
+// (one of 20011 in LDS: 28 us against 16 to 19 us over many).  Longer ones are cut
+// over many, at most kSplitRows rows at a time (their workspace).
+constexpr int kRowScores = 8192, kSplitRows = 512;
+
+static bool split(const SampleArgs &a) { return a.V > kRowScores; }
 
 SamplePlan sample_plan(const SampleArgs &a) {
     SamplePlan p{0};
-    if (a.V > kRowScores) p.ws_bytes = split_row_bytes(split_parts(a.V)) * a.B;
+    if (split(a)) p.ws_bytes = split_row_bytes(split_parts(a.V)) * (a.B < kSplitRows ? a.B : kSplitRows);
     return p;
 }
 
@@ -868,16 +946,7 @@ static void launch_row(const SampleArgs &a, hipStream_t s) {
     hipLaunchKernelGGL((sample_row_kernel<N, K>), dim3((unsigned)a.B), dim3(N), 0, s, a);
 }
 
-void launch_sample(const SampleArgs &a, hipStream_t s) {
-    if (a.B == 0) return;
-    if (a.V <= kRowScores) {
-        if (a.V <= 256) launch_row<256, 1>(a, s);
-        else if (a.V <= 1024) launch_row<256, 4>(a, s);
-        else if (a.V <= 4096) launch_row<1024, 4>(a, s);
-        else if (a.V <= 8192) launch_row<1024, 8>(a, s);
-        else launch_row<1024, 16>(a, s);
-        return;
-    }
+static void launch_split(const SampleArgs &a, hipStream_t s) {
     const bool use_k = a.top_k > 0 || a.temperature == 0.0, use_p = a.top_p < 1.0;
     launch_step<kExtent>(a, s);
     if (use_k || use_p) launch_step<kLevel1>(a, s);
@@ -893,9 +962,31 @@ void launch_sample(const SampleArgs &a, hipStream_t s) {
     // draws per wave: one until the chip's 8192 waves are taken, 16 at most
     const long long waves = (long long)a.B * a.S;
     const int draws = waves <= 8192 ? 1 : waves >= 16 * 8192 ? 16 : (int)((waves + 8191) / 8192);
-    const int per = draws * kPartThreads / 64, chunks = a.S > per ? (a.S + per - 1) / per : 1;
-    hipLaunchKernelGGL(sample_draw_kernel, dim3((unsigned)((long long)a.B * chunks)), dim3(kPartThreads), 0, s, a,
+    const int per = draws * kDrawThreads / 64, chunks = a.S > per ? (a.S + per - 1) / per : 1;
+    hipLaunchKernelGGL(sample_draw_kernel, dim3((unsigned)((long long)a.B * chunks)), dim3(kDrawThreads), 0, s, a,
                        chunks, draws);
+}
+
+void launch_sample(const SampleArgs &a, hipStream_t s) {
+    if (a.B == 0) return;
+    if (split(a)) {
+        const int elem = a.dtype == SC_F32 ? 4 : 2;
+        for (int r = 0; r < a.B; r += kSplitRows) {
+            SampleArgs b = a;
+            b.B = a.B - r < kSplitRows ? a.B - r : kSplitRows;
+            b.scores = static_cast<const char *>(a.scores) + r * a.ld * elem;
+            if (a.lens) b.lens = a.lens + r;
+            b.u = a.u + r * a.u_ld;
+            b.index = a.index + r * a.index_ld;
+            if (a.kept) b.kept = a.kept + r;
+            launch_split(b, s);
+        }
+        return;
+    }
+    if (a.V <= 256) launch_row<256, 1>(a, s);
+    else if (a.V <= 1024) launch_row<1024, 1>(a, s);
+    else if (a.V <= 4096) launch_row<1024, 4>(a, s);
+    else launch_row<1024, 8>(a, s);
 }
 
 }  // namespace sc

@@ -84,11 +84,11 @@ constexpr int kMaxPool = 1 << 26;
 
 // Masses are 64-bit integers, so that sums do not depend on their order: a
 // weight w in [0, 1] is rint(w * 2^shift), the largest shift with which V
-// weights of 1 stay below 2^62 (52 at most: a double's mantissa).
+// weights of 1 stay below 2^62 (51 at most: a double's mantissa).
 inline int sample_shift(int V) {
     int lg = 0;
     while ((1 << lg) < V) lg++;
-    return 62 - lg < 52 ? 62 - lg : 52;
+    return 62 - lg < 51 ? 62 - lg : 51;
 }
 
 void launch_sample(const SampleArgs &a, hipStream_t s);
