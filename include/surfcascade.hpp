@@ -309,6 +309,46 @@ class Miner {
     std::unique_ptr<sc_detector, Free> det_;
 };
 
+// What CascadeClassifier::Train does between mining rounds (sc_trainer_*,
+// sc_lr_*, sc_sample), on device memory: the responses of weak learners, their
+// gradient, the logistic loss and the roulette wheel.  Calls are asynchronous on
+// the trainer's stream; workspaces are the trainer's own.
+class Trainer {
+   public:
+    explicit Trainer(int device = 0) {
+        sc_trainer *t = nullptr;
+        check(sc_trainer_create(device, &t));
+        t_.reset(t);
+    }
+    void Response(const sc_samples &x, const sc_weak_bank &k, float *y, int64_t y_ld, int act = SC_ACT_SIGMOID,
+                  float alpha = 1.0f, const float *res = nullptr, int res_kind = SC_RES_NONE, int64_t res_ld = 0,
+                  float beta = 1.0f) {
+        check(sc_lr_response(t_.get(), &x, &k, act, alpha, res, res_kind, res_ld, beta, y, y_ld));
+    }
+    void ResponseGrad(const sc_samples &x, const sc_weak_bank &k, const float *dy, int64_t dy_ld, float *dw, float *db,
+                      int act = SC_ACT_SIGMOID, float alpha = 1.0f, int res_kind = SC_RES_NONE, float beta = 1.0f,
+                      float *dres = nullptr, int64_t dres_ld = 0) {
+        check(sc_lr_response_grad(t_.get(), &x, &k, act, alpha, dy, dy_ld, dw, db, res_kind, beta, dres, dres_ld,
+                                  nullptr, 0));
+    }
+    void Loss(const sc_samples &x, const sc_weak_bank &k, const float *target, const float *weight, float *loss,
+              float *dw, float *db) {
+        check(sc_lr_loss(t_.get(), &x, &k, target, weight, loss, dw, db, nullptr, 0));
+    }
+    void Sample(const void *scores, int dtype, int b, int v, int64_t ld, const double *u, int s, int32_t *index,
+                int32_t *kept = nullptr, const int32_t *lens = nullptr, const sc_sample_params *prm = nullptr) {
+        check(sc_sample(t_.get(), scores, dtype, b, v, ld, lens, prm, u, s, s, index, s, kept, nullptr, 0));
+    }
+    void Synchronize() { check(sc_trainer_synchronize(t_.get())); }
+    sc_trainer *handle() const { return t_.get(); }
+
+   private:
+    struct Free {
+        void operator()(sc_trainer *t) const { sc_trainer_destroy(t); }
+    };
+    std::unique_ptr<sc_trainer, Free> t_;
+};
+
 }  // namespace surfcascade
 
 #endif  // SURFCASCADE_HPP

@@ -8,16 +8,32 @@
 //   gradient   : g = alpha * dy * act'(z); dw = sum_r g x, db = sum_r g
 //   loss       : L = sum_r c (softplus(z) - t z), g = c (sigmoid(z) - t)
 // A (row, patch) descriptor is 128 B (64 B in 16 bits) that feeds 64 flops per
-// parameter set, so each is read once and everything else is done on it in
-// registers.  All sums are in 32 bits; the chunks of a gradient are joined in
-// 64 bits in a fixed order (no atomics: the same call gives the same bits).
+// parameter set (128 with its gradient), so up to 16 sets the matrix' own bytes
+// are the bound: each descriptor is read once from memory and everything is done
+// on it in registers.  Sums over rows are in 32 bits within a chunk of them; the
+// chunks are joined in 64 bits in a fixed order (no atomics: the same call gives
+// the same bits).
 //
-// Narrow form (this file's lr_kernel): one descriptor on LPI = 8 lanes (4 in
-// 16 bits), 16 B each, so a wave's load is 8 (16) neighbouring descriptors of
-// one row = 1 KB in one piece.  A wave keeps its learners' weights in
-// registers and walks rows, LPI of them at a time: the LPI x LPI partial dots
-// are summed by a butterfly that also transposes, leaving lane q with row q's
-// dot, so the sigmoid runs once per result on full lanes.
+// Up to kNarrowSets sets, the narrow form: one descriptor on LPI = 8 lanes (4 in
+// 16 bits), 16 B each, so a wave's load is 8 (16) neighbouring descriptors of one
+// row = 1 KB in one piece.  A wave keeps its learners' weights in registers and
+// walks rows, LPI of them at a time: the LPI x LPI partial dots are summed by a
+// butterfly that also transposes, leaving lane q with row q's dot, so the sigmoid
+// runs once per result on full lanes; a gradient spreads g back over the lanes.
+// More sets: the matrix cores (below), whose time hardly depends on their number
+// up to 16.  The borders, on 8191 x 608: responses of f32 with 5 sets 153 us
+// narrow and 205 wide (with 7 275: its stores are not whole 16-B pieces), with 8
+// sets 191 and 182; the gradient with 4 sets 150 us
+// narrow, with 5 241 and 206 wide; the loss with 5 sets 184 and 208 in f32, 155
+// and 130 in bf16.
+//
+// Measured (one MI355X; a 2 GiB copy moves 4.9 TB/s there, reads and writes):
+//   responses, 16384 x 608, f32, 1 set          221 us, 5.9 TB/s
+//   loss and gradient, 16384 x 608, f32, 1 set  219 us, 5.8 TB/s
+//   responses, 2001 x 608, f16, 16 sets          60 us, 3.5 TB/s
+//   loss and gradient, 8191 x 608, bf16, 16 sets 131 us, 2.5 TB/s (VALU: the
+//     sigmoid, its loss and the operand splits of 80 M results)
+//   gradient, 480 x 11870, bf16, 8 sets, dres   199 us, 3.8 TB/s
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -31,7 +47,8 @@ namespace {
 
 constexpr int kWaves = 4;  // waves per workgroup
 constexpr int kWideWaves = 8;   // ... of the wide form (4: 20 % slower on 16 sets of 608 patches)
-constexpr int kNarrowSets = 4;  // parameter sets per learner up to which the narrow form runs
+// parameter sets per learner up to which the narrow form runs
+constexpr int kNarrowSets = 4, kNarrowResponse = 7;
 
 struct F32 {
     static constexpr int kSize = 4;
@@ -197,7 +214,6 @@ __global__ __launch_bounds__(64 * kWaves) void lr_kernel(LrArgs a) {
     // learners for a gradient (joined in LDS below)
     const int mt = MODE == kResponse ? blockIdx.x * kWaves + wave : blockIdx.x;
     const int range = MODE == kResponse ? blockIdx.y : blockIdx.y * kWaves + wave;
-    const int h0 = blockIdx.z * H;
     const int m = mt * IPW + item;
     const bool learner = m < a.M;
     int p = 0;
@@ -211,8 +227,8 @@ __global__ __launch_bounds__(64 * kWaves) void lr_kernel(LrArgs a) {
     float w[H][EPL], bias[H];
 #pragma unroll
     for (int h = 0; h < H; h++) {
-        const bool on = learner && h0 + h < a.H;
-        const long long mh = (long long)m * a.H + h0 + h;
+        const bool on = learner && h < a.H;
+        const long long mh = (long long)m * a.H + h;
 #pragma unroll
         for (int e = 0; e < EPL; e += 4) load4(a.w + mh * kDesc + q * EPL + e, on, w[h] + e);
         bias[h] = on && a.b ? a.b[mh] : 0.0f;
@@ -274,8 +290,8 @@ __global__ __launch_bounds__(64 * kWaves) void lr_kernel(LrArgs a) {
             if (learner && rq < r1) {
 #pragma unroll
                 for (int h = 0; h < H; h++) {
-                    if (h0 + h >= a.H) break;
-                    const long long col = (long long)m * a.H + h0 + h;
+                    if (h >= a.H) break;
+                    const long long col = (long long)m * a.H + h;
                     float v = 0.0f;  // an absent row or patch has no response
                     if (idx >= 0 && present) v = a.alpha * (a.act == SC_ACT_SIGMOID ? sigmoid(z[h]) : z[h]);
                     if (a.res_kind == SC_RES_ROW) v += a.beta * a.res[(long long)rq * a.res_ld];
@@ -288,16 +304,14 @@ __global__ __launch_bounds__(64 * kWaves) void lr_kernel(LrArgs a) {
             for (int h = 0; h < H; h++) {
                 float g = 0.0f;
                 if constexpr (MODE == kGrad) {
-                    if (learner && rq < r1 && h0 + h < a.H) {
-                        const long long col = (long long)m * a.H + h0 + h;
+                    if (learner && rq < r1 && h < a.H) {
+                        const long long col = (long long)m * a.H + h;
                         const float dy = a.dy[(long long)rq * a.dy_ld + col];
                         pos = a.alpha * dy;
                         if (a.res_kind == SC_RES_FULL) a.dres[(long long)rq * a.dres_ld + col] = a.beta * dy;
                     }
                 }
-                if (idx >= 0 && present && h0 + h < a.H) {
-                    g = grad_of<MODE>(a.act, z[h], pos, neg, sum_l[h]);
-                }
+                if (idx >= 0 && present && h < a.H) g = grad_of<MODE>(a.act, z[h], pos, neg, sum_l[h]);
                 sum_g[h] += g;
                 spread_rows<LPI>(g, q, g_all[h]);
             }
@@ -329,9 +343,9 @@ __global__ __launch_bounds__(64 * kWaves) void lr_kernel(LrArgs a) {
 #pragma unroll
             for (int k = 1; k < kWaves; k++) s += s_acc[k][v][lane];
             const int h = v / (EPL + 2), e = v - h * (EPL + 2);
-            if (h0 + h >= a.H || (e >= EPL && q != 0)) continue;
+            if (h >= a.H || (e >= EPL && q != 0)) continue;
             if (e < EPL && !present) s = 0.0f;  // (0 * NaN of the patch read in its place)
-            const long long mh = (long long)m * a.H + h0 + h;
+            const long long mh = (long long)m * a.H + h;
             const int word = e < EPL ? q * EPL + e : kDesc + (e - EPL);
             if (a.part) a.part[((long long)blockIdx.y * a.M * a.H + mh) * kPartWords + word] = s;
             else if (word < kDesc) a.dw[mh * kDesc + word] = s;
@@ -372,13 +386,6 @@ struct WideRow<F32> {  // places 4q..4q+3 and 16+4q..: each load covers half a l
     }
     static __device__ __forceinline__ int place(int q, int four) { return four * 16 + q * 4; }
 };
-
-template <class T>
-__device__ __forceinline__ float load_one(const char *p) {
-    if constexpr (__is_same(T, F32)) return *reinterpret_cast<const float *>(p);
-    else if constexpr (__is_same(T, F16)) return (float)*reinterpret_cast<const _Float16 *>(p);
-    else return __uint_as_float((unsigned)*reinterpret_cast<const unsigned short *>(p) << 16);
-}
 
 // what a wave of the wide form works on
 struct WideUnit {
@@ -546,10 +553,10 @@ __device__ __forceinline__ PlacePair<T> load_pair(const char *p) {
 template <class T>
 struct WideTile {
     WideMeta v;
-    WideRow<T> x;                                        // row i
+    WideRow<T> x;        // row i
     PlacePair<T> xc[4];  // rows 4q .. 4q+3, places 2i and 2i+1
-    float dy[4];                                         // of those rows, set i
-    bool whole;                                          // no row of it is absent
+    float dy[4];         // of those rows, set i
+    bool whole;          // no row of it is absent
 };
 // (a lane's own offsets; everything else of an address is the same in a wave)
 struct WideOffsets {
@@ -669,8 +676,7 @@ __device__ __forceinline__ void wide_store(const LrArgs &a, const WideUnit &u, c
 template <class T>
 __device__ __forceinline__ float place_value(const WideTile<T> &t, int half, int k) {
     if constexpr (__is_same(T, F32)) return t.xc[k][half];
-    else if constexpr (__is_same(T, F16)) return (float)__builtin_bit_cast(half2_v, t.xc[k])[half];
-    else return __uint_as_float(half ? t.xc[k] & 0xffff0000u : t.xc[k] << 16);
+    else return (float)__builtin_bit_cast(half2_v, t.xc[k])[half];
 }
 
 // Gradient and loss, f32 products (16x16x4: nothing is rounded that the narrow
@@ -860,25 +866,28 @@ __global__ __launch_bounds__(32 * SUBS) void lr_tail_kernel(LrArgs a, int loss, 
 
 int items_per_wave(const LrArgs &a) { return a.dtype == SC_F32 ? 8 : 16; }
 int lanes_per_item(const LrArgs &a) { return a.dtype == SC_F32 ? 8 : 4; }
-int sets_per_wave(const LrArgs &a) { return a.H == 1 ? 1 : a.H == 2 ? 2 : 4; }
 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
 bool wide(const LrArgs &a) { return a.H > kNarrowSets; }
+bool wide_response(const LrArgs &a) { return a.H > kNarrowResponse; }
 
 template <class T, int MODE>
 void launch_form(const LrArgs &a, dim3 grid, hipStream_t s) {
-    if (wide(a)) {
+    if (MODE == kResponse ? wide_response(a) : wide(a)) {
         constexpr dim3 block(64 * kWideWaves);
         if constexpr (MODE == kResponse) hipLaunchKernelGGL((lr_wide_response_kernel<T>), grid, block, 0, s, a);
         else if constexpr (__is_same(T, BF16)) hipLaunchKernelGGL((lr_wide_bf16_kernel<MODE>), grid, block, 0, s, a);
         else hipLaunchKernelGGL((lr_wide_kernel<T, MODE>), grid, block, 0, s, a);
         return;
     }
-    switch (sets_per_wave(a)) {
-        case 1: hipLaunchKernelGGL((lr_kernel<T, 1, MODE>), grid, dim3(64 * kWaves), 0, s, a); break;
-        case 2: hipLaunchKernelGGL((lr_kernel<T, 2, MODE>), grid, dim3(64 * kWaves), 0, s, a); break;
-        default: hipLaunchKernelGGL((lr_kernel<T, 4, MODE>), grid, dim3(64 * kWaves), 0, s, a); break;
+    const dim3 block(64 * kWaves);
+    if (a.H == 1) hipLaunchKernelGGL((lr_kernel<T, 1, MODE>), grid, block, 0, s, a);
+    else if (a.H == 2) hipLaunchKernelGGL((lr_kernel<T, 2, MODE>), grid, block, 0, s, a);
+    else if (a.H <= 4) hipLaunchKernelGGL((lr_kernel<T, 4, MODE>), grid, block, 0, s, a);
+    else if constexpr (MODE == kResponse) {
+        if (a.H <= 6) hipLaunchKernelGGL((lr_kernel<T, 6, MODE>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((lr_kernel<T, 8, MODE>), grid, block, 0, s, a);
     }
 }
 
@@ -914,10 +923,8 @@ static int rows_per_wave(long long R, long long waves, int ranges, int step, lon
     return found;
 }
 
-// waves of the narrow form over learners and sets
-static long long narrow_waves(const LrArgs &a) {
-    return ceil_div(a.M, items_per_wave(a)) * ceil_div(a.H, sets_per_wave(a));
-}
+// waves over the learners (and sets, which the narrow form has all in one)
+static long long narrow_waves(const LrArgs &a) { return ceil_div(a.M, items_per_wave(a)); }
 static long long wide_waves(const LrArgs &a) { return a.M * ceil_div(a.H, 16); }
 
 LrPlan lr_plan(const LrArgs &a) {
@@ -935,25 +942,23 @@ LrPlan lr_plan(const LrArgs &a) {
 
 void launch_lr_response(const LrArgs &a0, hipStream_t s) {
     LrArgs a = a0;
-    const long long waves = wide(a) ? wide_waves(a) : narrow_waves(a);
+    const long long waves = wide_response(a) ? wide_waves(a) : narrow_waves(a);
     // As few rows as a wave can take: one pass, its loads issued at once (16384 x
     // 608 f32: 222 us with 8 rows, 235 with 16, 259 with 64).  The wide form
     // takes 32, for its prefetch, once there are waves enough (2001 x 608 x 16
     // f16: 59.5 us with 32, 63 with 16, 61 with 160).
-    const long long rows = !wide(a) ? 8 : waves * ceil_div(a.R, 32) < 2048 ? 16 : 32;
-    const long long least = ceil_div(ceil_div(a.R, 65535), wide(a) ? 16 : 8) * (wide(a) ? 16 : 8);  // (grid y)
+    const long long rows = !wide_response(a) ? 8 : waves * ceil_div(a.R, 32) < 2048 ? 16 : 32;
+    const long long least = ceil_div(ceil_div(a.R, 65535), wide_response(a) ? 16 : 8) * (wide_response(a) ? 16 : 8);  // (grid y)
     a.rows_per_wave = (int)(rows > least ? rows : least);
-    const dim3 grid = wide(a) ? dim3((unsigned)ceil_div(waves, kWideWaves), (unsigned)ceil_div(a.R, a.rows_per_wave))
-                              : dim3((unsigned)ceil_div(ceil_div(a.M, items_per_wave(a)), kWaves),
-                                     (unsigned)ceil_div(a.R, a.rows_per_wave), (unsigned)ceil_div(a.H, sets_per_wave(a)));
+    const dim3 grid = wide_response(a) ? dim3((unsigned)ceil_div(waves, kWideWaves), (unsigned)ceil_div(a.R, a.rows_per_wave))
+                              : dim3((unsigned)ceil_div(waves, kWaves), (unsigned)ceil_div(a.R, a.rows_per_wave));
     launch_mode<kResponse>(a, grid, s);
 }
 
 void launch_lr_grad(const LrArgs &a, bool loss, hipStream_t s) {
     if (a.chunks > 0) {
-        const dim3 grid = wide(a) ? dim3((unsigned)ceil_div(a.M * ceil_div(a.H, 16), kWideWaves), (unsigned)a.chunks)
-                                  : dim3((unsigned)ceil_div(a.M, items_per_wave(a)), (unsigned)a.chunks,
-                                         (unsigned)ceil_div(a.H, sets_per_wave(a)));
+        const dim3 grid = wide(a) ? dim3((unsigned)ceil_div(wide_waves(a), kWideWaves), (unsigned)a.chunks)
+                                  : dim3((unsigned)narrow_waves(a), (unsigned)a.chunks);
         if (loss) launch_mode<kLoss>(a, grid, s);
         else launch_mode<kGrad>(a, grid, s);
     }

@@ -26,8 +26,8 @@ struct sc_trainer {
         int before = 0;
         (void)hipGetDevice(&before);
         (void)hipSetDevice(device);
+        // (a caller's stream is not touched: freeing waits for the device)
         if (own_stream) (void)hipStreamSynchronize(own_stream);
-        if (stream != own_stream) (void)hipStreamSynchronize(stream);
         ws.release();
         if (event) (void)hipEventDestroy(event);
         if (own_stream) (void)hipStreamDestroy(own_stream);

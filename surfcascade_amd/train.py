@@ -249,7 +249,10 @@ class Trainer:
         ln = None if lens is None else self._need(lens, self._i32, (b,), "lens") or None
         index = u.new_empty(shape, dtype=self._i32)
         kept = index.new_empty((b,))
-        prm = _SampleParams(temperature, top_k, top_p, min_p)
+        most = 2**31 - 1  # (a C int; the library refuses rows that long, and such a top_k keeps all)
+        prm = _SampleParams(temperature, min(top_k, most), top_p, min_p)
+        if v > most or s > most or b > most:
+            raise ValueError("more than 2^31 - 1 rows, scores or draws")
 
         def call(ws, ws_bytes):
             return self._L.sc_sample(self._h, sc, dtype, b, v, ld, ln, prm, up, s, u_ld, index.data_ptr(), s,

@@ -96,7 +96,8 @@ SHAPES = [  # n, p, m, h (0: w is [m, 32]), rows, picked
     (1, 1, 1, 0, 0, False), (1, 608, 608, 0, 0, False), (7, 5, 5, 1, 0, False), (8, 9, 9, 2, 0, False),
     (9, 17, 33, 3, 0, True), (65, 16, 16, 4, 0, False), (64, 31, 31, 5, 100, False), (130, 40, 7, 8, 0, True),
     (33, 12, 12, 16, 33, False), (50, 10, 3, 17, 0, True), (20, 6, 6, 33, 41, False), (259, 64, 64, 0, 1, False),
-    (1000, 20, 20, 0, 0, False),
+    (1000, 20, 20, 0, 0, False), (40, 9, 9, 6, 0, False), (70, 21, 21, 7, 50, False), (48, 5, 5, 9, 0, False),
+    (17, 4, 4, 15, 0, False), (129, 3, 11, 20, 64, True),
 ]
 
 
@@ -215,7 +216,7 @@ def test_loss_without_weights_or_bias(tr):
     _check_sums((dw, db), gr, eg, ref, 77)
 
 
-@pytest.mark.parametrize("dtype,h", [("f32", 1), ("bf16", 1), ("f16", 8), ("bf16", 16)])
+@pytest.mark.parametrize("dtype,h", [("f32", 1), ("bf16", 1), ("f16", 8), ("bf16", 16), ("bf16", 3), ("f32", 16)])
 def test_loss_many_rows(tr, dtype, h):
     """Rows cut into chunks on the grid: the join of their partial sums.
     Random signs: the sums' own rounding stays far below the worst case of
@@ -230,6 +231,30 @@ def test_loss_many_rows(tr, dtype, h):
     loss, dw, db = tr.loss(_dev(x), _dev(w), _dev(t), _dev(b), weight=_dev(c))
     _near(loss, term.sum(0), et.sum(0) + 2048 * U * term.sum(0), "loss")
     _check_sums((dw, db), gr, eg, ref, 2048)
+
+
+def _one_hot(n, p, places):
+    x = torch.zeros(n, p, 32)
+    x[torch.arange(n), :, places] = 1.0
+    return x
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("h", [1, 2, 4, 7, 8, 16])
+def test_places_and_sets_are_not_mixed(tr, h, dtype):
+    """Descriptors of a single 1: every response is one weight, every gradient
+    one row's sum, exactly."""
+    n, p = 64, 6
+    places = torch.arange(n) % 32
+    x = _one_hot(n, p, places).to(DT[dtype])
+    w = torch.randn(p, h, 32, generator=_rng(31))
+    y = tr.response(x.cuda(), w.cuda(), activation="none").cpu()
+    assert torch.equal(y, w[:, :, places].permute(2, 0, 1))
+    dy = torch.randn(n, p, h, generator=_rng(32))
+    dw, db, _ = tr.response_grad(x.cuda(), w.cuda(), dy.cuda(), activation="none")
+    want = dy[:32].double() + dy[32:].double()  # rows k and 32 + k have place k
+    _near(dw, want.permute(1, 2, 0), 2 * U * (dy[:32].abs() + dy[32:].abs()).double().permute(1, 2, 0), "dw")
+    _near(db, dy.double().sum(0), 64 * U * dy.double().abs().sum(0), "db")
 
 
 @pytest.mark.parametrize("h", [0, 2, 8])
