@@ -199,6 +199,13 @@ __device__ __forceinline__ void block_scan2(V &x, W &y, V *s_x, W *s_y, V &total
     y += by;
 }
 
+__device__ __forceinline__ void extend(unsigned k, unsigned &lo, unsigned &hi, unsigned &c) {
+    if (!k) return;
+    lo = k < lo ? k : lo;
+    hi = k > hi ? k : hi;
+    c++;
+}
+
 // smallest and largest key and the count over a workgroup of N threads
 template <int N>
 __device__ __forceinline__ void block_extent(unsigned &lo, unsigned &hi, unsigned &c, unsigned *s_x) {
@@ -292,42 +299,18 @@ __device__ void descend(RowShared<N> &s, unsigned kmin, unsigned kmax, u64 need,
     }
 }
 
-// N threads, each with K neighbouring places: keys and masses in registers,
-// the keys in LDS too for the draws.
+// A row's kept places from its n keys in s_key (N K of them in place order, 0:
+// absent), and the draws.  Thread t has the K neighbouring ones from t K on, keys
+// and masses in registers.  top_k: still to be applied (0: no).  s_place: the
+// keys' places, where the keys are not all of the row's (NULL: their order).
 template <int N, int K>
-__global__ __launch_bounds__(N) void sample_row_kernel(SampleArgs a) {
-    __shared__ RowShared<N> s;
-    __shared__ unsigned s_key[N * K];
-    const int row = blockIdx.x, tid = threadIdx.x;
-    int n = a.lens ? a.lens[row] : a.V;
-    n = n < 0 ? 0 : n > a.V ? a.V : n;
-    const long long base = row * a.ld;
-    int *index = a.index + row * a.index_ld;
-    // neighbouring lanes load neighbouring places; the keys change owners in LDS
-    {
-        unsigned k[K];
-        load_keys<K>(a, base, n, k, [&](int j) { return j * N + tid; });
-#pragma unroll
-        for (int j = 0; j < K; j++) s_key[j * N + tid] = k[j];
-    }
-    __syncthreads();
+__device__ __forceinline__ void finish_row(const SampleArgs &a, int row, RowShared<N> &s, const unsigned *s_key,
+                                           const unsigned short *s_place, unsigned kmin, unsigned kmax, unsigned count,
+                                           int top_k) {
+    const int tid = threadIdx.x;
     unsigned key[K];
-    unsigned kmin = 0xffffffffu, kmax = 0, count = 0;
 #pragma unroll
-    for (int j = 0; j < K; j++) {
-        key[j] = s_key[tid * K + j];
-        if (key[j]) {
-            kmin = key[j] < kmin ? key[j] : kmin;
-            kmax = key[j] > kmax ? key[j] : kmax;
-            count++;
-        }
-    }
-    block_extent<N>(kmin, kmax, count, s.x);
-    if (count == 0) {  // nothing to draw from
-        for (int j = tid; j < a.S; j += N) index[j] = -1;
-        if (a.kept && tid == 0) a.kept[row] = 0;
-        return;
-    }
+    for (int j = 0; j < K; j++) key[j] = s_key[tid * K + j];
     const Weigh wg{score_of(kmax), 1.0 / a.temperature, ldexp(1.0, a.shift)};
     u64 mass[K];
     unsigned low = 0;  // places under min_p
@@ -337,8 +320,6 @@ __global__ __launch_bounds__(N) void sample_row_kernel(SampleArgs a) {
         mass[j] = wg.mass(w);
         low |= (unsigned)(w < a.min_p) << j;
     }
-
-    const int top_k = a.temperature == 0.0 ? 1 : a.top_k;  // temperature 0: the best place
     unsigned thr = 0;   // places with a larger key are kept,
     u64 quota = ~0ull;  // and this many of those with this key
     if (top_k > 0 && (unsigned)top_k < count)
@@ -374,7 +355,7 @@ __global__ __launch_bounds__(N) void sample_row_kernel(SampleArgs a) {
 #pragma unroll
         for (int j = 0; j < K; j++) ties += key[j] == thr;
         unsigned every;
-        ties = block_scan<N, unsigned>(ties, reinterpret_cast<unsigned *>(s.wave), every) - ties;
+        ties = block_scan<N, unsigned>(ties, s.x, every) - ties;
     }
     const unsigned ties_before = ties;
     u64 sum = 0;
@@ -389,10 +370,8 @@ __global__ __launch_bounds__(N) void sample_row_kernel(SampleArgs a) {
     }
     unsigned kept_all;
     u64 all;
-    __syncthreads();
-    block_scan<N, unsigned>(kept, s.x, kept_all);
-    const u64 upto = block_scan<N, u64>(sum, s.wave, all);
-    s.bins[tid] = upto;
+    block_scan2<N, u64, unsigned>(sum, kept, s.wave, s.x, all, kept_all);
+    s.bins[tid] = sum;
     s.ties[tid] = ties_before;
     __syncthreads();
     if (a.kept && tid == 0) a.kept[row] = (int)kept_all;
@@ -413,8 +392,112 @@ __global__ __launch_bounds__(N) void sample_row_kernel(SampleArgs a) {
             c += wg.mass(w);
             if (c > target) found = at * K + i;
         }
-        index[j] = found;
+        a.index[row * a.index_ld + j] = found >= 0 && s_place ? s_place[found] : found;
     }
+}
+
+// nothing to draw from
+template <int N>
+__device__ __forceinline__ void empty_row(const SampleArgs &a, int row) {
+    for (int j = threadIdx.x; j < a.S; j += N) a.index[row * a.index_ld + j] = -1;
+    if (a.kept && threadIdx.x == 0) a.kept[row] = 0;
+}
+
+__device__ __forceinline__ int row_length(const SampleArgs &a, int row) {
+    const int n = a.lens ? a.lens[row] : a.V;
+    return n < 0 ? 0 : n > a.V ? a.V : n;
+}
+
+template <int N, int K>
+__global__ __launch_bounds__(N) void sample_row_kernel(SampleArgs a) {
+    __shared__ RowShared<N> s;
+    __shared__ unsigned s_key[N * K];
+    const int row = blockIdx.x, tid = threadIdx.x, n = row_length(a, row);
+    // neighbouring lanes load neighbouring places; the keys change owners in LDS
+    unsigned key[K];
+    unsigned kmin = 0xffffffffu, kmax = 0, count = 0;
+    load_keys<K>(a, row * a.ld, n, key, [&](int j) { return j * N + tid; });
+#pragma unroll
+    for (int j = 0; j < K; j++) {
+        s_key[j * N + tid] = key[j];
+        extend(key[j], kmin, kmax, count);
+    }
+    block_extent<N>(kmin, kmax, count, s.x);
+    if (count == 0) return empty_row<N>(a, row);
+    finish_row<N, K>(a, row, s, s_key, nullptr, kmin, kmax, count, a.temperature == 0.0 ? 1 : a.top_k);
+}
+
+// ---- longer rows of which top_k keeps few ----------------------------------------
+//
+// One workgroup: the row's keys in registers, K a thread, for top_k's descent;
+// what it keeps, at most kTrimKept, moves into LDS in place order, and all that
+// needs weights runs on that.
+
+constexpr int kTrimThreads = 1024, kTrimOwn = 8, kTrimKept = kTrimThreads * kTrimOwn;
+
+template <int K>
+__global__ __launch_bounds__(kTrimThreads) void sample_trim_kernel(SampleArgs a) {
+    constexpr int N = kTrimThreads, kWaves = N / 64;
+    __shared__ RowShared<N> s;
+    __shared__ unsigned s_key[kTrimKept];
+    __shared__ unsigned short s_place[kTrimKept];
+    __shared__ unsigned s_above[K * kWaves], s_tied[K * kWaves];  // of 64 neighbouring places, then before them
+    const int row = blockIdx.x, tid = threadIdx.x, n = row_length(a, row);
+    unsigned key[K];
+    unsigned kmin = 0xffffffffu, kmax = 0, count = 0;
+    load_keys<K>(a, row * a.ld, n, key, [&](int j) { return j * N + tid; });
+#pragma unroll
+    for (int j = 0; j < K; j++) extend(key[j], kmin, kmax, count);
+    block_extent<N>(kmin, kmax, count, s.x);
+    if (count == 0) return empty_row<N>(a, row);
+    const int top_k = a.temperature == 0.0 ? 1 : a.top_k;  // 1 .. kTrimKept
+    unsigned thr = 0;
+    u64 quota = 0;
+    if ((unsigned)top_k < count)
+        descend<N>(s, kmin, kmax, (u64)top_k, 0.0,
+            [&](unsigned lo, int shift, unsigned bins) {
+#pragma unroll
+                for (int j = 0; j < K; j++)
+                    if (key[j] && key[j] >= lo && ((key[j] - lo) >> shift) < bins)
+                        atomicAdd(&s.bins[(key[j] - lo) >> shift], 1ull);
+            },
+            thr, quota);
+    const u64 below = (1ull << (tid & 63)) - 1;
+    const int wave = tid >> 6;
+#pragma unroll
+    for (int j = 0; j < K; j++) {
+        const u64 above = __ballot(key[j] > thr), tied = __ballot(key[j] && key[j] == thr);
+        if ((tid & 63) == 0) {
+            s_above[j * kWaves + wave] = __popcll(above);
+            s_tied[j * kWaves + wave] = __popcll(tied);
+        }
+    }
+    for (int i = tid; i < kTrimKept; i += N) s_key[i] = 0;
+    __syncthreads();
+    const bool mine = tid < K * kWaves;
+    const unsigned above = mine ? s_above[tid] : 0, tied = mine ? s_tied[tid] : 0;
+    unsigned past_above = above, past_tied = tied, every, ties;
+    block_scan2<N, unsigned, unsigned>(past_above, past_tied, s.x, s.x + kWaves, every, ties);
+    if (mine) {
+        s_above[tid] = past_above - above;
+        s_tied[tid] = past_tied - tied;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < K; j++) {
+        const u64 tied_here = __ballot(key[j] && key[j] == thr);
+        const u64 before = s_tied[j * kWaves + wave];
+        const bool in = key[j] > thr || (key[j] && key[j] == thr && before + __popcll(tied_here & below) < quota);
+        const u64 kept = __ballot(in);
+        if (in) {
+            const unsigned to = s_above[j * kWaves + wave] + (unsigned)(before < quota ? before : quota) +
+                                (unsigned)__popcll(kept & below);
+            s_key[to] = key[j];
+            s_place[to] = (unsigned short)(j * N + tid);
+        }
+    }
+    __syncthreads();
+    finish_row<N, kTrimOwn>(a, row, s, s_key, s_place, thr ? thr : kmin, kmax, count, 0);
 }
 
 // ---- long rows: many workgroups per row ------------------------------------
@@ -641,8 +724,7 @@ __global__ __launch_bounds__(kPartThreads) void sample_step_kernel(SampleArgs a)
     const int all = split_parts(a.V);
     const int row = blockIdx.x / all, part = blockIdx.x - row * all, tid = threadIdx.x;
     const Split w = split_of(a.ws, a.V, row);
-    int n = a.lens ? a.lens[row] : a.V;
-    n = n < 0 ? 0 : n > a.V ? a.V : n;
+    const int n = row_length(a, row);
     const int size = kGroups * 64 * w.f;
     const long long base = row * a.ld;
     const bool use_k = a.top_k > 0 || a.temperature == 0.0, use_p = a.top_p < 1.0;  // (the launches that run)
@@ -658,13 +740,7 @@ __global__ __launch_bounds__(kPartThreads) void sample_step_kernel(SampleArgs a)
         for (int jj = 0; jj < w.f; jj++) {
             if (jj) keys.load(jj);
 #pragma unroll
-            for (int j = 0; j < kPartKeys; j++) {
-                const unsigned k = keys.key[j];
-                if (!k) continue;
-                lo = k < lo ? k : lo;
-                hi = k > hi ? k : hi;
-                c++;
-            }
+            for (int j = 0; j < kPartKeys; j++) extend(keys.key[j], lo, hi, c);
         }
         block_extent<kPartThreads>(lo, hi, c, reinterpret_cast<unsigned *>(s.bins));
         if (tid == 0) {
@@ -853,8 +929,7 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a,
     const u64 quota = st.quota;
     const Weigh wg{score_of(st.kmax), 1.0 / a.temperature, ldexp(1.0, a.shift)};
     const u64 each = thr ? wg.mass(wg.weight(thr)) : 0;
-    int n = a.lens ? a.lens[row] : a.V;
-    n = n < 0 ? 0 : n > a.V ? a.V : n;
+    const int n = row_length(a, row);
     // cumulated by part: mass above the threshold, and ties, of which the first
     // `quota` are kept
     u64 total;
@@ -929,11 +1004,14 @@ void launch_step(const SampleArgs &a, hipStream_t s) {
 }  // namespace
 
 // Rows of up to kRowScores scores have one workgroup, whose registers hold them
-// (one of 20011 in LDS: 28 us against 16 to 19 us over many).  Longer ones are cut
-// over many, at most kSplitRows rows at a time (their workspace).
-constexpr int kRowScores = 8192, kSplitRows = 512;
+// all the way; up to kTrimScores, if top_k keeps few, one that trims them first.
+// The rest are cut over many, at most kSplitRows rows at a time (their workspace).
+constexpr int kRowScores = 8192, kTrimScores = 32768, kSplitRows = 512;
 
-static bool split(const SampleArgs &a) { return a.V > kRowScores; }
+static bool trim(const SampleArgs &a) {
+    return a.V <= kTrimScores && (a.temperature == 0.0 || (a.top_k > 0 && a.top_k <= kTrimKept));
+}
+static bool split(const SampleArgs &a) { return a.V > kRowScores && !trim(a); }
 
 SamplePlan sample_plan(const SampleArgs &a) {
     SamplePlan p{0};
@@ -986,7 +1064,9 @@ void launch_sample(const SampleArgs &a, hipStream_t s) {
     if (a.V <= 256) launch_row<256, 1>(a, s);
     else if (a.V <= 1024) launch_row<1024, 1>(a, s);
     else if (a.V <= 4096) launch_row<1024, 4>(a, s);
-    else launch_row<1024, 8>(a, s);
+    else if (a.V <= kRowScores) launch_row<1024, 8>(a, s);
+    else if (a.V <= kTrimScores / 2) hipLaunchKernelGGL(sample_trim_kernel<16>, dim3((unsigned)a.B), dim3(kTrimThreads), 0, s, a);
+    else hipLaunchKernelGGL(sample_trim_kernel<32>, dim3((unsigned)a.B), dim3(kTrimThreads), 0, s, a);
 }
 
 }  // namespace sc

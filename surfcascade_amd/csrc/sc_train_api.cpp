@@ -363,6 +363,8 @@ int sc_sample_workspace(int b, int v, int s, size_t *bytes) {
         a.B = b;
         a.V = v;
         a.S = s;
+        a.temperature = 1.0;  // (no trim: the most any parameters need)
+        a.top_p = 1.0;
         *bytes = sc::sample_plan(a).ws_bytes;
         return SC_OK;
     });

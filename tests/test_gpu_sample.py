@@ -174,6 +174,22 @@ def test_large_pool(tr):
         _check(tr, scores, u, **trim)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("v", [8193, 16384, 16385, 30000, 32768])
+def test_long_rows_trimmed_first(tr, v, dtype):
+    """Rows of which top_k keeps few, up to the border and past it."""
+    scores, u = _inputs(3, v, 300, v, dtype)
+    scores[1, ::3] = -float("inf")
+    lens = torch.tensor([v, v - 5, 8100], dtype=torch.int32)
+    for k in (1, 2, 63, 8191, 8192, 8193):
+        _check(tr, scores, u, top_k=k)
+        _check(tr, scores, u, lens=lens, top_k=k, top_p=0.9, min_p=1e-3, temperature=1.5)
+    equal = torch.full((1, v), 0.5).to(DT[dtype])
+    for k in (5, 8192):
+        _check(tr, equal, u[:1], top_k=k)
+        _check(tr, equal, u[:1], top_k=k, top_p=0.5)
+
+
 def test_larger_pools_and_many_rows(tr):
     """Past 2^22 scores a part's groups grow; past 128 rows each row has one
     workgroup again, however long it is."""
