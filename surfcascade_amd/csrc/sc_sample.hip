@@ -44,9 +44,11 @@ __device__ __forceinline__ float score_of(unsigned key) {
 }
 
 // The scores of K places of a row of n scores as they lie: only loads, so that
-// other loads can be issued behind them before the first is waited for.
+// other loads can be issued behind them before the first is waited for.  Slots
+// from `used` on (the same number in every thread) lie past the row's end.
 template <int K, class Place>
-__device__ __forceinline__ void load_raw(const SampleArgs &a, long long base, int n, unsigned (&raw)[K], Place place) {
+__device__ __forceinline__ void load_raw(const SampleArgs &a, long long base, int n, unsigned (&raw)[K], Place place,
+                                         int used = K) {
     if (n <= 0) {  // nothing to read (there may be no buffer at all)
 #pragma unroll
         for (int j = 0; j < K; j++) raw[j] = 0;
@@ -56,11 +58,11 @@ __device__ __forceinline__ void load_raw(const SampleArgs &a, long long base, in
     if (a.dtype == SC_F32) {
         const unsigned *p = static_cast<const unsigned *>(a.scores) + base;
 #pragma unroll
-        for (int j = 0; j < K; j++) raw[j] = p[place(j) < n ? place(j) : last];
+        for (int j = 0; j < K; j++) raw[j] = j < used ? p[place(j) < n ? place(j) : last] : 0;
     } else {
         const unsigned short *p = static_cast<const unsigned short *>(a.scores) + base;
 #pragma unroll
-        for (int j = 0; j < K; j++) raw[j] = p[place(j) < n ? place(j) : last];
+        for (int j = 0; j < K; j++) raw[j] = j < used ? p[place(j) < n ? place(j) : last] : 0;
     }
 }
 // ... and their keys (0 past the row's end)
@@ -75,8 +77,9 @@ __device__ __forceinline__ void to_keys(const SampleArgs &a, int n, unsigned (&r
     }
 }
 template <int K, class Place>
-__device__ __forceinline__ void load_keys(const SampleArgs &a, long long base, int n, unsigned (&key)[K], Place place) {
-    load_raw<K>(a, base, n, key, place);
+__device__ __forceinline__ void load_keys(const SampleArgs &a, long long base, int n, unsigned (&key)[K], Place place,
+                                          int used = K) {
+    load_raw<K>(a, base, n, key, place, used);
     to_keys<K>(a, n, key, place);
 }
 
@@ -257,26 +260,27 @@ struct RowShared {
 
 // Radix descent: the largest key at which the pool's sum from the top reaches
 // need (need = 0: share of the whole), and what its ties still have to bring.
-// fill(lo, shift, bins) adds what every pool member with a key in
+// fill(bin, lo, shift, bins) adds what every pool member with a key in
 // [lo, lo + (bins << shift)) counts for to bins[(key - lo) >> shift]: the whole
 // pool first, then the one bin where the sum crosses.
-template <int N, class Fill>
-__device__ void descend(RowShared<N> &s, unsigned kmin, unsigned kmax, u64 need, double share, Fill fill,
-                        unsigned &key, u64 &left) {
+template <int N, class Bin, class Fill>
+__device__ __forceinline__ void descend(RowShared<N> &s, unsigned kmin, unsigned kmax, u64 need, double share, Fill fill,
+                                        unsigned &key, u64 &left) {
     constexpr int kPer = kBins / N;
     int shift = 0;
     while (((kmax - kmin) >> shift) >= kBins) shift++;
     unsigned lo = kmin, bins = kBins;
     for (;;) {
-        for (int i = threadIdx.x; i < kBins; i += N) s.bins[i] = 0;
+        Bin *bin = reinterpret_cast<Bin *>(s.bins);
+        for (int i = threadIdx.x; i < kBins; i += N) bin[i] = 0;
         __syncthreads();
-        fill(lo, shift, bins);
+        fill(bin, lo, shift, bins);
         __syncthreads();
         const int top = kBins - 1 - kPer * (int)threadIdx.x;  // this thread: bins top, top-1, ...
-        u64 v[kPer], sum = 0, total;
+        Bin v[kPer], sum = 0, total;
 #pragma unroll
-        for (int j = 0; j < kPer; j++) sum += v[j] = s.bins[top - j];
-        u64 before = block_scan<N, u64>(sum, s.wave, total) - sum;
+        for (int j = 0; j < kPer; j++) sum += v[j] = bin[top - j];
+        u64 before = block_scan<N, Bin>(sum, reinterpret_cast<Bin *>(s.wave), total) - sum;
         if (need == 0) need = need_of(share, total);
         if (before < need && need <= before + sum) {
 #pragma unroll
@@ -300,22 +304,24 @@ __device__ void descend(RowShared<N> &s, unsigned kmin, unsigned kmax, u64 need,
 }
 
 // A row's kept places from its n keys in s_key (N K of them in place order, 0:
-// absent), and the draws.  Thread t has the K neighbouring ones from t K on, keys
-// and masses in registers.  top_k: still to be applied (0: no).  s_place: the
+// absent), and the draws.  Thread t has the `own` <= K neighbouring ones from
+// t own on (as few as hold them all), keys and masses in registers.  top_k: still to be applied (0: no).  s_place: the
 // keys' places, where the keys are not all of the row's (NULL: their order).
 template <int N, int K>
 __device__ __forceinline__ void finish_row(const SampleArgs &a, int row, RowShared<N> &s, const unsigned *s_key,
-                                           const unsigned short *s_place, unsigned kmin, unsigned kmax, unsigned count,
-                                           int top_k) {
+                                           const unsigned short *s_place, int own, unsigned kmin, unsigned kmax,
+                                           unsigned count, int top_k) {
     const int tid = threadIdx.x;
     unsigned key[K];
 #pragma unroll
-    for (int j = 0; j < K; j++) key[j] = s_key[tid * K + j];
+    for (int j = 0; j < K; j++) key[j] = j < own ? s_key[tid * own + j] : 0;
     const Weigh wg{score_of(kmax), 1.0 / a.temperature, ldexp(1.0, a.shift)};
     u64 mass[K];
     unsigned low = 0;  // places under min_p
 #pragma unroll
     for (int j = 0; j < K; j++) {
+        mass[j] = 0;
+        if (j >= own) continue;
         const double w = key[j] ? wg.weight(key[j]) : 0.0;
         mass[j] = wg.mass(w);
         low |= (unsigned)(w < a.min_p) << j;
@@ -323,26 +329,26 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, int row, RowShar
     unsigned thr = 0;   // places with a larger key are kept,
     u64 quota = ~0ull;  // and this many of those with this key
     if (top_k > 0 && (unsigned)top_k < count)
-        descend<N>(s, kmin, kmax, (u64)top_k, 0.0,
-            [&](unsigned lo, int shift, unsigned bins) {
+        descend<N, unsigned>(s, kmin, kmax, (u64)top_k, 0.0,
+            [&](unsigned *bin, unsigned lo, int shift, unsigned bins) {
 #pragma unroll
                 for (int j = 0; j < K; j++)
                     if (key[j] && key[j] >= lo && ((key[j] - lo) >> shift) < bins)
-                        atomicAdd(&s.bins[(key[j] - lo) >> shift], 1ull);
+                        atomicAdd(&bin[(key[j] - lo) >> shift], 1u);
             },
             thr, quota);
     if (a.top_p < 1.0) {
         const unsigned thr_k = thr;
         const u64 quota_k = quota;
         u64 left;
-        descend<N>(s, kmin, kmax, 0, a.top_p,
-            [&](unsigned lo, int shift, unsigned bins) {
+        descend<N, u64>(s, kmin, kmax, 0, a.top_p,
+            [&](u64 *bin, unsigned lo, int shift, unsigned bins) {
 #pragma unroll
                 for (int j = 0; j < K; j++)
                     if (key[j] > thr_k && key[j] >= lo && ((key[j] - lo) >> shift) < bins)
-                        atomicAdd(&s.bins[(key[j] - lo) >> shift], mass[j]);
+                        atomicAdd(&bin[(key[j] - lo) >> shift], mass[j]);
                 if (tid == 0 && thr_k && thr_k >= lo && ((thr_k - lo) >> shift) < bins)  // the ties top_k keeps
-                    atomicAdd(&s.bins[(thr_k - lo) >> shift], quota_k * wg.mass(wg.weight(thr_k)));
+                    atomicAdd(&bin[(thr_k - lo) >> shift], quota_k * wg.mass(wg.weight(thr_k)));
             },
             thr, left);
         const u64 each = wg.mass(wg.weight(thr));
@@ -385,12 +391,13 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, int row, RowShar
         int found = -1;
 #pragma unroll
         for (int i = 0; i < K; i++) {
-            const unsigned k = s_key[at * K + i];
+            if (i >= own) break;
+            const unsigned k = s_key[at * own + i];
             if (found >= 0 || !k || k < thr || (k == thr && tie++ >= quota)) continue;
             const double w = wg.weight(k);
             if (w < a.min_p) continue;
             c += wg.mass(w);
-            if (c > target) found = at * K + i;
+            if (c > target) found = at * own + i;
         }
         a.index[row * a.index_ld + j] = found >= 0 && s_place ? s_place[found] : found;
     }
@@ -416,7 +423,8 @@ __global__ __launch_bounds__(N) void sample_row_kernel(SampleArgs a) {
     // neighbouring lanes load neighbouring places; the keys change owners in LDS
     unsigned key[K];
     unsigned kmin = 0xffffffffu, kmax = 0, count = 0;
-    load_keys<K>(a, row * a.ld, n, key, [&](int j) { return j * N + tid; });
+    const int own = (n + N - 1) / N;
+    load_keys<K>(a, row * a.ld, n, key, [&](int j) { return j * N + tid; }, own);
 #pragma unroll
     for (int j = 0; j < K; j++) {
         s_key[j * N + tid] = key[j];
@@ -424,7 +432,7 @@ __global__ __launch_bounds__(N) void sample_row_kernel(SampleArgs a) {
     }
     block_extent<N>(kmin, kmax, count, s.x);
     if (count == 0) return empty_row<N>(a, row);
-    finish_row<N, K>(a, row, s, s_key, nullptr, kmin, kmax, count, a.temperature == 0.0 ? 1 : a.top_k);
+    finish_row<N, K>(a, row, s, s_key, nullptr, own, kmin, kmax, count, a.temperature == 0.0 ? 1 : a.top_k);
 }
 
 // ---- longer rows of which top_k keeps few ----------------------------------------
@@ -445,7 +453,8 @@ __global__ __launch_bounds__(kTrimThreads) void sample_trim_kernel(SampleArgs a)
     const int row = blockIdx.x, tid = threadIdx.x, n = row_length(a, row);
     unsigned key[K];
     unsigned kmin = 0xffffffffu, kmax = 0, count = 0;
-    load_keys<K>(a, row * a.ld, n, key, [&](int j) { return j * N + tid; });
+    const int steps = (n + N - 1) / N;
+    load_keys<K>(a, row * a.ld, n, key, [&](int j) { return j * N + tid; }, steps);
 #pragma unroll
     for (int j = 0; j < K; j++) extend(key[j], kmin, kmax, count);
     block_extent<N>(kmin, kmax, count, s.x);
@@ -454,12 +463,12 @@ __global__ __launch_bounds__(kTrimThreads) void sample_trim_kernel(SampleArgs a)
     unsigned thr = 0;
     u64 quota = 0;
     if ((unsigned)top_k < count)
-        descend<N>(s, kmin, kmax, (u64)top_k, 0.0,
-            [&](unsigned lo, int shift, unsigned bins) {
+        descend<N, unsigned>(s, kmin, kmax, (u64)top_k, 0.0,
+            [&](unsigned *bin, unsigned lo, int shift, unsigned bins) {
 #pragma unroll
                 for (int j = 0; j < K; j++)
-                    if (key[j] && key[j] >= lo && ((key[j] - lo) >> shift) < bins)
-                        atomicAdd(&s.bins[(key[j] - lo) >> shift], 1ull);
+                    if (j < steps && key[j] && key[j] >= lo && ((key[j] - lo) >> shift) < bins)
+                        atomicAdd(&bin[(key[j] - lo) >> shift], 1u);
             },
             thr, quota);
     const u64 below = (1ull << (tid & 63)) - 1;
@@ -497,7 +506,8 @@ __global__ __launch_bounds__(kTrimThreads) void sample_trim_kernel(SampleArgs a)
         }
     }
     __syncthreads();
-    finish_row<N, kTrimOwn>(a, row, s, s_key, s_place, thr ? thr : kmin, kmax, count, 0);
+    const int kept = (unsigned)top_k < count ? top_k : (int)count;
+    finish_row<N, kTrimOwn>(a, row, s, s_key, s_place, (kept + N - 1) / N, thr ? thr : kmin, kmax, count, 0);
 }
 
 // ---- long rows: many workgroups per row ------------------------------------
