@@ -248,59 +248,116 @@ __device__ __forceinline__ u64 need_of(double share, u64 total) {  // at least 1
 
 // ---- rows for one workgroup -----------------------------------------------------
 
+constexpr int kRanked = 128;  // as many keys are ranked at once
+
 template <int N>
 struct RowShared {
-    u64 bins[kBins];     // (later: cumulated masses of the threads' places)
-    unsigned ties[N];    // ties before each thread's places
+    u64 bins[kBins];   // (later: cumulated masses of the threads' places)
+    unsigned ties[N];  // ties before each thread's places
     u64 wave[N / 64];
     unsigned x[3 * (N / 64)];
-    unsigned key;        // what a descent found
+    u64 list_v[N];  // the members of one bin
+    unsigned list_k[N], listed;
+    unsigned key;      // what a descent found
     u64 left;
 };
 
+// One level of a descent: the bin of [lo, lo + (kBins << shift)) where the sum of
+// each()'s members from the top reaches need -> its first key and what is still
+// needed from it.  each(f) calls f(k, v) for every member's key and what it
+// counts for.
+template <int N, class Bin, class Each>
+__device__ __forceinline__ void level(RowShared<N> &s, unsigned lo, int shift, unsigned bins, u64 &need, double share,
+                                      unsigned &key, Each each) {
+    constexpr int kPer = kBins / N;
+    Bin *bin = reinterpret_cast<Bin *>(s.bins);
+    for (int i = threadIdx.x; i < kBins; i += N) bin[i] = 0;
+    if (threadIdx.x == 0) s.listed = 0;
+    __syncthreads();
+    each([&](unsigned k, Bin v) {
+        if (k >= lo && ((k - lo) >> shift) < bins) atomicAdd(&bin[(k - lo) >> shift], v);
+    });
+    __syncthreads();
+    const int top = kBins - 1 - kPer * (int)threadIdx.x;  // this thread: bins top, top-1, ...
+    Bin v[kPer], sum = 0, total;
+#pragma unroll
+    for (int j = 0; j < kPer; j++) sum += v[j] = bin[top - j];
+    u64 before = block_scan<N, Bin>(sum, reinterpret_cast<Bin *>(s.wave), total) - sum;
+    if (need == 0) need = need_of(share, total);
+    if (before < need && need <= before + sum) {
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+            if (before < need && need <= before + v[j]) {
+                s.key = lo + ((unsigned)(top - j) << shift);
+                s.left = need - before;
+            }
+            before += v[j];
+        }
+    }
+    __syncthreads();
+    key = s.key;
+    need = s.left;
+}
+
 // Radix descent: the largest key at which the pool's sum from the top reaches
 // need (need = 0: share of the whole), and what its ties still have to bring.
-// fill(bin, lo, shift, bins) adds what every pool member with a key in
-// [lo, lo + (bins << shift)) counts for to bins[(key - lo) >> shift]: the whole
-// pool first, then the one bin where the sum crosses.
-template <int N, class Bin, class Fill>
-__device__ __forceinline__ void descend(RowShared<N> &s, unsigned kmin, unsigned kmax, u64 need, double share, Fill fill,
+// The bin where the sum crosses is listed if that may fit (one member per
+// thread), and the next levels run on the list; up to kRanked members are ranked
+// at once, each one's sum of larger keys against need.
+template <int N, class Bin, class Each>
+__device__ __forceinline__ void descend(RowShared<N> &s, unsigned kmin, unsigned kmax, u64 need, double share, Each each,
                                         unsigned &key, u64 &left) {
-    constexpr int kPer = kBins / N;
     int shift = 0;
     while (((kmax - kmin) >> shift) >= kBins) shift++;
-    unsigned lo = kmin, bins = kBins;
+    unsigned lo = kmin, bins = kBins, listed = N + 1, mine = 0;
+    u64 value = 0;
     for (;;) {
-        Bin *bin = reinterpret_cast<Bin *>(s.bins);
-        for (int i = threadIdx.x; i < kBins; i += N) bin[i] = 0;
-        __syncthreads();
-        fill(bin, lo, shift, bins);
-        __syncthreads();
-        const int top = kBins - 1 - kPer * (int)threadIdx.x;  // this thread: bins top, top-1, ...
-        Bin v[kPer], sum = 0, total;
-#pragma unroll
-        for (int j = 0; j < kPer; j++) sum += v[j] = bin[top - j];
-        u64 before = block_scan<N, Bin>(sum, reinterpret_cast<Bin *>(s.wave), total) - sum;
-        if (need == 0) need = need_of(share, total);
-        if (before < need && need <= before + sum) {
-#pragma unroll
-            for (int j = 0; j < kPer; j++) {
-                if (before < need && need <= before + v[j]) {
-                    s.key = lo + ((unsigned)(top - j) << shift);
-                    s.left = need - before;
+        if (listed > N)
+            level<N, Bin>(s, lo, shift, bins, need, share, key, each);
+        else
+            level<N, Bin>(s, lo, shift, bins, need, share, key, [&](auto f) {
+                if (mine) f(mine, (Bin)value);
+            });
+        if (shift == 0) break;
+        lo = key;
+        if (listed > N) {
+            each([&](unsigned k, Bin v) {
+                if (k < lo || ((k - lo) >> shift)) return;
+                const unsigned at = atomicAdd(&s.listed, 1u);
+                if (at >= N) return;
+                s.list_k[at] = k;
+                s.list_v[at] = v;
+            });
+            __syncthreads();
+            listed = s.listed;
+            if (listed <= N && threadIdx.x < listed) {
+                mine = s.list_k[threadIdx.x];
+                value = s.list_v[threadIdx.x];
+            }
+            if (listed <= kRanked) {
+                if (mine) {
+                    u64 above = 0, with = 0;
+                    for (unsigned i = 0; i < listed; i++) {
+                        const unsigned k = s.list_k[i];
+                        const u64 w = s.list_v[i];
+                        above += k > mine ? w : 0;
+                        with += k >= mine ? w : 0;
+                    }
+                    if (above < need && need <= with) {  // (one key; its ties say the same)
+                        s.key = mine;
+                        s.left = need - above;
+                    }
                 }
-                before += v[j];
+                __syncthreads();
+                key = s.key;
+                need = s.left;
+                break;
             }
         }
-        __syncthreads();
-        key = s.key;
-        left = s.left;
-        if (shift == 0) return;
-        lo = key;
-        need = left;
         bins = shift > kBinBits ? kBins : 1u << shift;
         shift = shift > kBinBits ? shift - kBinBits : 0;
     }
+    left = need;
 }
 
 // A row's kept places from its n keys in s_key (N K of them in place order, 0:
@@ -330,11 +387,10 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, int row, RowShar
     u64 quota = ~0ull;  // and this many of those with this key
     if (top_k > 0 && (unsigned)top_k < count)
         descend<N, unsigned>(s, kmin, kmax, (u64)top_k, 0.0,
-            [&](unsigned *bin, unsigned lo, int shift, unsigned bins) {
+            [&](auto f) {
 #pragma unroll
                 for (int j = 0; j < K; j++)
-                    if (key[j] && key[j] >= lo && ((key[j] - lo) >> shift) < bins)
-                        atomicAdd(&bin[(key[j] - lo) >> shift], 1u);
+                    if (key[j]) f(key[j], 1u);
             },
             thr, quota);
     if (a.top_p < 1.0) {
@@ -342,13 +398,11 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, int row, RowShar
         const u64 quota_k = quota;
         u64 left;
         descend<N, u64>(s, kmin, kmax, 0, a.top_p,
-            [&](u64 *bin, unsigned lo, int shift, unsigned bins) {
+            [&](auto f) {
 #pragma unroll
                 for (int j = 0; j < K; j++)
-                    if (key[j] > thr_k && key[j] >= lo && ((key[j] - lo) >> shift) < bins)
-                        atomicAdd(&bin[(key[j] - lo) >> shift], mass[j]);
-                if (tid == 0 && thr_k && thr_k >= lo && ((thr_k - lo) >> shift) < bins)  // the ties top_k keeps
-                    atomicAdd(&bin[(thr_k - lo) >> shift], quota_k * wg.mass(wg.weight(thr_k)));
+                    if (key[j] > thr_k) f(key[j], mass[j]);
+                if (tid == 0 && thr_k) f(thr_k, quota_k * wg.mass(wg.weight(thr_k)));  // the ties top_k keeps
             },
             thr, left);
         const u64 each = wg.mass(wg.weight(thr));
@@ -464,11 +518,10 @@ __global__ __launch_bounds__(kTrimThreads) void sample_trim_kernel(SampleArgs a)
     u64 quota = 0;
     if ((unsigned)top_k < count)
         descend<N, unsigned>(s, kmin, kmax, (u64)top_k, 0.0,
-            [&](unsigned *bin, unsigned lo, int shift, unsigned bins) {
+            [&](auto f) {
 #pragma unroll
                 for (int j = 0; j < K; j++)
-                    if (j < steps && key[j] && key[j] >= lo && ((key[j] - lo) >> shift) < bins)
-                        atomicAdd(&bin[(key[j] - lo) >> shift], 1u);
+                    if (j < steps && key[j]) f(key[j], 1u);
             },
             thr, quota);
     const u64 below = (1ull << (tid & 63)) - 1;
