@@ -20,7 +20,14 @@
 //
 // Short rows: one workgroup each, one launch; a thread holds its keys and masses
 // in registers through all passes.  Long rows: many workgroups, one launch per
-// pass.
+// pass.  Scores are few bytes (1 M of them: 4 MB, 1 us): what bounds the short
+// form is one CU's issue (a weight is some 40 instructions, half of them in 64
+// bits) and a pass' barriers, the long form its launches, 4 to 12 us each, of
+// which most is waiting for the bins of the one before.  Measured (one MI355X):
+//   960 scores, 960 draws                                 7 us
+//   32 rows x 20011, top_k 2000, top_p, min_p, 128 draws  38 us (split: 60)
+//   1000003 scores, top_k 500000, top_p, 16384 draws      63 us
+//   64 rows x 128256, one draw, no trim 50 us, top_p 121 us
 #include <hip/hip_runtime.h>
 
 #include "sc_train.hpp"
@@ -579,7 +586,7 @@ __global__ __launch_bounds__(kTrimThreads) void sample_trim_kernel(SampleArgs a)
 
 constexpr int kPartThreads = 512;  // (256: 10 to 30 % slower to 200 parts; 1024: 50 % slower from 2000)
 constexpr int kDrawThreads = 256;
-constexpr int kGroups = 64;         // groups of 64 f places per part
+constexpr int kGroups = 64;  // groups of 64 f places per part, one per lane of a draw's wave
 constexpr int kMostParts = 1024;    // (a draw's workgroup holds their sums in LDS)
 
 enum BinArray { kC1, kM1, kC2, kK2, kC3, kK3, kM2, kM3, kBinArrays };  // K: masses of top_k's levels
@@ -1071,8 +1078,11 @@ void launch_step(const SampleArgs &a, hipStream_t s) {
 // The rest are cut over many, at most kSplitRows rows at a time (their workspace).
 constexpr int kRowScores = 8192, kTrimScores = 32768, kSplitRows = 512;
 
+// (top_k 3277 alone on one row of 32768: 41 us trimmed, 33 split, but 64 rows 42 and
+// 47; with top_p too 46 and 49, 64 rows 46 and 75)
 static bool trim(const SampleArgs &a) {
-    return a.V <= kTrimScores && (a.temperature == 0.0 || (a.top_k > 0 && a.top_k <= kTrimKept));
+    const bool few = a.temperature == 0.0 || (a.top_k > 0 && a.top_k <= kTrimKept);
+    return few && a.V <= kTrimScores && (a.V <= kTrimScores / 2 || a.B >= 32 || a.top_p < 1.0);
 }
 static bool split(const SampleArgs &a) { return a.V > kRowScores && !trim(a); }
 
@@ -1100,9 +1110,10 @@ static void launch_split(const SampleArgs &a, hipStream_t s) {
         launch_step<kP3Step>(a, s);
     }
     launch_step<kSums>(a, s);
-    // draws per wave: one until the chip's 8192 waves are taken, 16 at most
+    // draws per wave: one until half of the chip's 8192 waves are taken, 16 at most
+    // (every workgroup cumulates the parts first)
     const long long waves = (long long)a.B * a.S;
-    const int draws = waves <= 8192 ? 1 : waves >= 16 * 8192 ? 16 : (int)((waves + 8191) / 8192);
+    const int draws = waves <= 4096 ? 1 : waves >= 16 * 4096 ? 16 : (int)((waves + 4095) / 4096);
     const int per = draws * kDrawThreads / 64, chunks = a.S > per ? (a.S + per - 1) / per : 1;
     hipLaunchKernelGGL(sample_draw_kernel, dim3((unsigned)((long long)a.B * chunks)), dim3(kDrawThreads), 0, s, a,
                        chunks, draws);

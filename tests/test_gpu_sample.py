@@ -184,6 +184,9 @@ def test_long_rows_trimmed_first(tr, v, dtype):
     for k in (1, 2, 63, 8191, 8192, 8193):
         _check(tr, scores, u, top_k=k)
         _check(tr, scores, u, lens=lens, top_k=k, top_p=0.9, min_p=1e-3, temperature=1.5)
+    many, numbers = _inputs(40, v, 7, v + 1, dtype)  # (rows enough to be trimmed without top_p)
+    _check(tr, many, numbers, top_k=700)
+    _check(tr, many, numbers, temperature=0.0)
     equal = torch.full((1, v), 0.5).to(DT[dtype])
     for k in (5, 8192):
         _check(tr, equal, u[:1], top_k=k)
