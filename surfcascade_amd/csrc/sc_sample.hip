@@ -279,8 +279,8 @@ __device__ __forceinline__ void level(RowShared<N> &s, unsigned lo, int shift, u
     constexpr int kPer = kBins / N;
     Bin *bin = reinterpret_cast<Bin *>(s.bins);
     for (int i = threadIdx.x; i < kBins; i += N) bin[i] = 0;
-    if (threadIdx.x == 0) s.listed = 0;
     __syncthreads();
+    if (threadIdx.x == 0) s.listed = 0;  // (behind the barrier: what was listed last has been read)
     each([&](unsigned k, Bin v) {
         if (k >= lo && ((k - lo) >> shift) < bins) atomicAdd(&bin[(k - lo) >> shift], v);
     });

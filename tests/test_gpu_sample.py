@@ -281,3 +281,17 @@ def test_same_call_same_bits(tr):
     for _ in range(3):
         b = tr.sample(S, Q, top_k=90000, top_p=0.95)
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("v", [700, 4000, 8192, 20000])
+@pytest.mark.parametrize("trim", [dict(top_k=350), dict(top_p=0.5), dict(top_k=300, top_p=0.6)], ids=str)
+def test_crowded_bins(tr, v, trim):
+    """Rows whose descents end in a bin with more members than are ranked at
+    once, several levels deep: most scores within a few hundred steps of 1, two
+    far ones that make the range wide."""
+    g = torch.Generator().manual_seed(v)
+    near = 1.0 + torch.randint(0, 300, (300, v), generator=g).float() * 2.0 ** -20
+    near[:, 0], near[:, 1] = -3.0e38, -1.0
+    near[:, 600:] = -20.0 - torch.rand(300, v - 600, generator=g)
+    near = near[:, torch.randperm(v, generator=g)].contiguous()
+    _check(tr, near, torch.rand(300, 4, generator=g, dtype=torch.float64), **trim)
