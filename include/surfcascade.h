@@ -204,7 +204,8 @@ int sc_mine_batch_device(sc_detector *d, const uint8_t *d_frames, int n, int w, 
  * writes device memory of the trainer's GPU (checked: SC_ERR_INVALID), and may
  * be captured into a HIP graph.  The stream rules are a detector's: see
  * sc_detector_wait_stream, sc_stream_wait_detector, sc_detector_set_stream.
- * Switching to or from a stream that is being captured sets up no order.
+ * Switching to or from a stream that is being captured sets up no order
+ * (but for the trainer's own workspace, below, which stays safe to use).
  * Distinct trainers may be used from different threads, one is not thread-safe.
  *
  * Workspaces: a call that takes (ws, ws_bytes) uses that device memory

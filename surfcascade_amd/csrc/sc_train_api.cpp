@@ -20,6 +20,8 @@ struct sc_trainer {
     hipStream_t stream = nullptr;      // where launches go: own_stream, or the caller's
     hipStream_t own_stream = nullptr;  // created with the trainer, destroyed with it
     hipEvent_t event = nullptr;        // recorded and waited on at once (stream order)
+    hipEvent_t left = nullptr;         // end of the stream last left for one under capture ...
+    bool pending = false;              // ... whose work no later stream waits for yet
     sc::DevBuf<char> ws;               // workspace of calls that bring none
 
     ~sc_trainer() {
@@ -29,6 +31,7 @@ struct sc_trainer {
         // (a caller's stream is not touched: freeing waits for the device)
         if (own_stream) (void)hipStreamSynchronize(own_stream);
         ws.release();
+        if (left) (void)hipEventDestroy(left);
         if (event) (void)hipEventDestroy(event);
         if (own_stream) (void)hipStreamDestroy(own_stream);
         (void)hipSetDevice(before);
@@ -71,6 +74,14 @@ bool capturing(hipStream_t s) {
     return st != hipStreamCaptureStatusNone;
 }
 
+// The trainer's stream waits for the one left before a capture, whose calls may
+// still use the trainer's workspace.
+void catch_up(sc_trainer *t) {
+    if (!t->pending) return;
+    HIPCHK(hipStreamWaitEvent(t->stream, t->left, 0));
+    t->pending = false;
+}
+
 // `bytes` of workspace: the caller's, or the trainer's own.  Growing the own
 // one frees what an earlier call may still use only after the device is idle
 // (hipFree); inside a capture there is no growing, and two graphs must not
@@ -87,6 +98,7 @@ void *workspace(sc_trainer *t, size_t bytes, void *ws, size_t ws_bytes) {
     }
     if (capturing(t->stream))
         throw Error{SC_ERR_INVALID, "a call under stream capture needs a workspace of its own"};
+    catch_up(t);
     if (bytes > t->ws.n) HIPCHK(hipStreamSynchronize(t->stream));
     t->ws.ensure(bytes);
     return t->ws.p;
@@ -181,6 +193,7 @@ int sc_trainer_create(int device, sc_trainer **out) {
             HIPCHK(hipStreamCreateWithFlags(&t->own_stream, hipStreamNonBlocking));
             t->stream = t->own_stream;
             HIPCHK(hipEventCreateWithFlags(&t->event, hipEventDisableTiming));
+            HIPCHK(hipEventCreateWithFlags(&t->left, hipEventDisableTiming));
         } catch (...) {
             delete t;
             throw;
@@ -227,10 +240,15 @@ int sc_trainer_set_stream(sc_trainer *t, void *stream, int use_own) {
                 throw Error{SC_ERR_INVALID, "stream of device " + std::to_string(dev) + ", trainer on " +
                                                 std::to_string(t->device)};
         }
-        // an event may not tie a capturing stream to one outside the capture
-        if (!capturing(t->stream) && !capturing(s)) {
-            HIPCHK(hipEventRecord(t->event, t->stream));
-            HIPCHK(hipStreamWaitEvent(s, t->event, 0));
+        // an event may not tie a capturing stream to one outside the capture:
+        // eager work then waits for eager work (a captured call has no part in
+        // the trainer's workspace)
+        if (!capturing(t->stream)) {
+            catch_up(t);
+            const bool to = capturing(s);
+            HIPCHK(hipEventRecord(to ? t->left : t->event, t->stream));
+            if (to) t->pending = true;
+            else HIPCHK(hipStreamWaitEvent(s, t->event, 0));
         }
         t->stream = s;
         return SC_OK;

@@ -690,3 +690,34 @@ def test_boosting_round(tr):
     fa = feat.double().cpu()
     want = torch.stack([torch.sigmoid(fa[:, j] @ wd[j] + bd[j]) for j in pick.tolist()], 1).mean(1)
     assert torch.allclose(score.double().cpu(), want, rtol=0, atol=1e-4)
+
+
+def test_workspace_order_around_a_capture():
+    """A call on a third stream, after one was captured on a second, waits for
+    the first stream's call: both use the trainer's workspace."""
+    tr = sc.Trainer()
+    X, W, T = torch.rand(9000, 4, 32).cuda(), torch.rand(4, 32).cuda(), torch.zeros(9000).cuda()
+    want = [v.clone() for v in tr.loss(X, W, T)]
+    a, b, c = (torch.cuda.Stream() for _ in range(3))
+    torch.cuda.synchronize()
+    g, end = torch.cuda.CUDAGraph(), torch.cuda.Event()
+    with torch.cuda.stream(a):
+        torch.cuda._sleep(100_000_000)
+        busy = torch.cuda.Event()
+        busy.record()
+        first = tr.loss(X, W, T)
+    with torch.cuda.stream(b):
+        g.capture_begin()
+        y = tr.response(X, W)
+        g.capture_end()
+    with torch.cuda.stream(c):
+        second = tr.loss(X, W, T)
+        end.record()
+        done = end.query()
+        assert not (done and not busy.query())
+    torch.cuda.synchronize()
+    for got in (first, second):
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, tr.response(X, W))
