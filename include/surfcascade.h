@@ -279,8 +279,9 @@ int sc_lr_workspace(const sc_samples *x, const sc_weak_bank *k, size_t *bytes);
  *   g = alpha * dy * act'(z), 0 for an absent row or learner
  *   dw[j][k] = sum_r g x[row r, patch j], db[j][k] = sum_r g
  *   dres = beta * dy, summed over a row's results for SC_RES_ROW
- * (dres NULL with SC_RES_NONE).  Sums over rows in 32 bits over a chunk of
- * rows and in 64 bits over the chunks, dres sums in 64 bits.  There is no
+ * (dres NULL with SC_RES_NONE; no result overlaps another operand).  Sums over rows in 32 bits over a chunk of
+ * rows and in 64 bits over the chunks, dres sums in 64 bits.  A g that is
+ * infinite or NaN leaves its learner's and set's dw and db so.  There is no
  * gradient of the descriptors: they are read off images. */
 int sc_lr_response_grad(sc_trainer *t, const sc_samples *x, const sc_weak_bank *k, int act,
                         float alpha, const float *dy, int64_t dy_ld, float *dw, float *db,
@@ -305,7 +306,8 @@ typedef struct {
 } sc_sample_params;
 void sc_sample_params_default(sc_sample_params *p);
 int sc_sample_workspace(int b, int v, int s, size_t *bytes);
-/* s draws with replacement from each of b rows of v scores (log-weights,
+/* s draws with replacement from each of b rows of v scores (b and s at most
+ * 2^30, v at most 2^26; log-weights,
  * scores + i*ld, dtype as sc_samples; lens != NULL: row i has lens[i] scores,
  * clamped to [0, v]).  Place i of a row weighs exp((s_i - max) / temperature);
  * -inf and NaN are absent, +inf outweighs every finite score.  The kept places

@@ -1075,8 +1075,9 @@ void launch_step(const SampleArgs &a, hipStream_t s) {
 
 // Rows of up to kRowScores scores have one workgroup, whose registers hold them
 // all the way; up to kTrimScores, if top_k keeps few, one that trims them first.
-// The rest are cut over many, at most kSplitRows rows at a time (their workspace).
-constexpr int kRowScores = 8192, kTrimScores = 32768, kSplitRows = 512;
+// The rest are cut over many, at most kSplitRows rows at a time (their workspace);
+// a grid of 1024 threads a row has at most kGridRows (fewer than 2^32 threads).
+constexpr int kRowScores = 8192, kTrimScores = 32768, kSplitRows = 512, kGridRows = 1 << 21;
 
 // (top_k 3277 alone on one row of 32768: 41 us trimmed, 33 split, but 64 rows 42 and
 // 47; with top_p too 46 and 49, 64 rows 46 and 75)
@@ -1111,36 +1112,41 @@ static void launch_split(const SampleArgs &a, hipStream_t s) {
     }
     launch_step<kSums>(a, s);
     // draws per wave: one until half of the chip's 8192 waves are taken, 16 at most
-    // (every workgroup cumulates the parts first)
     const long long waves = (long long)a.B * a.S;
-    const int draws = waves <= 4096 ? 1 : waves >= 16 * 4096 ? 16 : (int)((waves + 4095) / 4096);
+    // (a grid has fewer than 2^32 threads, so past 2^28 draws more again)
+    const int draws = waves <= 4096           ? 1
+                      : waves < 16 * 4096     ? (int)((waves + 4095) / 4096)
+                      : waves <= 16ll << 24   ? 16
+                                              : (int)((waves >> 24) + 1);
     const int per = draws * kDrawThreads / 64, chunks = a.S > per ? (a.S + per - 1) / per : 1;
     hipLaunchKernelGGL(sample_draw_kernel, dim3((unsigned)((long long)a.B * chunks)), dim3(kDrawThreads), 0, s, a,
                        chunks, draws);
 }
 
-void launch_sample(const SampleArgs &a, hipStream_t s) {
-    if (a.B == 0) return;
-    if (split(a)) {
-        const int elem = a.dtype == SC_F32 ? 4 : 2;
-        for (int r = 0; r < a.B; r += kSplitRows) {
-            SampleArgs b = a;
-            b.B = a.B - r < kSplitRows ? a.B - r : kSplitRows;
-            b.scores = static_cast<const char *>(a.scores) + r * a.ld * elem;
-            if (a.lens) b.lens = a.lens + r;
-            b.u = a.u + r * a.u_ld;
-            b.index = a.index + r * a.index_ld;
-            if (a.kept) b.kept = a.kept + r;
-            launch_split(b, s);
-        }
-        return;
-    }
-    if (a.V <= 256) launch_row<256, 1>(a, s);
+static void launch_rows(const SampleArgs &a, bool cut, hipStream_t s) {
+    if (cut) launch_split(a, s);
+    else if (a.V <= 256) launch_row<256, 1>(a, s);
     else if (a.V <= 1024) launch_row<1024, 1>(a, s);
     else if (a.V <= 4096) launch_row<1024, 4>(a, s);
     else if (a.V <= kRowScores) launch_row<1024, 8>(a, s);
     else if (a.V <= kTrimScores / 2) hipLaunchKernelGGL(sample_trim_kernel<16>, dim3((unsigned)a.B), dim3(kTrimThreads), 0, s, a);
     else hipLaunchKernelGGL(sample_trim_kernel<32>, dim3((unsigned)a.B), dim3(kTrimThreads), 0, s, a);
+}
+
+void launch_sample(const SampleArgs &a, hipStream_t s) {
+    const bool cut = split(a);
+    const int most = cut ? kSplitRows : kGridRows;
+    const int elem = a.dtype == SC_F32 ? 4 : 2;
+    for (int r = 0; r < a.B; r += most) {
+        SampleArgs b = a;
+        b.B = a.B - r < most ? a.B - r : most;
+        b.scores = static_cast<const char *>(a.scores) + r * a.ld * elem;
+        if (a.lens) b.lens = a.lens + r;
+        b.u = a.u + r * a.u_ld;
+        b.index = a.index + r * a.index_ld;
+        if (a.kept) b.kept = a.kept + r;
+        launch_rows(b, cut, s);
+    }
 }
 
 }  // namespace sc

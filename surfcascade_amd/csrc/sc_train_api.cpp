@@ -377,6 +377,7 @@ int sc_sample_workspace(int b, int v, int s, size_t *bytes) {
         need(bytes, "null argument");
         need(b >= 0 && v >= 0 && s >= 0, "negative size");
         need(v <= sc::kMaxPool, "more than 2^26 scores in a row");
+        need(b <= kMostRows && s <= kMostRows, "more than 2^30 rows or draws");
         sc::SampleArgs a{};
         a.B = b;
         a.V = v;
@@ -398,6 +399,7 @@ int sc_sample(sc_trainer *t, const void *scores, int dtype, int b, int v, int64_
         need(dtype == SC_F32 || dtype == SC_F16 || dtype == SC_BF16, "unknown score type");
         need(b >= 0 && v >= 0 && s >= 0, "negative size");
         need(v <= sc::kMaxPool, "more than 2^26 scores in a row");
+        need(b <= kMostRows && s <= kMostRows, "more than 2^30 rows or draws");
         need(ld >= v || b <= 1, "rows of scores overlap (ld < v)");
         need(u_ld >= s || b <= 1, "rows of u overlap");
         need(index_ld >= s || b <= 1, "rows of index overlap");

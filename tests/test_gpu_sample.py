@@ -295,3 +295,23 @@ def test_crowded_bins(tr, v, trim):
     near[:, 600:] = -20.0 - torch.rand(300, v - 600, generator=g)
     near = near[:, torch.randperm(v, generator=g)].contiguous()
     _check(tr, near, torch.rand(300, 4, generator=g, dtype=torch.float64), **trim)
+
+
+def test_more_rows_than_a_grid_has(tr):
+    """2^21 rows are one launch; the rows behind them are a second."""
+    b = 2**21 + 5
+    scores = torch.rand(b, 3, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    u = torch.full((b, 1), 0.5, dtype=torch.float64, device="cuda")
+    idx, kept = tr.sample(scores, u, temperature=0.0)
+    assert torch.equal(idx[:, 0].long(), scores.argmax(1)) and bool((kept == 1).all())
+
+
+def test_more_draws_than_a_grid_has(tr):
+    """Past 2^28 draws a wave makes more than 16 of them."""
+    v, reps = 8193, 2**28 // 8193 + 2
+    place = torch.arange(v, device="cuda")
+    u = ((place.double() + 0.5) / v).repeat(reps)[None]
+    assert u.numel() > 2**28
+    idx, kept = tr.sample(torch.zeros(1, v, device="cuda"), u)
+    assert int(kept) == v
+    assert bool((idx.view(reps, v) == place.int()).all())

@@ -157,3 +157,10 @@ def test_no_gpu_is_a_device_error():
     with pytest.raises(sc.SurfCascadeError) as e:
         sc.Trainer()
     assert e.value.code == -5
+
+
+@pytest.mark.parametrize("kw", [dict(b=2**30 + 1), dict(s=2**30 + 1, u_ld=2**31, index_ld=2**31)])
+def test_too_many_rows_or_draws(L, kw):
+    assert _sample(L, **kw) == INVALID and "2^30" in _msg(L)
+    size = ctypes.c_size_t()
+    assert L.sc_sample_workspace(kw.get("b", 1), 10, kw.get("s", 1), ctypes.byref(size)) == INVALID
