@@ -726,7 +726,8 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void lr_wide_kernel(LrArgs a) {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-// v = a + b + c, each a bfloat16 (8 + 8 + 8 bits of 24): the high halves
+// v = a + b + c, each a bfloat16 (8 + 8 + 8 bits of 24): the high halves (an
+// infinite v: a, and NaN for what is left of it)
 __device__ __forceinline__ void split3(float v, unsigned &a, unsigned &b, unsigned &c) {
     a = __float_as_uint(v) & 0xffff0000u;
     const float r = v - __uint_as_float(a);
@@ -758,6 +759,8 @@ __global__ __launch_bounds__(64 * kWideWaves) void lr_wide_bf16_kernel(LrArgs a)
         unsigned lo[3], hi[3];
         split3(wf[2 * k], lo[0], lo[1], lo[2]);
         split3(wf[2 * k + 1], hi[0], hi[1], hi[2]);
+        if (__builtin_isinf(wf[2 * k])) lo[1] = lo[2] = 0;  // (an infinite weight's response is no NaN)
+        if (__builtin_isinf(wf[2 * k + 1])) hi[1] = hi[2] = 0;
 #pragma unroll
         for (int e = 0; e < 3; e++) w[e][k] = pack(lo[e], hi[e]);
     }
@@ -845,23 +848,27 @@ __global__ __launch_bounds__(32 * SUBS) void lr_tail_kernel(LrArgs a, int loss, 
     }
     __shared__ double s_sum[SUBS][32];
     const long long words = (long long)a.M * a.H * kPartWords;
-    const long long i = (long long)blockIdx.x * 32 + (threadIdx.x & 31);
     const int sub = threadIdx.x >> 5;
-    double s = 0.0;
-    if (i < words) {
+    for (long long i0 = (long long)blockIdx.x * 32; i0 < words; i0 += (long long)joins * 32) {
+        const long long i = i0 + (threadIdx.x & 31);
+        double s = 0.0;
+        if (i < words) {
 #pragma unroll 4
-        for (int k = sub; k < a.chunks; k += SUBS) s += (double)a.part[k * words + i];
-    }
-    s_sum[sub][threadIdx.x & 31] = s;
-    __syncthreads();
-    if (sub != 0 || i >= words) return;
+            for (int k = sub; k < a.chunks; k += SUBS) s += (double)a.part[k * words + i];
+        }
+        s_sum[sub][threadIdx.x & 31] = s;
+        __syncthreads();
+        if (sub == 0 && i < words) {
 #pragma unroll
-    for (int k = 1; k < SUBS; k++) s += s_sum[k][threadIdx.x];
-    const long long mh = i / kPartWords;
-    const int word = (int)(i - mh * kPartWords);
-    if (word < kDesc) a.dw[mh * kDesc + word] = (float)s;
-    else if (word == kDesc) a.db[mh] = (float)s;
-    else if (loss) a.loss[mh] = (float)s;
+            for (int k = 1; k < SUBS; k++) s += s_sum[k][threadIdx.x];
+            const long long mh = i / kPartWords;
+            const int word = (int)(i - mh * kPartWords);
+            if (word < kDesc) a.dw[mh * kDesc + word] = (float)s;
+            else if (word == kDesc) a.db[mh] = (float)s;
+            else if (loss) a.loss[mh] = (float)s;
+        }
+        __syncthreads();
+    }
 }
 
 int items_per_wave(const LrArgs &a) { return a.dtype == SC_F32 ? 8 : 16; }
@@ -963,7 +970,8 @@ void launch_lr_grad(const LrArgs &a, bool loss, hipStream_t s) {
         else launch_mode<kGrad>(a, grid, s);
     }
     const long long words = (long long)a.M * a.H * kPartWords;
-    const int joins = a.chunks == 1 ? 0 : (int)ceil_div(words, 32);
+    // (a grid has fewer than 2^32 threads)
+    const int joins = a.chunks == 1 ? 0 : words < (32ll << 20) ? (int)ceil_div(words, 32) : 1 << 20;
     // a wave per row, or 16 lanes where rows are short
     const int lanes = (long long)a.M * a.H > 64 ? 64 : 16, block = a.chunks > 32 ? 1024 : 256;
     long long sums = !loss && a.res_kind == SC_RES_ROW ? ceil_div(a.R, block / lanes) : 0;

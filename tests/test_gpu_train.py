@@ -721,3 +721,30 @@ def test_workspace_order_around_a_capture():
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(y, tr.response(X, W))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("h", [1, 16])
+def test_infinite_weights(tr, h, dtype):
+    """z = -inf: a sigmoid of 0 and, for target 0, gradients of 0 (the loss has a
+    0 * inf, also in its formula)."""
+    x = (0.25 + torch.rand(70, 3, 32, generator=_rng(5))).to(DT[dtype]).cuda()
+    w = torch.zeros(3, h, 32, device="cuda")
+    w[1, h // 2, 7] = -math.inf
+    y = tr.response(x, w)
+    assert bool((y[:, 1, h // 2] == 0).all()) and not bool(torch.isnan(y).any())
+    dw, db, _ = tr.response_grad(x, w, torch.ones_like(y))
+    assert bool((dw[1, h // 2] == 0).all()) and float(db[1, h // 2]) == 0
+    _, dw, db = tr.loss(x, w, torch.zeros(70, device="cuda"))
+    assert bool((dw[1, h // 2] == 0).all()) and float(db[1, h // 2]) == 0
+    assert bool(torch.isfinite(dw).all()) and bool(torch.isfinite(db).all())
+
+
+def test_no_rows_of_very_many_learners(tr):
+    """2^25 learner sets, whose zeros are more workgroups' than a grid has."""
+    w = torch.ones(2**20, 32, 32, device="cuda")
+    patch = torch.zeros(2**20, dtype=torch.int32, device="cuda")
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    out = tr.loss(torch.rand(4, 2, 32, device="cuda"), w, torch.zeros(4, device="cuda"), patch=patch, rows=none)
+    for v in out:
+        assert not bool(v.any())
