@@ -31,7 +31,11 @@ class Trainer:
     descriptors contiguous (any stride between samples).  w: float32
     [m, 32] or [m, h, 32]; b: None or float32 [m] or [m, h].  patch: None or
     int32 [m]; rows: None or int32 [r].  A row or patch number out of range is
-    absent (include/surfcascade.h)."""
+    absent (include/surfcascade.h).
+
+    Results carry no autograd history: `response_grad` and `loss` return the
+    gradients, and operands that ask for one are refused (detach them, or call
+    under torch.no_grad())."""
 
     def __init__(self, device: int = 0):
         import torch
@@ -102,8 +106,15 @@ class Trainer:
             raise ValueError("rows of %s overlap (strides %s)" % (what, stride))
         return t.data_ptr(), max(stride[0], cols)
 
+    def _no_grad(self, *operands):
+        for t in operands:
+            if t is not None and t.requires_grad and self._torch.is_grad_enabled():
+                raise ValueError("results carry no autograd history: detach the operands (response_grad and loss "
+                                 "return gradients)")
+
     def _operands(self, samples, w, b, patch, rows):
         f32, i32 = self._f32, self._i32
+        self._no_grad(samples, w, b)
         dtype = self._dtypes.get(samples.dtype)
         if dtype is None or samples.get_device() != self.device:
             raise ValueError("samples must be float32, float16 or bfloat16 on cuda:%d (got %s on %s)"
@@ -141,11 +152,12 @@ class Trainer:
         other calls), which torch's allocator hands out under a capture."""
         if rc == 0:
             return False
-        if rc == -1 and self._torch.cuda.is_current_stream_capturing():
-            n = bytes_()
-            if n:
-                self._ws = self._torch.empty(n, dtype=self._torch.uint8, device=self._dev)
-                return True
+        if rc == -1:
+            with self._torch.cuda.device(self._dev):
+                n = bytes_() if self._torch.cuda.is_current_stream_capturing() else 0
+                if n:
+                    self._ws = self._torch.empty(n, dtype=self._torch.uint8, device=self._dev)
+                    return True
         _check(rc)
         return False
 
@@ -154,11 +166,13 @@ class Trainer:
                  residual=None, beta=1.0, out=None):
         """alpha * act(x . w + b) + beta * residual for every row and learner
         -> float32 [r, m] or [r, m, h] (sc_lr_response).  residual: None, one
-        value per row [r], or one per result; out may be that residual."""
+        value per row [r], or one per result; out may be the latter, and
+        overlaps no other operand."""
         self._follow()
         x, k, r, sets, cols = self._operands(samples, w, b, patch, rows)
         res, kind, res_ld = None, 0, 0
         if residual is not None:
+            self._no_grad(residual)
             if residual.dim() == 1:
                 kind, res_ld = 1, residual.stride(0)
                 if residual.shape[0] != r or residual.dtype is not self._f32 \
@@ -185,6 +199,7 @@ class Trainer:
         residual: None or "none", "row" or "full", the residual's kind."""
         self._follow()
         x, k, r, sets, cols = self._operands(samples, w, b, patch, rows)
+        self._no_grad(grad_out)
         dy, dy_ld = self._rowwise(grad_out, self._f32, r, cols, "grad_out")
         kind = _RES[residual]
         dw, db, dres, dr = w.new_empty(w.shape), w.new_empty(sets), None, None
@@ -207,6 +222,7 @@ class Trainer:
         float32 [n], by sample; a sample of weight 0 is not looked at."""
         self._follow()
         x, k, r, sets, cols = self._operands(samples, w, b, patch, rows)
+        self._no_grad(target, weight)
         n = samples.shape[0]
         t = self._need(target, self._f32, (n,), "target")
         c = None if weight is None else self._need(weight, self._f32, (n,), "weight") or None
@@ -232,6 +248,7 @@ class Trainer:
         [b, s], in [0, 1)) -> (index int32 like u, kept int32 [b])
         (sc_sample).  lens: int32 [b], the length of each row."""
         self._follow()
+        self._no_grad(scores)
         dtype, dim = self._dtypes.get(scores.dtype), scores.dim()
         if dtype is None or scores.get_device() != self.device:
             raise ValueError("scores must be float32, float16 or bfloat16 on cuda:%d (got %s on %s)"

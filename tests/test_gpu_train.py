@@ -748,3 +748,20 @@ def test_no_rows_of_very_many_learners(tr):
     out = tr.loss(torch.rand(4, 2, 32, device="cuda"), w, torch.zeros(4, device="cuda"), patch=patch, rows=none)
     for v in out:
         assert not bool(v.any())
+
+
+def test_operands_that_want_gradients_are_refused(tr):
+    """Nothing connects a result to its operands, so it must not look as if."""
+    x, w, b, _, _ = _make(9, 3, 3, 2, "f32", 1)
+    X, W, B = x.cuda(), w.cuda(), b.cuda()
+    t, u = torch.zeros(9, device="cuda"), torch.rand(4, dtype=torch.float64, device="cuda")
+    leaf = W.clone().requires_grad_()
+    for call in (lambda w: tr.response(X, w, B), lambda w: tr.response(X, W, w[..., 0].contiguous()),
+                 lambda w: tr.response(X, W, B, residual=w[:, :, 0].sum().expand(9, 3, 2).contiguous()),
+                 lambda w: tr.loss(X, w, t, B), lambda w: tr.response_grad(X, w, torch.ones(9, 3, 2, device="cuda")),
+                 lambda w: tr.sample(w[0, 0], u)):
+        with pytest.raises(ValueError, match="autograd"):
+            call(leaf)
+        call(W)
+        with torch.no_grad():
+            call(leaf)
