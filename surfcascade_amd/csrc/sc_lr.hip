@@ -23,16 +23,15 @@
 // More sets: the matrix cores (below), whose time hardly depends on their number
 // up to 16.  The borders, on 8191 x 608: responses of f32 with 5 sets 153 us
 // narrow and 205 wide (with 7 275: its stores are not whole 16-B pieces), with 8
-// sets 191 and 182; the gradient with 4 sets 150 us
-// narrow, with 5 241 and 206 wide; the loss with 5 sets 184 and 208 in f32, 155
-// and 130 in bf16.
+// sets 191 and 182; the gradient with 4 sets 150 us narrow, with 5 241 and 206
+// wide; the loss with 5 sets 184 and 208 in f32, 155 and 130 in bf16.
 //
 // Measured (one MI355X; a 2 GiB copy moves 4.9 TB/s there, reads and writes):
 //   responses, 16384 x 608, f32, 1 set          221 us, 5.9 TB/s
 //   loss and gradient, 16384 x 608, f32, 1 set  219 us, 5.8 TB/s
 //   responses, 2001 x 608, f16, 16 sets          60 us, 3.5 TB/s
-//   loss and gradient, 8191 x 608, bf16, 16 sets 131 us, 2.5 TB/s (VALU: the
-//     sigmoid, its loss and the operand splits of 80 M results)
+//   loss and gradient, 8191 x 608, bf16, 16 sets 129 us, 2.5 TB/s (the VALU, 68 %
+//     of the cycles: the sigmoid, its loss and the operand splits of 80 M results)
 //   gradient, 480 x 11870, bf16, 8 sets, dres   199 us, 3.8 TB/s
 #include <hip/hip_runtime.h>
 
@@ -168,19 +167,21 @@ __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf
 
 enum Mode { kResponse = 0, kGrad = 1, kLoss = 2 };
 
-// log(1 + e) / e for e in [0, 1]: a polynomial of degree 8 fitted for the
-// least relative error (3.0e-8; 2.8 roundings of 2^-24 as evaluated)
-__device__ __forceinline__ float log1p_over(float e) {
-    float p = 0.005232677f;
-    p = __builtin_fmaf(p, e, -0.029505169f);
-    p = __builtin_fmaf(p, e, 0.078225836f);
-    p = __builtin_fmaf(p, e, -0.13663235f);
-    p = __builtin_fmaf(p, e, 0.19106002f);
-    p = __builtin_fmaf(p, e, -0.24842981f);
-    p = __builtin_fmaf(p, e, 0.33319098f);
-    p = __builtin_fmaf(p, e, -0.49999493f);
-    return __builtin_fmaf(p, e, 0.99999994f);
+// log(1 + e) / e for e in [0, 1], in units of `unit`: a polynomial of degree 8
+// fitted for the least relative error (3.0e-8; 3 roundings of 2^-24 as evaluated)
+__device__ __forceinline__ float log1p_over(float e, float unit) {
+    float p = 0.005232677f * unit;
+    p = __builtin_fmaf(p, e, -0.029505169f * unit);
+    p = __builtin_fmaf(p, e, 0.078225836f * unit);
+    p = __builtin_fmaf(p, e, -0.13663235f * unit);
+    p = __builtin_fmaf(p, e, 0.19106002f * unit);
+    p = __builtin_fmaf(p, e, -0.24842981f * unit);
+    p = __builtin_fmaf(p, e, 0.33319098f * unit);
+    p = __builtin_fmaf(p, e, -0.49999493f * unit);
+    return __builtin_fmaf(p, e, 0.99999994f * unit);
 }
+
+constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
 // What a row brings to its results' gradients: for the loss its weight on
 // either side, pos = c (1 - t) and neg = c t; for a response pos = alpha dy.
@@ -188,14 +189,15 @@ __device__ __forceinline__ float log1p_over(float e) {
 //   c (softplus(z) - t z) = c log(1 + e) + (z >= 0 ? pos : -neg) z
 //   c (sigmoid(z) - t)    = d (z >= 0 ? pos - neg e : pos e - neg)
 // neither of which takes a difference of nearly equal numbers.  A NaN z is a
-// NaN e, and stays one.
-template <int MODE>
+// NaN e, and stays one.  BITS: z comes, and the loss goes, in units of log 2
+// (a product less per result).
+template <int MODE, bool BITS = false>
 __device__ __forceinline__ float grad_of(int act, float z, float pos, float neg, float &loss) {
-    const float e = __expf(-fabsf(z)), d = __builtin_amdgcn_rcpf(1.0f + e);
+    const float e = BITS ? __builtin_amdgcn_exp2f(-fabsf(z)) : __expf(-fabsf(z)), d = __builtin_amdgcn_rcpf(1.0f + e);
     if constexpr (MODE == kLoss) {
         const bool up = z >= 0.0f;
         const float near = up ? pos : -neg, far = up ? -neg : pos;
-        loss = __builtin_fmaf((pos + neg) * e, log1p_over(e), __builtin_fmaf(near, z, loss));
+        loss = __builtin_fmaf((pos + neg) * e, log1p_over(e, BITS ? kLog2E : 1.0f), __builtin_fmaf(near, z, loss));
         return d * __builtin_fmaf(far, e, near);
     } else {
         return act == SC_ACT_SIGMOID ? pos * e * d * d : pos;
@@ -629,13 +631,13 @@ __device__ __forceinline__ void wide_grad(const LrArgs &a, const WideUnit &u, co
     }
     if (t.whole) {
 #pragma unroll
-        for (int k = 0; k < 4; k++) g[k] = grad_of<MODE>(a.act, z[k], pos[k], neg[k], sum_l);
+        for (int k = 0; k < 4; k++) g[k] = grad_of<MODE, __is_same(T, BF16)>(a.act, z[k], pos[k], neg[k], sum_l);
     } else {
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             const bool there = u.present && __shfl(t.v.idx, q * 4 + k, 64) >= 0;
             float l = 0.0f;
-            const float gk = grad_of<MODE>(a.act, z[k], pos[k], neg[k], l);
+            const float gk = grad_of<MODE, __is_same(T, BF16)>(a.act, z[k], pos[k], neg[k], l);
             g[k] = there ? gk : 0.0f;
             sum_l += there ? l : 0.0f;
             if (!there) t.xc[k] = PlacePair<T>{};
@@ -755,6 +757,8 @@ __global__ __launch_bounds__(64 * kWideWaves) void lr_wide_bf16_kernel(LrArgs a)
     load4(a.w + col * kDesc + 8 * q, on, wf);
     load4(a.w + col * kDesc + 8 * q + 4, on, wf + 4);
 #pragma unroll
+    for (int k = 0; k < 8; k++) wf[k] *= kLog2E;  // (z in units of log 2)
+#pragma unroll
     for (int k = 0; k < 4; k++) {
         unsigned lo[3], hi[3];
         split3(wf[2 * k], lo[0], lo[1], lo[2]);
@@ -764,7 +768,7 @@ __global__ __launch_bounds__(64 * kWideWaves) void lr_wide_bf16_kernel(LrArgs a)
 #pragma unroll
         for (int e = 0; e < 3; e++) w[e][k] = pack(lo[e], hi[e]);
     }
-    const float bias = on && a.b ? a.b[col] : 0.0f;
+    const float bias = on && a.b ? kLog2E * a.b[col] : 0.0f;
     const WideOffsets o = wide_offsets<T>(a, u, i, q, col);
     float4_v acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
     float sum_g = 0.0f, sum_l = 0.0f;
@@ -820,18 +824,19 @@ __global__ __launch_bounds__(64 * kWideWaves) void lr_wide_bf16_kernel(LrArgs a)
         m1 = wide_meta<MODE>(a, u, r + 112, i);
         products(r + 32, t[2], t[3]);
     }
-    wide_store<MODE>(a, u, acc, sum_g, sum_l, i, q);
+    wide_store<MODE>(a, u, acc, sum_g, kLn2 * sum_l, i, q);
 }
 
 // What follows the row chunks, in one launch.  The first `joins` workgroups join
-// their partial sums: 32 neighbouring words each, every lane row of SUBS walks
-// every SUBS-th chunk, in 64 bits (no chunk at all, no rows: zeros).  The others
-// write the gradient of a residual of one value per row, beta * the sum of the
-// row's dy: `lanes` of a wave a row, in 64 bits.
-template <int SUBS>
-__global__ __launch_bounds__(32 * SUBS) void lr_tail_kernel(LrArgs a, int loss, int joins, int lanes) {
+// their partial sums: WORDS neighbouring ones each, every one of SUBS rows of
+// threads walks every SUBS-th chunk, in 64 bits.  The others write the gradient
+// of a residual of one value per row, beta * the sum of the row's dy: `lanes` of
+// a wave a row, in 64 bits.  (Loss of 8191 x 608 x 16: 13 chunks, 17 MB of
+// partial sums, 7.2 us; with 8 rows of 32 threads 8.5.)
+template <int SUBS, int WORDS>
+__global__ __launch_bounds__(WORDS * SUBS) void lr_tail_kernel(LrArgs a, int loss, int joins, int lanes) {
     if ((int)blockIdx.x >= joins) {
-        const long long cols = (long long)a.M * a.H, rows = 32 * SUBS / lanes;
+        const long long cols = (long long)a.M * a.H, rows = WORDS * SUBS / lanes;
         const int at = threadIdx.x & (lanes - 1);
         const long long step = (gridDim.x - joins) * rows;
         for (long long r0 = (blockIdx.x - joins) * rows; r0 < a.R; r0 += step) {
@@ -846,28 +851,35 @@ __global__ __launch_bounds__(32 * SUBS) void lr_tail_kernel(LrArgs a, int loss, 
         }
         return;
     }
-    __shared__ double s_sum[SUBS][32];
+    __shared__ double s_sum[SUBS][WORDS];
     const long long words = (long long)a.M * a.H * kPartWords;
-    const int sub = threadIdx.x >> 5;
-    for (long long i0 = (long long)blockIdx.x * 32; i0 < words; i0 += (long long)joins * 32) {
-        const long long i = i0 + (threadIdx.x & 31);
-        double s = 0.0;
-        if (i < words) {
-#pragma unroll 4
-            for (int k = sub; k < a.chunks; k += SUBS) s += (double)a.part[k * words + i];
-        }
-        s_sum[sub][threadIdx.x & 31] = s;
-        __syncthreads();
-        if (sub == 0 && i < words) {
+    const long long i = (long long)blockIdx.x * WORDS + threadIdx.x % WORDS;
+    const int sub = threadIdx.x / WORDS;
+    double s = 0.0;
+    if (i < words) {
+#pragma unroll 8
+        for (int k = sub; k < a.chunks; k += SUBS) s += (double)a.part[k * words + i];
+    }
+    s_sum[sub][threadIdx.x % WORDS] = s;
+    __syncthreads();
+    if (sub != 0 || i >= words) return;
 #pragma unroll
-            for (int k = 1; k < SUBS; k++) s += s_sum[k][threadIdx.x];
-            const long long mh = i / kPartWords;
-            const int word = (int)(i - mh * kPartWords);
-            if (word < kDesc) a.dw[mh * kDesc + word] = (float)s;
-            else if (word == kDesc) a.db[mh] = (float)s;
-            else if (loss) a.loss[mh] = (float)s;
-        }
-        __syncthreads();
+    for (int k = 1; k < SUBS; k++) s += s_sum[k][threadIdx.x];
+    const long long mh = i / kPartWords;
+    const int word = (int)(i - mh * kPartWords);
+    if (word < kDesc) a.dw[mh * kDesc + word] = (float)s;
+    else if (word == kDesc) a.db[mh] = (float)s;
+    else if (loss) a.loss[mh] = (float)s;
+}
+
+// the sums of no rows
+__global__ __launch_bounds__(256) void lr_zero_kernel(LrArgs a, int loss) {
+    const long long sets = (long long)a.M * a.H, step = (long long)gridDim.x * 256;
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < sets * kDesc; i += step) {
+        a.dw[i] = 0.0f;
+        if (i >= sets) continue;
+        a.db[i] = 0.0f;
+        if (loss) a.loss[i] = 0.0f;
     }
 }
 
@@ -968,18 +980,19 @@ void launch_lr_grad(const LrArgs &a, bool loss, hipStream_t s) {
                                   : dim3((unsigned)narrow_waves(a), (unsigned)a.chunks);
         if (loss) launch_mode<kLoss>(a, grid, s);
         else launch_mode<kGrad>(a, grid, s);
+    } else if (a.M && a.H) {
+        const long long blocks = ceil_div((long long)a.M * a.H * kDesc, 256);
+        hipLaunchKernelGGL(lr_zero_kernel, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, s, a, loss ? 1 : 0);
     }
-    const long long words = (long long)a.M * a.H * kPartWords;
-    // (a grid has fewer than 2^32 threads)
-    const int joins = a.chunks == 1 ? 0 : words < (32ll << 20) ? (int)ceil_div(words, 32) : 1 << 20;
+    const int joins = a.chunks > 1 ? (int)ceil_div((long long)a.M * a.H * kPartWords, a.chunks > 32 ? 32 : 64) : 0;
     // a wave per row, or 16 lanes where rows are short
     const int lanes = (long long)a.M * a.H > 64 ? 64 : 16, block = a.chunks > 32 ? 1024 : 256;
     long long sums = !loss && a.res_kind == SC_RES_ROW ? ceil_div(a.R, block / lanes) : 0;
     if (sums > 4096) sums = 4096;
     if (joins + sums == 0) return;
     const dim3 grid((unsigned)(joins + sums));
-    if (block == 1024) hipLaunchKernelGGL(lr_tail_kernel<32>, grid, dim3(block), 0, s, a, loss ? 1 : 0, joins, lanes);
-    else hipLaunchKernelGGL(lr_tail_kernel<8>, grid, dim3(block), 0, s, a, loss ? 1 : 0, joins, lanes);
+    if (block == 1024) hipLaunchKernelGGL((lr_tail_kernel<32, 32>), grid, dim3(block), 0, s, a, loss ? 1 : 0, joins, lanes);
+    else hipLaunchKernelGGL((lr_tail_kernel<4, 64>), grid, dim3(block), 0, s, a, loss ? 1 : 0, joins, lanes);
 }
 
 }  // namespace sc
