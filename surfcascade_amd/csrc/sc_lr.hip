@@ -24,7 +24,7 @@
 // up to 16.  The borders, on 8191 x 608: responses of f32 with 5 sets 153 us
 // narrow and 205 wide (with 7 275: its stores are not whole 16-B pieces), with 8
 // sets 191 and 182; the gradient with 4 sets 150 us narrow, with 5 241 and 206
-// wide; the loss with 5 sets 184 and 208 in f32, 155 and 130 in bf16.
+// wide; the loss with 5 sets 184 and 208 in f32, 155 and 105 in bf16.
 //
 // Measured (one MI355X; a 2 GiB copy moves 4.9 TB/s there, reads and writes):
 //   responses, 16384 x 608, f32, 1 set          221 us, 5.9 TB/s
@@ -32,7 +32,9 @@
 //   responses, 2001 x 608, f16, 16 sets          60 us, 3.5 TB/s
 //   loss and gradient, 8191 x 608, bf16, 16 sets 129 us, 2.5 TB/s (the VALU, 68 %
 //     of the cycles: the sigmoid, its loss and the operand splits of 80 M results)
-//   gradient, 480 x 11870, bf16, 8 sets, dres   199 us, 3.8 TB/s
+//   gradient, 480 x 11870, bf16, 8 sets, dres   198 us, 3.8 TB/s (memory: one or
+//     two learners per wave, loads and stores past the caches, neighbours on one
+//     XCD, 2 or 4 waves per SIMD all take that)
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -48,6 +50,8 @@ constexpr int kWaves = 4;  // waves per workgroup
 constexpr int kWideWaves = 8;   // ... of the wide form (4: 20 % slower on 16 sets of 608 patches)
 // parameter sets per learner up to which the narrow form runs
 constexpr int kNarrowSets = 4, kNarrowResponse = 7;
+// ... and up to which the wide form of 16-bit samples takes two learners per wave
+constexpr int kPairSets = 8;
 
 struct F32 {
     static constexpr int kSize = 4;
@@ -402,6 +406,15 @@ struct WideUnit {
 };
 
 template <class T>
+__device__ __forceinline__ void wide_rows(const LrArgs &a, WideUnit &u) {
+    u.step = a.ld * T::kSize;
+    u.in_order = !a.rows && u.step < (1 << 26);
+    u.dense = a.dy_ld < (1 << 26) && a.dres_ld < (1 << 26);
+    const long long lo = (long long)blockIdx.y * a.rows_per_wave;
+    u.r0 = (int)(lo < a.R ? lo : a.R);
+    u.r1 = (int)(lo + a.rows_per_wave < a.R ? lo + a.rows_per_wave : a.R);
+}
+template <class T>
 __device__ __forceinline__ bool wide_unit(const LrArgs &a, int wave, WideUnit &u) {
     const int sets = (a.H + 15) / 16, unit = blockIdx.x * (blockDim.x >> 6) + wave;
     u.m = unit / sets;
@@ -410,12 +423,7 @@ __device__ __forceinline__ bool wide_unit(const LrArgs &a, int wave, WideUnit &u
     const int p = a.patch ? a.patch[u.m] : u.m;
     u.present = (unsigned)p < (unsigned)a.n_patches;
     u.x = static_cast<const char *>(a.x) + (long long)(u.present ? p : 0) * kDesc * T::kSize;
-    u.step = a.ld * T::kSize;
-    u.in_order = !a.rows && u.step < (1 << 26);
-    u.dense = a.dy_ld < (1 << 26) && a.dres_ld < (1 << 26);
-    const long long lo = (long long)blockIdx.y * a.rows_per_wave;
-    u.r0 = (int)(lo < a.R ? lo : a.R);
-    u.r1 = (int)(lo + a.rows_per_wave < a.R ? lo + a.rows_per_wave : a.R);
+    wide_rows<T>(a, u);
     return true;
 }
 
@@ -573,6 +581,30 @@ __device__ __forceinline__ WideOffsets wide_offsets(const LrArgs &a, const WideU
     o.dres = (unsigned)(4 * q * a.dres_ld + col);
     return o;
 }
+__device__ __forceinline__ void load_dy(const LrArgs &a, const WideUnit &u, const WideOffsets &o, int r, int q,
+                                        long long col, float (&dy)[4]) {
+    if (u.dense && r + 16 <= u.r1) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) dy[k] = (a.dy + (long long)(r + k) * a.dy_ld)[o.dy];
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int row = r + q * 4 + k < u.r1 ? r + q * 4 + k : u.r0;
+            dy[k] = a.dy[(long long)row * a.dy_ld + col];
+        }
+    }
+}
+__device__ __forceinline__ void store_dres(const LrArgs &a, const WideUnit &u, const WideOffsets &o, int r, int q,
+                                           long long col, const float (&dy)[4]) {
+    if (u.dense && r + 16 <= u.r1) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) (a.dres + (long long)(r + k) * a.dres_ld)[o.dres] = a.beta * dy[k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (r + q * 4 + k < u.r1) a.dres[(long long)(r + q * 4 + k) * a.dres_ld + col] = a.beta * dy[k];
+    }
+}
 template <class T, int MODE>
 __device__ __forceinline__ void wide_load(const LrArgs &a, const WideUnit &u, const WideOffsets &o, int r, WideMeta v,
                                           int i, int q, long long col, WideTile<T> &t) {
@@ -590,18 +622,7 @@ __device__ __forceinline__ void wide_load(const LrArgs &a, const WideUnit &u, co
         for (int k = 0; k < 4; k++)
             t.xc[k] = load_pair<T>(u.x + __shfl(j, q * 4 + k, 64) * u.step + 2 * i * T::kSize);
     }
-    if constexpr (MODE == kGrad) {
-        if (u.dense && r + 16 <= u.r1) {
-#pragma unroll
-            for (int k = 0; k < 4; k++) t.dy[k] = (a.dy + (long long)(r + k) * a.dy_ld)[o.dy];
-        } else {
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const int row = r + q * 4 + k < u.r1 ? r + q * 4 + k : u.r0;
-                t.dy[k] = a.dy[(long long)row * a.dy_ld + col];
-            }
-        }
-    }
+    if constexpr (MODE == kGrad) load_dy(a, u, o, r, q, col, t.dy);
 }
 
 // g of this lane's four results; clears what an absent row loaded
@@ -619,16 +640,7 @@ __device__ __forceinline__ void wide_grad(const LrArgs &a, const WideUnit &u, co
             neg[k] = 0.0f;
         }
     }
-    if (MODE == kGrad && a.res_kind == SC_RES_FULL && on) {
-        if (u.dense && r + 16 <= u.r1) {
-#pragma unroll
-            for (int k = 0; k < 4; k++) (a.dres + (long long)(r + k) * a.dres_ld)[o.dres] = a.beta * t.dy[k];
-        } else {
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-                if (r + q * 4 + k < u.r1) a.dres[(long long)(r + q * 4 + k) * a.dres_ld + col] = a.beta * t.dy[k];
-        }
-    }
+    if (MODE == kGrad && a.res_kind == SC_RES_FULL && on) store_dres(a, u, o, r, q, col, t.dy);
     if (t.whole) {
 #pragma unroll
         for (int k = 0; k < 4; k++) g[k] = grad_of<MODE, __is_same(T, BF16)>(a.act, z[k], pos[k], neg[k], sum_l);
@@ -636,49 +648,49 @@ __device__ __forceinline__ void wide_grad(const LrArgs &a, const WideUnit &u, co
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             const bool there = u.present && __shfl(t.v.idx, q * 4 + k, 64) >= 0;
-            float l = 0.0f;
+            float l = sum_l;
             const float gk = grad_of<MODE, __is_same(T, BF16)>(a.act, z[k], pos[k], neg[k], l);
             g[k] = there ? gk : 0.0f;
-            sum_l += there ? l : 0.0f;
+            sum_l = there ? l : sum_l;
             if (!there) t.xc[k] = PlacePair<T>{};
         }
     }
     sum_g += (g[0] + g[1]) + (g[2] + g[3]);
 }
 
-// a wave's sums -> the partial sums of its chunk, or the results
+// a wave's sums -> the partial sums of its chunk, or the results: of a lane's
+// places 2i and 2i+1, of `left` sets from `first` on; of its own set `col`
 template <int MODE>
-__device__ __forceinline__ void wide_store(const LrArgs &a, const WideUnit &u, const float4_v *acc, float sum_g,
-                                           float sum_l, int i, int q) {
+__device__ __forceinline__ void wide_store(const LrArgs &a, const float4_v *acc, float sum_g, float sum_l, int i, int q,
+                                           long long first, int left, bool on, long long col) {
     sum_g += __shfl_xor(sum_g, 16, 64);
     sum_g += __shfl_xor(sum_g, 32, 64);
     sum_l += __shfl_xor(sum_l, 16, 64);
     sum_l += __shfl_xor(sum_l, 32, 64);
-    const long long first = (long long)u.m * a.H + u.h0;
     float *part = a.part ? a.part + (long long)blockIdx.y * a.M * a.H * kPartWords : nullptr;
 #pragma unroll
-    for (int k = 0; k < 4; k++) {  // set 4q+k, places 2i and 2i+1
-        if (u.h0 + q * 4 + k >= a.H) continue;
-        const long long mh = first + q * 4 + k;
+    for (int k = 0; k < 4; k++) {
+        if (k >= left) continue;
+        const long long mh = first + k;
         float *to = part ? part + mh * kPartWords : a.dw + mh * kDesc;
         to[2 * i] = acc[0][k];
         to[2 * i + 1] = acc[1][k];
     }
-    if (u.h0 + i < a.H && q == 0) {
+    if (on && q == 0) {
         if (part) {
-            part[(first + i) * kPartWords + kDesc] = sum_g;
-            part[(first + i) * kPartWords + kDesc + 1] = sum_l;
+            part[col * kPartWords + kDesc] = sum_g;
+            part[col * kPartWords + kDesc + 1] = sum_l;
         } else {
-            a.db[first + i] = sum_g;
-            if (MODE == kLoss) a.loss[first + i] = sum_l;
+            a.db[col] = sum_g;
+            if (MODE == kLoss) a.loss[col] = sum_l;
         }
     }
 }
 
 template <class T>
-__device__ __forceinline__ float place_value(const WideTile<T> &t, int half, int k) {
-    if constexpr (__is_same(T, F32)) return t.xc[k][half];
-    else return (float)__builtin_bit_cast(half2_v, t.xc[k])[half];
+__device__ __forceinline__ float place_value(PlacePair<T> v, int half) {
+    if constexpr (__is_same(T, F32)) return v[half];
+    else return (float)__builtin_bit_cast(half2_v, v)[half];
 }
 
 // Gradient and loss, f32 products (16x16x4: nothing is rounded that the narrow
@@ -707,8 +719,8 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void lr_wide_kernel(LrArgs a) {
         wide_grad<T, MODE>(a, u, o, t, z, r, q, on, col, g, sum_g, sum_l);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            acc[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(g[k], place_value<T>(t, 0, k), acc[0], 0, 0, 0);
-            acc[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(g[k], place_value<T>(t, 1, k), acc[1], 0, 0, 0);
+            acc[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(g[k], place_value<T>(t.xc[k], 0), acc[0], 0, 0, 0);
+            acc[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(g[k], place_value<T>(t.xc[k], 1), acc[1], 0, 0, 0);
         }
     };
     WideMeta ahead = wide_meta<MODE>(a, u, u.r0 + 16, i);
@@ -723,7 +735,7 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void lr_wide_kernel(LrArgs a) {
         ahead = wide_meta<MODE>(a, u, r + 48, i);
         products(r + 16, two);
     }
-    wide_store<MODE>(a, u, acc, sum_g, sum_l, i, q);
+    wide_store<MODE>(a, acc, sum_g, sum_l, i, q, (long long)u.m * a.H + u.h0 + 4 * q, a.H - u.h0 - 4 * q, on, col);
 }
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -738,6 +750,21 @@ __device__ __forceinline__ void split3(float v, unsigned &a, unsigned &b, unsign
 }
 // two high halves -> one register, `lo` first
 __device__ __forceinline__ unsigned pack(unsigned lo, unsigned hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
+
+// a lane's 8 weights in units of 1 / log 2 (z comes in units of log 2 then)
+__device__ __forceinline__ void split_weights(const float (&wf)[8], uint4_v (&w)[3]) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        unsigned lo[3], hi[3];
+        const float a = kLog2E * wf[2 * k], b = kLog2E * wf[2 * k + 1];
+        split3(a, lo[0], lo[1], lo[2]);
+        split3(b, hi[0], hi[1], hi[2]);
+        if (__builtin_isinf(a)) lo[1] = lo[2] = 0;  // (an infinite weight's response is no NaN)
+        if (__builtin_isinf(b)) hi[1] = hi[2] = 0;
+#pragma unroll
+        for (int e = 0; e < 3; e++) w[e][k] = pack(lo[e], hi[e]);
+    }
+}
 
 // Gradient and loss of bfloat16 samples on the bfloat16 matrix cores (16x16x32,
 // a fifth of the f32 ones' time for these products): the samples are exact
@@ -756,18 +783,7 @@ __global__ __launch_bounds__(64 * kWideWaves) void lr_wide_bf16_kernel(LrArgs a)
     float wf[8];
     load4(a.w + col * kDesc + 8 * q, on, wf);
     load4(a.w + col * kDesc + 8 * q + 4, on, wf + 4);
-#pragma unroll
-    for (int k = 0; k < 8; k++) wf[k] *= kLog2E;  // (z in units of log 2)
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-        unsigned lo[3], hi[3];
-        split3(wf[2 * k], lo[0], lo[1], lo[2]);
-        split3(wf[2 * k + 1], hi[0], hi[1], hi[2]);
-        if (__builtin_isinf(wf[2 * k])) lo[1] = lo[2] = 0;  // (an infinite weight's response is no NaN)
-        if (__builtin_isinf(wf[2 * k + 1])) hi[1] = hi[2] = 0;
-#pragma unroll
-        for (int e = 0; e < 3; e++) w[e][k] = pack(lo[e], hi[e]);
-    }
+    split_weights(wf, w);
     const float bias = on && a.b ? kLog2E * a.b[col] : 0.0f;
     const WideOffsets o = wide_offsets<T>(a, u, i, q, col);
     float4_v acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
@@ -824,7 +840,185 @@ __global__ __launch_bounds__(64 * kWideWaves) void lr_wide_bf16_kernel(LrArgs a)
         m1 = wide_meta<MODE>(a, u, r + 112, i);
         products(r + 32, t[2], t[3]);
     }
-    wide_store<MODE>(a, u, acc, sum_g, kLn2 * sum_l, i, q);
+    wide_store<MODE>(a, acc, sum_g, kLn2 * sum_l, i, q, (long long)u.m * a.H + u.h0 + 4 * q, a.H - u.h0 - 4 * q, on, col);
+}
+
+// Up to 8 sets of 16-bit samples, a wave owns two neighbouring learners, lane i's
+// results being those of set i % 8 of learner i / 8: every learner has its own
+// products, half of which is left (a descriptor's NaN stays its learner's), but
+// dy, dres and the arithmetic of g fill the wave.  8191 x 608 x 8, alone and in
+// pairs: loss 127 and 108 us in bf16, 189 and 159 in f16, gradient 143 and 103,
+// 168 and 146; f32 206 and 253, 197 and 196 (it has no registers for two).  480 x
+// 11870 x 8 with dres: 198 us either way, the memory's.
+template <class T>
+struct PairTile {
+    WideMeta v;
+    WideRow<T> x[2];
+    PlacePair<T> xc[2][4];
+    float dy[4];
+    bool whole;
+};
+
+typedef unsigned uint2_v __attribute__((ext_vector_type(2)));
+typedef short short4_v __attribute__((ext_vector_type(4)));
+
+template <class T, int MODE>
+__global__ __launch_bounds__(64 * kWideWaves, 4) void lr_pair_kernel(LrArgs a) {
+    constexpr bool kBf16 = __is_same(T, BF16);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int i = lane & 15, q = lane >> 4;
+    WideUnit u;
+    u.m = 2 * (blockIdx.x * kWideWaves + wave);
+    if (u.m >= a.M) return;
+    const char *x[2];
+    bool present[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int m = u.m + k < a.M ? u.m + k : u.m;
+        const int p = a.patch ? a.patch[m] : m;
+        present[k] = (unsigned)p < (unsigned)a.n_patches;
+        x[k] = static_cast<const char *>(a.x) + (long long)(present[k] ? p : 0) * kDesc * T::kSize;
+    }
+    u.h0 = 0;
+    u.present = present[0] && present[1];
+    wide_rows<T>(a, u);
+    const int mine = i >> 3;
+    const bool on = (i & 7) < a.H && u.m + mine < a.M;
+    const bool here = mine ? present[1] : present[0];
+    const long long col = on ? (long long)(u.m + mine) * a.H + (i & 7) : (long long)u.m * a.H;
+    float wf[8];
+    uint4_v w[3];
+#pragma unroll
+    for (int k = 0; k < 2; k++) load4(a.w + col * kDesc + WideRow<T>::place(q, k), on, wf + 4 * k);
+    float bias = on && a.b ? a.b[col] : 0.0f;
+    if constexpr (kBf16) {
+        bias *= kLog2E;
+        split_weights(wf, w);
+    }
+    const WideOffsets o = wide_offsets<T>(a, u, i, q, col);
+    float4_v acc[2][2] = {};
+    float sum_g = 0.0f, sum_l = 0.0f;
+    auto load = [&](int r, const WideMeta &v, PairTile<T> &t) {
+        t.v = v;
+        t.whole = u.present && __ballot(v.idx < 0) == 0;
+        if (u.in_order && r + 16 <= u.r1) {
+#pragma unroll
+            for (int l = 0; l < 2; l++) {
+                const char *base = x[l] + r * u.step;
+                t.x[l].load(base + o.row);
+#pragma unroll
+                for (int k = 0; k < 4; k++) t.xc[l][k] = load_pair<T>(base + k * u.step + o.place);
+            }
+        } else {
+            const int j = v.idx < 0 ? 0 : v.idx;
+#pragma unroll
+            for (int l = 0; l < 2; l++) t.x[l].load(x[l] + j * u.step + q * 16);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const long long at = __shfl(j, q * 4 + k, 64) * u.step + 2 * i * T::kSize;
+                t.xc[0][k] = load_pair<T>(x[0] + at);
+                t.xc[1][k] = load_pair<T>(x[1] + at);
+            }
+        }
+        if constexpr (MODE == kGrad) load_dy(a, u, o, r, q, col, t.dy);
+    };
+    auto products = [&](int r, PairTile<T> &t) {
+        float4_v z[2];
+#pragma unroll
+        for (int l = 0; l < 2; l++) {
+            z[l] = float4_v{bias, bias, bias, bias};
+            if constexpr (kBf16) {
+#pragma unroll
+                for (int e = 2; e >= 0; e--)
+                    z[l] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, t.x[l].a),
+                                                                   __builtin_bit_cast(bf16x8, w[e]), z[l], 0, 0, 0);
+            } else {
+                float f[8];
+                t.x[l].values(f);
+#pragma unroll
+                for (int k = 0; k < 8; k++) z[l] = __builtin_amdgcn_mfma_f32_16x16x4f32(f[k], wf[k], z[l], 0, 0, 0);
+            }
+        }
+        if (MODE == kGrad && a.res_kind == SC_RES_FULL && on) store_dres(a, u, o, r, q, col, t.dy);
+        float g[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float zk = mine ? z[1][k] : z[0][k];
+            float pos, neg = 0.0f;
+            if constexpr (MODE == kLoss) {
+                pos = __shfl(t.v.pos, q * 4 + k, 64);
+                neg = __shfl(t.v.neg, q * 4 + k, 64);
+            } else {
+                pos = a.alpha * t.dy[k];
+            }
+            if (t.whole) {
+                g[k] = grad_of<MODE, kBf16>(a.act, zk, pos, neg, sum_l);
+            } else {
+                const bool row = __shfl(t.v.idx, q * 4 + k, 64) >= 0;
+                float l = sum_l;
+                const float gk = grad_of<MODE, kBf16>(a.act, zk, pos, neg, l);
+                g[k] = row && here ? gk : 0.0f;
+                sum_l = row && here ? l : sum_l;
+                if (!(row && present[0])) t.xc[0][k] = PlacePair<T>{};
+                if (!(row && present[1])) t.xc[1][k] = PlacePair<T>{};
+            }
+        }
+        sum_g += (g[0] + g[1]) + (g[2] + g[3]);
+        if constexpr (kBf16) {
+            uint2_v gs[3];
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                unsigned lo[3], hi[3];
+                split3(g[2 * k], lo[0], lo[1], lo[2]);
+                split3(g[2 * k + 1], hi[0], hi[1], hi[2]);
+#pragma unroll
+                for (int p = 0; p < 3; p++) gs[p][k] = pack(lo[p], hi[p]);
+            }
+#pragma unroll
+            for (int l = 0; l < 2; l++) {
+                uint2_v xs[2];
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    xs[0][k] = __builtin_amdgcn_perm(t.xc[l][2 * k + 1], t.xc[l][2 * k], 0x05040100u);  // the low halves
+                    xs[1][k] = pack(t.xc[l][2 * k], t.xc[l][2 * k + 1]);
+                }
+#pragma unroll
+                for (int p = 2; p >= 0; p--)
+#pragma unroll
+                    for (int half = 0; half < 2; half++)
+                        acc[l][half] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(short4_v, gs[p]),
+                                                                                 __builtin_bit_cast(short4_v, xs[half]),
+                                                                                 acc[l][half], 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int l = 0; l < 2; l++)
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+#pragma unroll
+                    for (int half = 0; half < 2; half++)
+                        acc[l][half] = __builtin_amdgcn_mfma_f32_16x16x4f32(g[k], place_value<T>(t.xc[l][k], half),
+                                                                            acc[l][half], 0, 0, 0);
+        }
+    };
+    WideMeta ahead = wide_meta<MODE>(a, u, u.r0 + 16, i);
+    PairTile<T> one, two;
+    load(u.r0, wide_meta<MODE>(a, u, u.r0, i), one);
+    for (int r = u.r0; r < u.r1; r += 32) {
+        load(r + 16, ahead, two);
+        ahead = wide_meta<MODE>(a, u, r + 32, i);
+        products(r, one);
+        if (r + 16 >= u.r1) break;
+        load(r + 32, ahead, one);
+        ahead = wide_meta<MODE>(a, u, r + 48, i);
+        products(r + 16, two);
+    }
+    if constexpr (kBf16) sum_l *= kLn2;
+#pragma unroll
+    for (int half = 0; half < 2; half++) acc[0][half] = q >> 1 ? acc[1][half] : acc[0][half];
+    // lane (i, q): places 2i and 2i+1 of the sets 4 (q % 2) .. of learner q / 2; sums: of its own set
+    wide_store<MODE>(a, acc[0], sum_g, sum_l, i, q, (long long)(u.m + (q >> 1)) * a.H + 4 * (q & 1),
+                     u.m + (q >> 1) < a.M ? a.H - 4 * (q & 1) : 0, on, col);
 }
 
 // What follows the row chunks, in one launch.  The first `joins` workgroups join
@@ -889,6 +1083,7 @@ int lanes_per_item(const LrArgs &a) { return a.dtype == SC_F32 ? 8 : 4; }
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
 bool wide(const LrArgs &a) { return a.H > kNarrowSets; }
+bool pair(const LrArgs &a) { return wide(a) && a.H <= kPairSets && a.dtype != SC_F32; }
 bool wide_response(const LrArgs &a) { return a.H > kNarrowResponse; }
 
 template <class T, int MODE>
@@ -896,7 +1091,9 @@ void launch_form(const LrArgs &a, dim3 grid, hipStream_t s) {
     if (MODE == kResponse ? wide_response(a) : wide(a)) {
         constexpr dim3 block(64 * kWideWaves);
         if constexpr (MODE == kResponse) hipLaunchKernelGGL((lr_wide_response_kernel<T>), grid, block, 0, s, a);
-        else if constexpr (__is_same(T, BF16)) hipLaunchKernelGGL((lr_wide_bf16_kernel<MODE>), grid, block, 0, s, a);
+        else if (pair(a)) {
+            if constexpr (T::kSize == 2) hipLaunchKernelGGL((lr_pair_kernel<T, MODE>), grid, block, 0, s, a);
+        } else if constexpr (__is_same(T, BF16)) hipLaunchKernelGGL((lr_wide_bf16_kernel<MODE>), grid, block, 0, s, a);
         else hipLaunchKernelGGL((lr_wide_kernel<T, MODE>), grid, block, 0, s, a);
         return;
     }
@@ -945,13 +1142,14 @@ static int rows_per_wave(long long R, long long waves, int ranges, int step, lon
 // waves over the learners (and sets, which the narrow form has all in one)
 static long long narrow_waves(const LrArgs &a) { return ceil_div(a.M, items_per_wave(a)); }
 static long long wide_waves(const LrArgs &a) { return a.M * ceil_div(a.H, 16); }
+static long long wide_grad_waves(const LrArgs &a) { return pair(a) ? ceil_div(a.M, 2) : wide_waves(a); }
 
 LrPlan lr_plan(const LrArgs &a) {
     LrPlan p{0, 0, 0};
     if (a.R == 0 || a.M == 0 || a.H == 0) return p;
     // (a chunk of the narrow form is one range of rows per wave of a workgroup)
     const int ranges = wide(a) ? 1 : kWaves;
-    p.rows_per_wave = wide(a) ? rows_per_wave(a.R, wide_waves(a), 1, 16, 4096)
+    p.rows_per_wave = wide(a) ? rows_per_wave(a.R, wide_grad_waves(a), 1, 16, 4096)
                               : rows_per_wave(a.R, narrow_waves(a) * kWaves, kWaves, lanes_per_item(a),
                                               1024 * (a.H == 1 ? 6 : a.H == 2 ? 4 : 3));
     p.chunks = (int)ceil_div(a.R, (long long)p.rows_per_wave * ranges);
@@ -976,7 +1174,7 @@ void launch_lr_response(const LrArgs &a0, hipStream_t s) {
 
 void launch_lr_grad(const LrArgs &a, bool loss, hipStream_t s) {
     if (a.chunks > 0) {
-        const dim3 grid = wide(a) ? dim3((unsigned)ceil_div(wide_waves(a), kWideWaves), (unsigned)a.chunks)
+        const dim3 grid = wide(a) ? dim3((unsigned)ceil_div(wide_grad_waves(a), kWideWaves), (unsigned)a.chunks)
                                   : dim3((unsigned)narrow_waves(a), (unsigned)a.chunks);
         if (loss) launch_mode<kLoss>(a, grid, s);
         else launch_mode<kGrad>(a, grid, s);

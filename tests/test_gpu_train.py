@@ -765,3 +765,51 @@ def test_operands_that_want_gradients_are_refused(tr):
         call(W)
         with torch.no_grad():
             call(leaf)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("h,m", [(5, 2), (6, 7), (8, 1), (8, 9), (7, 16)])
+def test_neighbouring_learners_stay_apart(tr, h, m, dtype):
+    """A NaN in one learner's descriptors, weights or dy is that learner's alone;
+    an absent patch's learner is zero whatever stands in the samples."""
+    n, p = 67, 20
+    x, w, b, _, _ = _make(n, p, m, h, dtype, 40 + m)
+    patch = torch.arange(m, dtype=torch.int32) + 2
+    dy = torch.randn(n, m, h, generator=_rng(m))
+    t = (torch.rand(n, generator=_rng(h)) < 0.5).float()
+
+    def run(x, w, dy, patch):
+        dw, db, dres = tr.response_grad(x.cuda(), w.cuda(), dy.cuda(), b.cuda(), patch=patch.cuda(), residual="full")
+        return [v.cpu() for v in (dw, db, dres.permute(1, 0, 2), *tr.loss(x.cuda(), w.cuda(), t.cuda(), b.cuda(),
+                                                                          patch=patch.cuda()))]
+
+    clean = run(x, w, dy, patch)
+    assert all(bool(torch.isfinite(v).all()) for v in clean)
+    for bad in range(m):
+        xs, ws, ds, ps = x.clone(), w.clone(), dy.clone(), patch.clone()
+        xs[33, bad + 2, 5] = math.nan
+        for got, want in zip(run(xs, w, dy, patch), clean):  # (dres does not read the samples)
+            keep = torch.arange(m) != bad
+            assert torch.equal(got[keep], want[keep])
+        ws[bad, h - 1] = math.nan
+        got = run(x, ws, dy, patch)
+        assert bool(torch.isnan(got[1][bad, h - 1])) and bool(torch.isnan(got[3][bad, h - 1]))
+        for g, c in zip(got, clean):
+            keep = torch.ones(m, h, dtype=torch.bool)
+            keep[bad, h - 1] = False
+            if g.dim() == 3 and g.shape[1] == n:
+                continue
+            assert torch.equal(g[keep], c[keep])
+        ds[12, bad, 0] = math.nan
+        got = run(x, w, ds, patch)
+        assert bool(torch.isnan(got[1][bad, 0]))
+        keep = torch.ones(m, h, dtype=torch.bool)
+        keep[bad, 0] = False
+        assert torch.equal(got[0][keep], clean[0][keep]) and torch.equal(got[1][keep], clean[1][keep])
+        ps[bad] = p + 3
+        xs = x.clone()
+        xs[:, 0] = math.nan  # (nobody's patch)
+        for k, (g, c) in enumerate(zip(run(xs, w, dy, ps), clean)):
+            keep = torch.arange(m) != bad
+            assert torch.equal(g[keep], c[keep])
+            assert k == 2 or not bool(g[bad].any())
