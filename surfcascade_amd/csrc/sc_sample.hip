@@ -269,20 +269,20 @@ struct RowShared {
     u64 left;
 };
 
-// One level of a descent: the bin of [lo, lo + (kBins << shift)) where the sum of
-// each()'s members from the top reaches need -> its first key and what is still
-// needed from it.  each(f) calls f(k, v) for every member's key and what it
-// counts for.
-template <int N, class Bin, class Each>
-__device__ __forceinline__ void level(RowShared<N> &s, unsigned lo, int shift, unsigned bins, u64 &need, double share,
-                                      unsigned &key, Each each) {
+// One level of a descent: the bin where the sum of each()'s members from the top
+// reaches need (need = 0: share of the whole) -> `at`, and what is still needed
+// from it.  each(f) calls f(k, v) for every member's key and what it counts for;
+// bin_of(k) >= kBins: not in this level.
+template <int N, class Bin, class Each, class Map>
+__device__ __forceinline__ void level(RowShared<N> &s, u64 &need, double share, unsigned &at, Each each, Map bin_of) {
     constexpr int kPer = kBins / N;
     Bin *bin = reinterpret_cast<Bin *>(s.bins);
     for (int i = threadIdx.x; i < kBins; i += N) bin[i] = 0;
     __syncthreads();
     if (threadIdx.x == 0) s.listed = 0;  // (behind the barrier: what was listed last has been read)
     each([&](unsigned k, Bin v) {
-        if (k >= lo && ((k - lo) >> shift) < bins) atomicAdd(&bin[(k - lo) >> shift], v);
+        const unsigned b = bin_of(k);
+        if (b < kBins) atomicAdd(&bin[b], v);
     });
     __syncthreads();
     const int top = kBins - 1 - kPer * (int)threadIdx.x;  // this thread: bins top, top-1, ...
@@ -295,76 +295,116 @@ __device__ __forceinline__ void level(RowShared<N> &s, unsigned lo, int shift, u
 #pragma unroll
         for (int j = 0; j < kPer; j++) {
             if (before < need && need <= before + v[j]) {
-                s.key = lo + ((unsigned)(top - j) << shift);
+                s.key = top - j;
                 s.left = need - before;
             }
             before += v[j];
         }
     }
     __syncthreads();
-    key = s.key;
+    at = s.key;
     need = s.left;
 }
 
-// Radix descent: the largest key at which the pool's sum from the top reaches
-// need (need = 0: share of the whole), and what its ties still have to bring.
-// The bin where the sum crosses is listed if that may fit (one member per
-// thread), and the next levels run on the list; up to kRanked members are ranked
-// at once, each one's sum of larger keys against need.
+// The members in bin `at`, one per thread if they fit -> their number (more than
+// N: they do not)
+template <int N, class Bin, class Each, class Map>
+__device__ __forceinline__ unsigned list(RowShared<N> &s, unsigned at, unsigned &mine, u64 &value, Each each, Map bin_of) {
+    each([&](unsigned k, Bin v) {
+        if (bin_of(k) != at) return;
+        const unsigned to = atomicAdd(&s.listed, 1u);
+        if (to >= N) return;
+        s.list_k[to] = k;
+        s.list_v[to] = v;
+    });
+    __syncthreads();
+    const unsigned listed = s.listed;
+    if (listed <= N && threadIdx.x < listed) {
+        mine = s.list_k[threadIdx.x];
+        value = s.list_v[threadIdx.x];
+    }
+    return listed;
+}
+
+// up to kRanked listed members: each one's sum of larger keys against need
+template <int N>
+__device__ __forceinline__ void rank(RowShared<N> &s, unsigned listed, unsigned mine, u64 need, unsigned &key, u64 &left) {
+    if (mine) {
+        u64 above = 0, with = 0;
+        for (unsigned i = 0; i < listed; i++) {
+            const unsigned k = s.list_k[i];
+            const u64 w = s.list_v[i];
+            above += k > mine ? w : 0;
+            with += k >= mine ? w : 0;
+        }
+        if (above < need && need <= with) {  // (one key; its ties say the same)
+            s.key = mine;
+            s.left = need - above;
+        }
+    }
+    __syncthreads();
+    key = s.key;
+    left = s.left;
+}
+
+// Descent: the largest key at which the pool's sum from the top reaches need
+// (need = 0: share of the whole), and what its ties still have to bring.
+// The first level's bins are even steps of the score over its range, `window` at
+// most, below which there is one bin: that spreads most pools over all of them,
+// while the keys' own leading bits put a normal distribution into some twenty,
+// where the atomics wait for each other (20011 scores: 6 us).  The bin where the
+// sum crosses is listed, and ranked if it has at most kRanked members.  If it does
+// not fit, the levels are 11 bits of the key each, until it does.
 template <int N, class Bin, class Each>
-__device__ __forceinline__ void descend(RowShared<N> &s, unsigned kmin, unsigned kmax, u64 need, double share, Each each,
-                                        unsigned &key, u64 &left) {
+__device__ __forceinline__ void descend(RowShared<N> &s, unsigned kmin, unsigned kmax, float window, u64 need, double share,
+                                        Each each, unsigned &key, u64 &left) {
+    unsigned listed = N + 1, mine = 0, at;
+    u64 value = 0;
+    const float top = score_of(kmax), width = fminf(top - score_of(kmin), window), low = top - width, per = kBins / width;
+    if (kmax - kmin >= kBins && per > 0.0f && per < __builtin_inff()) {
+        auto even = [&](unsigned k) {
+            const float b = (score_of(k) - low) * per;
+            return b > 0.0f ? b < kBins - 1 ? (unsigned)b : kBins - 1u : 0u;
+        };
+        u64 rest = need;
+        level<N, Bin>(s, rest, share, at, each, even);
+        listed = list<N, Bin>(s, at, mine, value, each, even);
+        if (listed <= kRanked) return rank(s, listed, mine, rest, key, left);
+        if (listed <= N) {
+            need = rest;
+            kmin = mine ? mine : 0xffffffffu;
+            kmax = mine;
+            unsigned some = 0;
+            block_extent<N>(kmin, kmax, some, s.x);
+        }
+    }
     int shift = 0;
     while (((kmax - kmin) >> shift) >= kBins) shift++;
-    unsigned lo = kmin, bins = kBins, listed = N + 1, mine = 0;
-    u64 value = 0;
+    unsigned lo = kmin, bins = kBins;
+    auto listed_ones = [&](auto f) {
+        if (mine) f(mine, (Bin)value);
+    };
     for (;;) {
-        if (listed > N)
-            level<N, Bin>(s, lo, shift, bins, need, share, key, each);
-        else
-            level<N, Bin>(s, lo, shift, bins, need, share, key, [&](auto f) {
-                if (mine) f(mine, (Bin)value);
-            });
-        if (shift == 0) break;
-        lo = key;
-        if (listed > N) {
-            each([&](unsigned k, Bin v) {
-                if (k < lo || ((k - lo) >> shift)) return;
-                const unsigned at = atomicAdd(&s.listed, 1u);
-                if (at >= N) return;
-                s.list_k[at] = k;
-                s.list_v[at] = v;
-            });
-            __syncthreads();
-            listed = s.listed;
-            if (listed <= N && threadIdx.x < listed) {
-                mine = s.list_k[threadIdx.x];
-                value = s.list_v[threadIdx.x];
-            }
-            if (listed <= kRanked) {
-                if (mine) {
-                    u64 above = 0, with = 0;
-                    for (unsigned i = 0; i < listed; i++) {
-                        const unsigned k = s.list_k[i];
-                        const u64 w = s.list_v[i];
-                        above += k > mine ? w : 0;
-                        with += k >= mine ? w : 0;
-                    }
-                    if (above < need && need <= with) {  // (one key; its ties say the same)
-                        s.key = mine;
-                        s.left = need - above;
-                    }
-                }
-                __syncthreads();
-                key = s.key;
-                need = s.left;
-                break;
-            }
+        auto bits = [&](unsigned k) { return k < lo || ((k - lo) >> shift) >= bins ? (unsigned)kBins : (k - lo) >> shift; };
+        if (listed > N) level<N, Bin>(s, need, share, at, each, bits);
+        else level<N, Bin>(s, need, share, at, listed_ones, bits);
+        if (shift && listed > N) {
+            listed = list<N, Bin>(s, at, mine, value, each, bits);
+            if (listed <= kRanked) return rank(s, listed, mine, need, key, left);
         }
+        lo += at << shift;
+        if (shift == 0) break;
         bins = shift > kBinBits ? kBins : 1u << shift;
         shift = shift > kBinBits ? shift - kBinBits : 0;
     }
+    key = lo;
     left = need;
+}
+
+// Scores that a descent of counts sets apart: those whose weights are above e^-128,
+// mostly all.  (What masks leave lies far below; 0 of temperature 0: all of them.)
+__device__ __forceinline__ float count_window(const SampleArgs &a) {
+    return a.temperature > 0.0 ? (float)(128.0 * a.temperature) : __builtin_inff();
 }
 
 // A row's kept places from its n keys in s_key (N K of them in place order, 0:
@@ -393,7 +433,7 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, int row, RowShar
     unsigned thr = 0;   // places with a larger key are kept,
     u64 quota = ~0ull;  // and this many of those with this key
     if (top_k > 0 && (unsigned)top_k < count)
-        descend<N, unsigned>(s, kmin, kmax, (u64)top_k, 0.0,
+        descend<N, unsigned>(s, kmin, kmax, count_window(a), (u64)top_k, 0.0,
             [&](auto f) {
 #pragma unroll
                 for (int j = 0; j < K; j++)
@@ -404,7 +444,8 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, int row, RowShar
         const unsigned thr_k = thr;
         const u64 quota_k = quota;
         u64 left;
-        descend<N, u64>(s, kmin, kmax, 0, a.top_p,
+        // (a mass is a multiple of 2^-51 at least: nothing 37 temperatures below the best has any)
+        descend<N, u64>(s, kmin, kmax, (float)(37.0 * a.temperature), 0, a.top_p,
             [&](auto f) {
 #pragma unroll
                 for (int j = 0; j < K; j++)
@@ -504,6 +545,10 @@ __global__ __launch_bounds__(N) void sample_row_kernel(SampleArgs a) {
 
 constexpr int kTrimThreads = 1024, kTrimOwn = 8, kTrimKept = kTrimThreads * kTrimOwn;
 
+__device__ __forceinline__ unsigned below(u64 lanes) {  // how many of them lie below this one
+    return __builtin_amdgcn_mbcnt_hi((unsigned)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)lanes, 0));
+}
+
 template <int K>
 __global__ __launch_bounds__(kTrimThreads) void sample_trim_kernel(SampleArgs a) {
     constexpr int N = kTrimThreads, kWaves = N / 64;
@@ -524,27 +569,33 @@ __global__ __launch_bounds__(kTrimThreads) void sample_trim_kernel(SampleArgs a)
     unsigned thr = 0;
     u64 quota = 0;
     if ((unsigned)top_k < count)
-        descend<N, unsigned>(s, kmin, kmax, (u64)top_k, 0.0,
+        descend<N, unsigned>(s, kmin, kmax, count_window(a), (u64)top_k, 0.0,
             [&](auto f) {
 #pragma unroll
                 for (int j = 0; j < K; j++)
                     if (j < steps && key[j]) f(key[j], 1u);
             },
             thr, quota);
-    const u64 below = (1ull << (tid & 63)) - 1;
-    const int wave = tid >> 6;
+    // 64 neighbouring places are a wave's j-th: lane j has their counts, then
+    // what lies before them
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    unsigned above = 0, tied = 0;
 #pragma unroll
     for (int j = 0; j < K; j++) {
-        const u64 above = __ballot(key[j] > thr), tied = __ballot(key[j] && key[j] == thr);
-        if ((tid & 63) == 0) {
-            s_above[j * kWaves + wave] = __popcll(above);
-            s_tied[j * kWaves + wave] = __popcll(tied);
-        }
+        if (j >= steps) break;
+        const unsigned more = __popcll(__ballot(key[j] > thr)), same = thr ? __popcll(__ballot(key[j] == thr)) : 0;
+        above = lane == j ? more : above;
+        tied = lane == j ? same : tied;
+    }
+    if (lane < K) {
+        s_above[lane * kWaves + wave] = above;
+        s_tied[lane * kWaves + wave] = tied;
     }
     for (int i = tid; i < kTrimKept; i += N) s_key[i] = 0;
     __syncthreads();
     const bool mine = tid < K * kWaves;
-    const unsigned above = mine ? s_above[tid] : 0, tied = mine ? s_tied[tid] : 0;
+    above = mine ? s_above[tid] : 0;
+    tied = mine ? s_tied[tid] : 0;
     unsigned past_above = above, past_tied = tied, every, ties;
     block_scan2<N, unsigned, unsigned>(past_above, past_tied, s.x, s.x + kWaves, every, ties);
     if (mine) {
@@ -552,15 +603,20 @@ __global__ __launch_bounds__(kTrimThreads) void sample_trim_kernel(SampleArgs a)
         s_tied[tid] = past_tied - tied;
     }
     __syncthreads();
+    above = s_above[(lane & (K - 1)) * kWaves + wave];
+    tied = s_tied[(lane & (K - 1)) * kWaves + wave];
+    const unsigned some = (unsigned)quota;  // of the ties (at most top_k)
 #pragma unroll
     for (int j = 0; j < K; j++) {
-        const u64 tied_here = __ballot(key[j] && key[j] == thr);
-        const u64 before = s_tied[j * kWaves + wave];
-        const bool in = key[j] > thr || (key[j] && key[j] == thr && before + __popcll(tied_here & below) < quota);
-        const u64 kept = __ballot(in);
-        if (in) {
-            const unsigned to = s_above[j * kWaves + wave] + (unsigned)(before < quota ? before : quota) +
-                                (unsigned)__popcll(kept & below);
+        if (j >= steps) break;
+        u64 in = __ballot(key[j] > thr);
+        const unsigned before = lane_of(tied, j), first = before < some ? before : some;
+        if (before < some) {
+            const u64 here = __ballot(key[j] == thr);
+            in |= (unsigned)__popcll(here) <= some - before ? here : __ballot(key[j] == thr && below(here) < some - before);
+        }
+        if (in >> lane & 1) {
+            const unsigned to = lane_of(above, j) + first + below(in);
             s_key[to] = key[j];
             s_place[to] = (unsigned short)(j * N + tid);
         }
