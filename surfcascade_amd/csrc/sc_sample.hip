@@ -272,14 +272,17 @@ struct RowShared {
 // One level of a descent: the bin where the sum of each()'s members from the top
 // reaches need (need = 0: share of the whole) -> `at`, and what is still needed
 // from it.  each(f) calls f(k, v) for every member's key and what it counts for;
-// bin_of(k) >= kBins: not in this level.
+// bin_of(k) >= kBins: not in this level (all of them sum to less than need: so `at`).
 template <int N, class Bin, class Each, class Map>
 __device__ __forceinline__ void level(RowShared<N> &s, u64 &need, double share, unsigned &at, Each each, Map bin_of) {
     constexpr int kPer = kBins / N;
     Bin *bin = reinterpret_cast<Bin *>(s.bins);
     for (int i = threadIdx.x; i < kBins; i += N) bin[i] = 0;
     __syncthreads();
-    if (threadIdx.x == 0) s.listed = 0;  // (behind the barrier: what was listed last has been read)
+    if (threadIdx.x == 0) {  // (behind the barrier: what was found and listed last has been read)
+        s.listed = 0;
+        s.key = kBins;
+    }
     each([&](unsigned k, Bin v) {
         const unsigned b = bin_of(k);
         if (b < kBins) atomicAdd(&bin[b], v);
@@ -349,26 +352,27 @@ __device__ __forceinline__ void rank(RowShared<N> &s, unsigned listed, unsigned 
 
 // Descent: the largest key at which the pool's sum from the top reaches need
 // (need = 0: share of the whole), and what its ties still have to bring.
-// The first level's bins are even steps of the score over its range, `window` at
-// most, below which there is one bin: that spreads most pools over all of them,
-// while the keys' own leading bits put a normal distribution into some twenty,
-// where the atomics wait for each other (20011 scores: 6 us).  The bin where the
-// sum crosses is listed, and ranked if it has at most kRanked members.  If it does
-// not fit, the levels are 11 bits of the key each, until it does.
+// The first level's bins are even steps of the score, `window` down from the best
+// at most: that spreads most pools over all of them, while the keys' own leading
+// bits put a normal distribution into some twenty, and masks into one, where the
+// atomics wait for each other (20011 scores: 6 us).  The bin where the sum crosses
+// is listed, and ranked if it has at most kRanked members.  Without such a bin, or
+// if it does not fit, the levels are 11 bits of the key each, until one does.
 template <int N, class Bin, class Each>
 __device__ __forceinline__ void descend(RowShared<N> &s, unsigned kmin, unsigned kmax, float window, u64 need, double share,
                                         Each each, unsigned &key, u64 &left) {
     unsigned listed = N + 1, mine = 0, at;
     u64 value = 0;
-    const float top = score_of(kmax), width = fminf(top - score_of(kmin), window), low = top - width, per = kBins / width;
+    const float top = score_of(kmax), range = top - score_of(kmin), width = fminf(range, window), per = kBins / width;
+    const float low = range < window ? score_of(kmin) : top - width;  // (the whole range loses no score to a rounding)
     if (kmax - kmin >= kBins && per > 0.0f && per < __builtin_inff()) {
         auto even = [&](unsigned k) {
             const float b = (score_of(k) - low) * per;
-            return b > 0.0f ? b < kBins - 1 ? (unsigned)b : kBins - 1u : 0u;
+            return b >= 0.0f ? b < kBins - 1 ? (unsigned)b : kBins - 1u : (unsigned)kBins;
         };
         u64 rest = need;
         level<N, Bin>(s, rest, share, at, each, even);
-        listed = list<N, Bin>(s, at, mine, value, each, even);
+        if (at < kBins) listed = list<N, Bin>(s, at, mine, value, each, even);
         if (listed <= kRanked) return rank(s, listed, mine, rest, key, left);
         if (listed <= N) {
             need = rest;
@@ -402,10 +406,8 @@ __device__ __forceinline__ void descend(RowShared<N> &s, unsigned kmin, unsigned
 }
 
 // Scores that a descent of counts sets apart: those whose weights are above e^-128,
-// mostly all.  (What masks leave lies far below; 0 of temperature 0: all of them.)
-__device__ __forceinline__ float count_window(const SampleArgs &a) {
-    return a.temperature > 0.0 ? (float)(128.0 * a.temperature) : __builtin_inff();
-}
+// mostly all.  (What masks leave lies far below.)
+__device__ __forceinline__ float count_window(const SampleArgs &a) { return (float)(128.0 * a.temperature); }
 
 // A row's kept places from its n keys in s_key (N K of them in place order, 0:
 // absent), and the draws.  Thread t has the `own` <= K neighbouring ones from
@@ -432,7 +434,10 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, int row, RowShar
     }
     unsigned thr = 0;   // places with a larger key are kept,
     u64 quota = ~0ull;  // and this many of those with this key
-    if (top_k > 0 && (unsigned)top_k < count)
+    if (top_k == 1) {
+        thr = kmax;
+        quota = 1;
+    } else if (top_k > 0 && (unsigned)top_k < count)
         descend<N, unsigned>(s, kmin, kmax, count_window(a), (u64)top_k, 0.0,
             [&](auto f) {
 #pragma unroll
@@ -444,7 +449,7 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, int row, RowShar
         const unsigned thr_k = thr;
         const u64 quota_k = quota;
         u64 left;
-        // (a mass is a multiple of 2^-51 at least: nothing 37 temperatures below the best has any)
+        // (a mass is a multiple of 2^-51 at most: a place 37 temperatures below the best has none)
         descend<N, u64>(s, kmin, kmax, (float)(37.0 * a.temperature), 0, a.top_p,
             [&](auto f) {
 #pragma unroll
@@ -568,7 +573,10 @@ __global__ __launch_bounds__(kTrimThreads) void sample_trim_kernel(SampleArgs a)
     const int top_k = a.temperature == 0.0 ? 1 : a.top_k;  // 1 .. kTrimKept
     unsigned thr = 0;
     u64 quota = 0;
-    if ((unsigned)top_k < count)
+    if (top_k == 1) {
+        thr = kmax;
+        quota = 1;
+    } else if ((unsigned)top_k < count)
         descend<N, unsigned>(s, kmin, kmax, count_window(a), (u64)top_k, 0.0,
             [&](auto f) {
 #pragma unroll
@@ -1135,11 +1143,13 @@ void launch_step(const SampleArgs &a, hipStream_t s) {
 // a grid of 1024 threads a row has at most kGridRows (fewer than 2^32 threads).
 constexpr int kRowScores = 8192, kTrimScores = 32768, kSplitRows = 512, kGridRows = 1 << 21;
 
-// (top_k 3277 alone on one row of 32768: 41 us trimmed, 33 split, but 64 rows 42 and
-// 47; with top_p too 46 and 49, 64 rows 46 and 75)
+// (one row of 20011, top_k 2001 alone: 128 draws 25 us trimmed and 32 split, 4096
+// draws 31 and 34, with top_k 6670 43 and 34, with top_p too 35 and 50; 16 rows of
+// 32768, 4096 draws, top_k 3276: 42 and 64)
 static bool trim(const SampleArgs &a) {
     const bool few = a.temperature == 0.0 || (a.top_k > 0 && a.top_k <= kTrimKept);
-    return few && a.V <= kTrimScores && (a.V <= kTrimScores / 2 || a.B >= 32 || a.top_p < 1.0);
+    const bool light = a.V <= kTrimScores / 2 || a.S <= 1024 || a.B >= 8 || a.top_p < 1.0 || a.temperature == 0.0;
+    return few && light && a.V <= kTrimScores;
 }
 static bool split(const SampleArgs &a) { return a.V > kRowScores && !trim(a); }
 

@@ -3,6 +3,8 @@ sorting what the kernel selects.  Places are whole numbers and have to be
 equal.  Weights are rounded to units of 2^-36 at most and cumulated weights
 differ from numpy's by about 1e-13 of a typical weight, so a random number
 would have to lie that near to a border for another place."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -315,3 +317,19 @@ def test_more_draws_than_a_grid_has(tr):
     idx, kept = tr.sample(torch.zeros(1, v, device="cuda"), u)
     assert int(kept) == v
     assert bool((idx.view(reps, v) == place.int()).all())
+
+
+@pytest.mark.parametrize("v", [700, 5000, 20000])
+@pytest.mark.parametrize("temperature", [1e-3, 1.0, 1e4])
+@pytest.mark.parametrize("at,scale", [(0.0, 2.0), (1.0e6, 2.0), (-3.0e7, 40.0), (0.0, 1.0e30), (0.0, 1.0e-30)])
+def test_scores_far_from_zero(tr, at, scale, temperature, v):
+    """Ranges from a few roundings of the scores to more than float32 holds, with
+    a mask of the lowest value or without one, weights from all equal to one."""
+    g = torch.Generator().manual_seed(v)
+    scores = at + scale * torch.randn(4, v, generator=g)
+    scores[1, ::3] = torch.finfo(torch.float32).min
+    scores[2, 5::7] = torch.finfo(torch.float32).max
+    scores[3, 11] = math.inf
+    u = torch.rand(4, 9, generator=g, dtype=torch.float64)
+    for trim in (dict(top_k=v // 3), dict(top_k=40), dict(top_p=0.7), dict(top_k=v // 3, top_p=0.9)):
+        _check(tr, scores, u, temperature=temperature, **trim)
