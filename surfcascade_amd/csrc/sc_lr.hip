@@ -32,9 +32,7 @@
 //   responses, 2001 x 608, f16, 16 sets          60 us, 3.5 TB/s
 //   loss and gradient, 8191 x 608, bf16, 16 sets 129 us, 2.5 TB/s (the VALU, 68 %
 //     of the cycles: the sigmoid, its loss and the operand splits of 80 M results)
-//   gradient, 480 x 11870, bf16, 8 sets, dres   198 us, 3.8 TB/s (memory: one or
-//     two learners per wave, loads and stores past the caches, neighbours on one
-//     XCD, 2 or 4 waves per SIMD all take that)
+//   gradient, 480 x 11870, bf16, 8 sets, dres   171 us, 4.4 TB/s
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -849,7 +847,7 @@ __global__ __launch_bounds__(64 * kWideWaves) void lr_wide_bf16_kernel(LrArgs a)
 // dy, dres and the arithmetic of g fill the wave.  8191 x 608 x 8, alone and in
 // pairs: loss 127 and 108 us in bf16, 189 and 159 in f16, gradient 143 and 103,
 // 168 and 146; f32 206 and 253, 197 and 196 (it has no registers for two).  480 x
-// 11870 x 8 with dres: 198 us either way, the memory's.
+// 11870 x 8 with dres: 198 and 171.
 template <class T>
 struct PairTile {
     WideMeta v;
@@ -1119,10 +1117,12 @@ void launch_mode(const LrArgs &a, dim3 grid, hipStream_t s) {
 }  // namespace
 
 // Gradient and loss: rows are cut into chunks, of `ranges` waves' rows each.
-// The grid runs in rounds of as many waves as the registers of 256 CUs hold
-// (room), so the time is about rounds x (rows per wave + what a wave's start
-// and end cost, some 48 rows' time): the best of 1 to 4 full rounds.
-static int rows_per_wave(long long R, long long waves, int ranges, int step, long long room) {
+// Time goes in steps of as many waves as the registers of 256 CUs hold (room),
+// each of a wave's rows and what its start and end cost (some 48 rows' time), and
+// an eighth of one for the last waves; `join` is what a wave's partial sums cost,
+// written and read again, beside a row, and 24 rows the launch that does it.  The
+// best of 1 to 4 full rounds of waves.
+static int rows_per_wave(long long R, long long waves, int ranges, int step, long long room, int join) {
     if (R <= 16 * ranges) return (int)(ceil_div(ceil_div(R, ranges), step) * step);  // one chunk: nothing to join
     const long long most = ceil_div(R, (long long)ranges * step);
     long long best = -1;
@@ -1131,7 +1131,9 @@ static int rows_per_wave(long long R, long long waves, int ranges, int step, lon
         long long chunks = rounds * room / waves;
         chunks = chunks < 1 ? 1 : chunks > most ? most : chunks;
         const long long rows = ceil_div(ceil_div(R, chunks * ranges), step) * step;
-        const long long cost = ceil_div(waves * ceil_div(R, rows * ranges), room) * (rows + 48);
+        const long long all = waves * ceil_div(R, rows * ranges);
+        long long cost = ((all > room ? all : room) + room / 8) * (rows + 48);
+        if (join && all > waves) cost += join * all + 24 * room;
         if (best >= 0 && cost >= best) continue;
         best = cost;
         found = (int)rows;
@@ -1149,9 +1151,9 @@ LrPlan lr_plan(const LrArgs &a) {
     if (a.R == 0 || a.M == 0 || a.H == 0) return p;
     // (a chunk of the narrow form is one range of rows per wave of a workgroup)
     const int ranges = wide(a) ? 1 : kWaves;
-    p.rows_per_wave = wide(a) ? rows_per_wave(a.R, wide_grad_waves(a), 1, 16, 4096)
+    p.rows_per_wave = wide(a) ? rows_per_wave(a.R, wide_grad_waves(a), 1, 16, 4096, 20)
                               : rows_per_wave(a.R, narrow_waves(a) * kWaves, kWaves, lanes_per_item(a),
-                                              1024 * (a.H == 1 ? 6 : a.H == 2 ? 4 : 3));
+                                              1024 * (a.H == 1 ? 6 : a.H == 2 ? 4 : 3), 0);
     p.chunks = (int)ceil_div(a.R, (long long)p.rows_per_wave * ranges);
     if (p.chunks > 1) p.part_bytes = (size_t)p.chunks * a.M * a.H * kPartWords * sizeof(float);
     return p;
@@ -1182,15 +1184,19 @@ void launch_lr_grad(const LrArgs &a, bool loss, hipStream_t s) {
         const long long blocks = ceil_div((long long)a.M * a.H * kDesc, 256);
         hipLaunchKernelGGL(lr_zero_kernel, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, s, a, loss ? 1 : 0);
     }
-    const int joins = a.chunks > 1 ? (int)ceil_div((long long)a.M * a.H * kPartWords, a.chunks > 32 ? 32 : 64) : 0;
+    // threads over the chunks of a word: 32 of many chunks, 4, or 1 of a few (2 chunks
+    // of 480 x 11870 x 8: 28 us with 4, 15 with 1)
+    const int subs = a.chunks > 32 ? 32 : a.chunks > 4 ? 4 : 1, block = subs == 32 ? 1024 : 256;
+    const int joins = a.chunks > 1 ? (int)ceil_div((long long)a.M * a.H * kPartWords, block / subs) : 0;
     // a wave per row, or 16 lanes where rows are short
-    const int lanes = (long long)a.M * a.H > 64 ? 64 : 16, block = a.chunks > 32 ? 1024 : 256;
+    const int lanes = (long long)a.M * a.H > 64 ? 64 : 16;
     long long sums = !loss && a.res_kind == SC_RES_ROW ? ceil_div(a.R, block / lanes) : 0;
     if (sums > 4096) sums = 4096;
     if (joins + sums == 0) return;
     const dim3 grid((unsigned)(joins + sums));
-    if (block == 1024) hipLaunchKernelGGL((lr_tail_kernel<32, 32>), grid, dim3(block), 0, s, a, loss ? 1 : 0, joins, lanes);
-    else hipLaunchKernelGGL((lr_tail_kernel<4, 64>), grid, dim3(block), 0, s, a, loss ? 1 : 0, joins, lanes);
+    if (subs == 32) hipLaunchKernelGGL((lr_tail_kernel<32, 32>), grid, dim3(block), 0, s, a, loss ? 1 : 0, joins, lanes);
+    else if (subs == 4) hipLaunchKernelGGL((lr_tail_kernel<4, 64>), grid, dim3(block), 0, s, a, loss ? 1 : 0, joins, lanes);
+    else hipLaunchKernelGGL((lr_tail_kernel<1, 256>), grid, dim3(block), 0, s, a, loss ? 1 : 0, joins, lanes);
 }
 
 }  // namespace sc

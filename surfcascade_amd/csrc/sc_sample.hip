@@ -13,19 +13,22 @@
 // no sort.  Weights are doubles and masses integers (sample_shift), so a sum
 // is the same in any order and a draw never depends on how the row was split.
 //
-// The threshold comes from a radix descent of 11 bits a pass over the row's own
-// key range: bins hold counts for top_k, masses for top_p, and the bin where
-// the sum from the top crosses is split again.  Cumulated masses then need one
-// pass in place order, and a draw is a search through them.
+// The threshold comes from a descent: bins hold counts for top_k, masses for
+// top_p, and the bin where the sum from the top crosses is split again, by 11
+// bits of the key a level, over many workgroups; in one workgroup the first
+// level's bins are even steps of the score and the crossing bin's few members are
+// ranked.  Cumulated masses then need one pass in place order, and a draw is a
+// search through them.
 //
-// Short rows: one workgroup each, one launch; a thread holds its keys and masses
-// in registers through all passes.  Long rows: many workgroups, one launch per
-// pass.  Scores are few bytes (1 M of them: 4 MB, 1 us): what bounds the short
-// form is one CU's issue (a weight is some 40 instructions, half of them in 64
-// bits) and a pass' barriers, the long form its launches, 4 to 12 us each, of
-// which most is waiting for the bins of the one before.  Measured (one MI355X):
-//   960 scores, 960 draws                                 7 us
-//   32 rows x 20011, top_k 2000, top_p, min_p, 128 draws  38 us (split: 60)
+// Short rows, and longer ones of which top_k keeps few: one workgroup each, one
+// launch; a thread holds its keys and masses in registers through all passes.
+// Other rows: many workgroups, one launch per pass.  Scores are few bytes (1 M of
+// them: 4 MB, 1 us): what bounds the first form is one CU's issue (a weight is
+// some 40 instructions, half of them in 64 bits) and a pass' barriers, the second
+// its launches, 4 to 13 us each, of which most is waiting for the bins of the one
+// before.  Measured (one MI355X):
+//   960 scores, 960 draws                                 7 us, top_k and top_p 13
+//   32 rows x 20011, top_k 2000, top_p, min_p, 128 draws  30 us (split: 60)
 //   1000003 scores, top_k 500000, top_p, 16384 draws      63 us
 //   64 rows x 128256, one draw, no trim 50 us, top_p 121 us
 #include <hip/hip_runtime.h>
