@@ -30,7 +30,7 @@
 //   responses, 16384 x 608, f32, 1 set          221 us, 5.9 TB/s
 //   loss and gradient, 16384 x 608, f32, 1 set  219 us, 5.8 TB/s
 //   responses, 2001 x 608, f16, 16 sets          60 us, 3.5 TB/s
-//   loss and gradient, 8191 x 608, bf16, 16 sets 129 us, 2.5 TB/s (the VALU, 68 %
+//   loss and gradient, 8191 x 608, bf16, 16 sets 130 us, 2.5 TB/s (the VALU, 68 %
 //     of the cycles: the sigmoid, its loss and the operand splits of 80 M results)
 //   gradient, 480 x 11870, bf16, 8 sets, dres   171 us, 4.4 TB/s
 #include <hip/hip_runtime.h>
