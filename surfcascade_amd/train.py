@@ -45,6 +45,7 @@ class Trainer:
         self.device = int(device)
         self._dev = torch.device("cuda", self.device)
         self._f32, self._f64, self._i32 = torch.float32, torch.float64, torch.int32
+        self._like = torch.empty_like
         self._ws = None
         h = ctypes.c_void_p()
         _check(self._L.sc_trainer_create(self.device, ctypes.byref(h)))
@@ -106,15 +107,16 @@ class Trainer:
             raise ValueError("rows of %s overlap (strides %s)" % (what, stride))
         return t.data_ptr(), max(stride[0], cols)
 
-    def _no_grad(self, *operands):
-        for t in operands:
-            if t is not None and t.requires_grad and self._torch.is_grad_enabled():
-                raise ValueError("results carry no autograd history: detach the operands (response_grad and loss "
-                                 "return gradients)")
+    def _no_grad(self, *wanted):
+        """wanted: the operands' requires_grad"""
+        if any(wanted) and self._torch.is_grad_enabled():
+            raise ValueError("results carry no autograd history: detach the operands (response_grad and loss "
+                             "return gradients)")
 
     def _operands(self, samples, w, b, patch, rows):
         f32, i32 = self._f32, self._i32
-        self._no_grad(samples, w, b)
+        if w.requires_grad or samples.requires_grad or (b is not None and b.requires_grad):
+            self._no_grad(True)
         dtype = self._dtypes.get(samples.dtype)
         if dtype is None or samples.get_device() != self.device:
             raise ValueError("samples must be float32, float16 or bfloat16 on cuda:%d (got %s on %s)"
@@ -172,7 +174,7 @@ class Trainer:
         x, k, r, sets, cols = self._operands(samples, w, b, patch, rows)
         res, kind, res_ld = None, 0, 0
         if residual is not None:
-            self._no_grad(residual)
+            self._no_grad(residual.requires_grad)
             if residual.dim() == 1:
                 kind, res_ld = 1, residual.stride(0)
                 if residual.shape[0] != r or residual.dtype is not self._f32 \
@@ -199,10 +201,10 @@ class Trainer:
         residual: None or "none", "row" or "full", the residual's kind."""
         self._follow()
         x, k, r, sets, cols = self._operands(samples, w, b, patch, rows)
-        self._no_grad(grad_out)
+        self._no_grad(grad_out.requires_grad)
         dy, dy_ld = self._rowwise(grad_out, self._f32, r, cols, "grad_out")
         kind = _RES[residual]
-        dw, db, dres, dr = w.new_empty(w.shape), w.new_empty(sets), None, None
+        dw, db, dres, dr = self._like(w), w.new_empty(sets) if b is None else self._like(b), None, None
         if kind:
             dres = w.new_empty((r,) if kind == 1 else (r,) + sets)
             dr = dres.data_ptr()
@@ -222,11 +224,12 @@ class Trainer:
         float32 [n], by sample; a sample of weight 0 is not looked at."""
         self._follow()
         x, k, r, sets, cols = self._operands(samples, w, b, patch, rows)
-        self._no_grad(target, weight)
+        self._no_grad(target.requires_grad, weight is not None and weight.requires_grad)
         n = samples.shape[0]
         t = self._need(target, self._f32, (n,), "target")
         c = None if weight is None else self._need(weight, self._f32, (n,), "weight") or None
-        loss, dw, db = w.new_empty(sets), w.new_empty(w.shape), w.new_empty(sets)
+        db, dw = w.new_empty(sets) if b is None else self._like(b), self._like(w)
+        loss = self._like(db)
 
         def call(ws, ws_bytes):
             return self._L.sc_lr_loss(self._h, x, k, t, c, loss.data_ptr(), dw.data_ptr(), db.data_ptr(), ws, ws_bytes)
@@ -248,7 +251,7 @@ class Trainer:
         [b, s], in [0, 1)) -> (index int32 like u, kept int32 [b])
         (sc_sample).  lens: int32 [b], the length of each row."""
         self._follow()
-        self._no_grad(scores)
+        self._no_grad(scores.requires_grad)
         dtype, dim = self._dtypes.get(scores.dtype), scores.dim()
         if dtype is None or scores.get_device() != self.device:
             raise ValueError("scores must be float32, float16 or bfloat16 on cuda:%d (got %s on %s)"
@@ -265,7 +268,7 @@ class Trainer:
         up, u_ld = self._rowwise(u, self._f64, b, s, "u")
         ln = None if lens is None else self._need(lens, self._i32, (b,), "lens") or None
         index = u.new_empty(shape, dtype=self._i32)
-        kept = index.new_empty((b,))
+        kept = index.new_empty(b)
         most = 2**31 - 1  # (a C int; the library refuses rows that long, and such a top_k keeps all)
         prm = _SampleParams(temperature, min(top_k, most), top_p, min_p)
         if v > most or s > most or b > most:
