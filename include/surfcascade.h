@@ -279,8 +279,9 @@ int sc_lr_workspace(const sc_samples *x, const sc_weak_bank *k, size_t *bytes);
  *   g = alpha * dy * act'(z), 0 for an absent row or learner
  *   dw[j][k] = sum_r g x[row r, patch j], db[j][k] = sum_r g
  *   dres = beta * dy, summed over a row's results for SC_RES_ROW
- * (dres NULL with SC_RES_NONE; no result overlaps another operand).  Sums over rows in 32 bits over a chunk of
- * rows and in 64 bits over the chunks, dres sums in 64 bits.  A g that is
+ * (dres NULL with SC_RES_NONE; no result overlaps another operand).  Sums over
+ * rows in 32 bits over a chunk of rows (at most 2048 to a running sum, and at
+ * most four of these), in 64 bits over the chunks; dres sums in 64 bits.  A g that is
  * infinite or NaN leaves its learner's and set's dw and db so.  There is no
  * gradient of the descriptors: they are read off images. */
 int sc_lr_response_grad(sc_trainer *t, const sc_samples *x, const sc_weak_bank *k, int act,

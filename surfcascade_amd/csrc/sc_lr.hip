@@ -10,8 +10,8 @@
 // A (row, patch) descriptor is 128 B (64 B in 16 bits) that feeds 64 flops per
 // parameter set (128 with its gradient), so up to 16 sets the matrix' own bytes
 // are the bound: each descriptor is read once from memory and everything is done
-// on it in registers.  Sums over rows are in 32 bits within a chunk of them; the
-// chunks are joined in 64 bits in a fixed order (no atomics: the same call gives
+// on it in registers.  Sums over rows are in 32 bits within a chunk of them (a
+// wave's: 2048 at most); the chunks are joined in 64 bits in a fixed order (no atomics: the same call gives
 // the same bits).
 //
 // Up to kNarrowSets sets, the narrow form: one descriptor on LPI = 8 lanes (4 in
@@ -244,7 +244,7 @@ __global__ __launch_bounds__(64 * kWaves) void lr_kernel(LrArgs a) {
 #pragma unroll
         for (int e = 0; e < EPL; e++) acc[h][e] = 0.0f;
     }
-    const long long r_lo = (long long)range * a.rows_per_wave;
+    const long long r_lo = a.row0 + (long long)range * a.rows_per_wave;
     const int r0 = (int)(r_lo < a.R ? r_lo : a.R);
     const int r1 = (int)(r_lo + a.rows_per_wave < a.R ? r_lo + a.rows_per_wave : a.R);
     const char *x = static_cast<const char *>(a.x);
@@ -408,7 +408,7 @@ __device__ __forceinline__ void wide_rows(const LrArgs &a, WideUnit &u) {
     u.step = a.ld * T::kSize;
     u.in_order = !a.rows && u.step < (1 << 26);
     u.dense = a.dy_ld < (1 << 26) && a.dres_ld < (1 << 26);
-    const long long lo = (long long)blockIdx.y * a.rows_per_wave;
+    const long long lo = a.row0 + (long long)blockIdx.y * a.rows_per_wave;
     u.r0 = (int)(lo < a.R ? lo : a.R);
     u.r1 = (int)(lo + a.rows_per_wave < a.R ? lo + a.rows_per_wave : a.R);
 }
@@ -1021,12 +1021,13 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void lr_pair_kernel(LrArgs a) {
 
 // What follows the row chunks, in one launch.  The first `joins` workgroups join
 // their partial sums: WORDS neighbouring ones each, every one of SUBS rows of
-// threads walks every SUBS-th chunk, in 64 bits.  The others write the gradient
+// threads walks every SUBS-th chunk, in 64 bits; where the rows take several
+// launches, acc carries the sums from one's join to the next's.  The others write the gradient
 // of a residual of one value per row, beta * the sum of the row's dy: `lanes` of
 // a wave a row, in 64 bits.  (Loss of 8191 x 608 x 16: 13 chunks, 17 MB of
 // partial sums, 7.2 us; with 8 rows of 32 threads 8.5.)
 template <int SUBS, int WORDS>
-__global__ __launch_bounds__(WORDS * SUBS) void lr_tail_kernel(LrArgs a, int loss, int joins, int lanes) {
+__global__ __launch_bounds__(WORDS * SUBS) void lr_tail_kernel(LrArgs a, int loss, int joins, int lanes, int last) {
     if ((int)blockIdx.x >= joins) {
         const long long cols = (long long)a.M * a.H, rows = WORDS * SUBS / lanes;
         const int at = threadIdx.x & (lanes - 1);
@@ -1057,6 +1058,13 @@ __global__ __launch_bounds__(WORDS * SUBS) void lr_tail_kernel(LrArgs a, int los
     if (sub != 0 || i >= words) return;
 #pragma unroll
     for (int k = 1; k < SUBS; k++) s += s_sum[k][threadIdx.x];
+    if (a.acc) {
+        if (a.row0) s += a.acc[i];
+        if (!last) {
+            a.acc[i] = s;
+            return;
+        }
+    }
     const long long mh = i / kPartWords;
     const int word = (int)(i - mh * kPartWords);
     if (word < kDesc) a.dw[mh * kDesc + word] = (float)s;
@@ -1146,16 +1154,37 @@ static long long narrow_waves(const LrArgs &a) { return ceil_div(a.M, items_per_
 static long long wide_waves(const LrArgs &a) { return a.M * ceil_div(a.H, 16); }
 static long long wide_grad_waves(const LrArgs &a) { return pair(a) ? ceil_div(a.M, 2) : wide_waves(a); }
 
+// The rows of a wave's sums in 32 bits, whatever the occupancy would have: some
+// 2^11 roundings.  (w = 0 and equal weights, 600000 rows x 5000 x 16 of bf16: with
+// 200000 rows a wave, which fill the chip, loss and dw are off by 5e-4 and 1e-3 of
+// their values in 59 ms, with 2048 by 3e-6 and 7e-6 in 55; 400000 x 32768 of f32:
+// dw 1.5e-3 in 61 ms and 3e-5 in 56.)
+constexpr int kSumRows = 2048;
+// partial sums of one launch, where rows are cut for that reason alone
+constexpr size_t kPartBytes = (size_t)1 << 28;
+
 LrPlan lr_plan(const LrArgs &a) {
-    LrPlan p{0, 0, 0};
+    LrPlan p{0, 0, 0, 0, 0};
     if (a.R == 0 || a.M == 0 || a.H == 0) return p;
     // (a chunk of the narrow form is one range of rows per wave of a workgroup)
     const int ranges = wide(a) ? 1 : kWaves;
     p.rows_per_wave = wide(a) ? rows_per_wave(a.R, wide_grad_waves(a), 1, 16, 4096, 20)
                               : rows_per_wave(a.R, narrow_waves(a) * kWaves, kWaves, lanes_per_item(a),
                                               1024 * (a.H == 1 ? 6 : a.H == 2 ? 4 : 3), 0);
-    p.chunks = (int)ceil_div(a.R, (long long)p.rows_per_wave * ranges);
-    if (p.chunks > 1) p.part_bytes = (size_t)p.chunks * a.M * a.H * kPartWords * sizeof(float);
+    const long long fill = ceil_div(a.R, (long long)p.rows_per_wave * ranges);
+    if (p.rows_per_wave > kSumRows) p.rows_per_wave = kSumRows;
+    const long long chunks = ceil_div(a.R, (long long)p.rows_per_wave * ranges);
+    const size_t words = (size_t)a.M * a.H * kPartWords;
+    long long at_once = chunks;
+    if (chunks > fill) {  // as many as fill the chip, or as the memory above holds (grid y: 65535), evenly
+        at_once = (long long)(kPartBytes / (words * sizeof(float)));
+        at_once = at_once < fill ? fill : at_once > 65535 ? 65535 : at_once;
+        at_once = ceil_div(chunks, ceil_div(chunks, at_once));
+    }
+    p.chunks = (int)chunks;
+    p.at_once = (int)at_once;
+    if (chunks > 1) p.part_bytes = at_once * words * sizeof(float);
+    if (chunks > at_once) p.acc_bytes = words * sizeof(double);
     return p;
 }
 
@@ -1174,7 +1203,8 @@ void launch_lr_response(const LrArgs &a0, hipStream_t s) {
     launch_mode<kResponse>(a, grid, s);
 }
 
-void launch_lr_grad(const LrArgs &a, bool loss, hipStream_t s) {
+// the sums of one launch's chunks, their join and, behind the last, dres
+static void launch_chunks(const LrArgs &a, bool loss, bool last, hipStream_t s) {
     if (a.chunks > 0) {
         const dim3 grid = wide(a) ? dim3((unsigned)ceil_div(wide_grad_waves(a), kWideWaves), (unsigned)a.chunks)
                                   : dim3((unsigned)narrow_waves(a), (unsigned)a.chunks);
@@ -1187,16 +1217,30 @@ void launch_lr_grad(const LrArgs &a, bool loss, hipStream_t s) {
     // threads over the chunks of a word: 32 of many chunks, 4, or 1 of a few (2 chunks
     // of 480 x 11870 x 8: 28 us with 4, 15 with 1)
     const int subs = a.chunks > 32 ? 32 : a.chunks > 4 ? 4 : 1, block = subs == 32 ? 1024 : 256;
-    const int joins = a.chunks > 1 ? (int)ceil_div((long long)a.M * a.H * kPartWords, block / subs) : 0;
+    const int joins = a.part ? (int)ceil_div((long long)a.M * a.H * kPartWords, block / subs) : 0;
     // a wave per row, or 16 lanes where rows are short
     const int lanes = (long long)a.M * a.H > 64 ? 64 : 16;
-    long long sums = !loss && a.res_kind == SC_RES_ROW ? ceil_div(a.R, block / lanes) : 0;
+    long long sums = last && !loss && a.res_kind == SC_RES_ROW ? ceil_div(a.R, block / lanes) : 0;
     if (sums > 4096) sums = 4096;
     if (joins + sums == 0) return;
     const dim3 grid((unsigned)(joins + sums));
-    if (subs == 32) hipLaunchKernelGGL((lr_tail_kernel<32, 32>), grid, dim3(block), 0, s, a, loss ? 1 : 0, joins, lanes);
-    else if (subs == 4) hipLaunchKernelGGL((lr_tail_kernel<4, 64>), grid, dim3(block), 0, s, a, loss ? 1 : 0, joins, lanes);
-    else hipLaunchKernelGGL((lr_tail_kernel<1, 256>), grid, dim3(block), 0, s, a, loss ? 1 : 0, joins, lanes);
+    if (subs == 32) hipLaunchKernelGGL((lr_tail_kernel<32, 32>), grid, dim3(block), 0, s, a, loss ? 1 : 0, joins, lanes, last);
+    else if (subs == 4) hipLaunchKernelGGL((lr_tail_kernel<4, 64>), grid, dim3(block), 0, s, a, loss ? 1 : 0, joins, lanes, last);
+    else hipLaunchKernelGGL((lr_tail_kernel<1, 256>), grid, dim3(block), 0, s, a, loss ? 1 : 0, joins, lanes, last);
+}
+
+void launch_lr_grad(const LrArgs &a0, const LrPlan &p, void *ws, bool loss, hipStream_t s) {
+    LrArgs a = a0;
+    a.rows_per_wave = p.rows_per_wave;
+    a.acc = p.acc_bytes ? static_cast<double *>(ws) : nullptr;
+    a.part = p.part_bytes ? reinterpret_cast<float *>(static_cast<char *>(ws) + p.acc_bytes) : nullptr;
+    int from = 0;
+    do {
+        a.chunks = p.chunks - from < p.at_once ? p.chunks - from : p.at_once;
+        a.row0 = (int)((long long)from * p.rows_per_wave * (wide(a) ? 1 : kWaves));
+        from += a.chunks;
+        launch_chunks(a, loss, from == p.chunks, s);
+    } while (from < p.chunks);
 }
 
 }  // namespace sc

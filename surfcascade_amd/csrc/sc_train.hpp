@@ -40,22 +40,25 @@ struct LrArgs {
     // gradient / loss outputs
     float *dw, *db, *loss;
     float *part;        // partial sums per row chunk (NULL: one chunk, results written directly)
-    int chunks;         // row chunks (grid y)
+    double *acc;        // sums over the launches so far (NULL: one launch)
+    int row0;           // first row of a launch
+    int chunks;         // its row chunks (grid y)
     int rows_per_wave;  // rows a wave walks
 };
 
 constexpr int kPartWords = kDesc + 2;  // per learner and set: dW, db, loss
 
-// the launch shape of the gradient / loss kernels (workspace = part)
+// The launch shape of the gradient / loss kernels: the rows in `chunks`, of
+// which a launch has `at_once`.  Workspace: acc, then part.
 struct LrPlan {
-    int chunks, rows_per_wave;
-    size_t part_bytes;
+    int chunks, at_once, rows_per_wave;
+    size_t acc_bytes, part_bytes;
 };
 LrPlan lr_plan(const LrArgs &a);
 
 void launch_lr_response(const LrArgs &a, hipStream_t s);
-// sums per chunk, their join, and dres
-void launch_lr_grad(const LrArgs &a, bool loss, hipStream_t s);
+// sums per chunk, their join, and dres (acc, part and the launch shape from the plan)
+void launch_lr_grad(const LrArgs &a, const LrPlan &p, void *ws, bool loss, hipStream_t s);
 
 struct SampleArgs {
     const void *scores;

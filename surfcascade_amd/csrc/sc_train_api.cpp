@@ -160,12 +160,9 @@ void lr_pointers(const sc_trainer *t, const sc::LrArgs &a) {
     need_ptr(t, a.b, "b", true);
 }
 
-int lr_grad(sc_trainer *t, sc::LrArgs &a, bool loss, void *ws, size_t ws_bytes) {
+int lr_grad(sc_trainer *t, const sc::LrArgs &a, bool loss, void *ws, size_t ws_bytes) {
     const sc::LrPlan p = sc::lr_plan(a);
-    a.chunks = p.chunks;
-    a.rows_per_wave = p.rows_per_wave;
-    a.part = static_cast<float *>(workspace(t, p.part_bytes, ws, ws_bytes));
-    sc::launch_lr_grad(a, loss, t->stream);
+    sc::launch_lr_grad(a, p, workspace(t, p.acc_bytes + p.part_bytes, ws, ws_bytes), loss, t->stream);
     HIPCHK(hipGetLastError());
     return SC_OK;
 }
@@ -299,7 +296,8 @@ int sc_lr_workspace(const sc_samples *x, const sc_weak_bank *k, size_t *bytes) {
     return guarded([&] {
         need(bytes, "null argument");
         const sc::LrArgs a = lr_args(x, k);
-        *bytes = a.M && a.H ? sc::lr_plan(a).part_bytes : 0;
+        const sc::LrPlan p = sc::lr_plan(a);
+        *bytes = p.acc_bytes + p.part_bytes;
         return SC_OK;
     });
 }
