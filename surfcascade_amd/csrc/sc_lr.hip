@@ -169,21 +169,19 @@ __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf
 
 enum Mode { kResponse = 0, kGrad = 1, kLoss = 2 };
 
-// log(1 + e) / e for e in [0, 1], in units of `unit`: a polynomial of degree 8
-// fitted for the least relative error (3.0e-8; 3 roundings of 2^-24 as evaluated)
-__device__ __forceinline__ float log1p_over(float e, float unit) {
-    float p = 0.005232677f * unit;
-    p = __builtin_fmaf(p, e, -0.029505169f * unit);
-    p = __builtin_fmaf(p, e, 0.078225836f * unit);
-    p = __builtin_fmaf(p, e, -0.13663235f * unit);
-    p = __builtin_fmaf(p, e, 0.19106002f * unit);
-    p = __builtin_fmaf(p, e, -0.24842981f * unit);
-    p = __builtin_fmaf(p, e, 0.33319098f * unit);
-    p = __builtin_fmaf(p, e, -0.49999493f * unit);
-    return __builtin_fmaf(p, e, 0.99999994f * unit);
+// log(1 + e) / e for e in [0, 1]: a polynomial of degree 8 fitted for the least
+// relative error (3.0e-8; 3 roundings of 2^-24 as evaluated)
+__device__ __forceinline__ float log1p_over(float e) {
+    float p = 0.005232677f;
+    p = __builtin_fmaf(p, e, -0.029505169f);
+    p = __builtin_fmaf(p, e, 0.078225836f);
+    p = __builtin_fmaf(p, e, -0.13663235f);
+    p = __builtin_fmaf(p, e, 0.19106002f);
+    p = __builtin_fmaf(p, e, -0.24842981f);
+    p = __builtin_fmaf(p, e, 0.33319098f);
+    p = __builtin_fmaf(p, e, -0.49999493f);
+    return __builtin_fmaf(p, e, 0.99999994f);
 }
-
-constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
 // What a row brings to its results' gradients: for the loss its weight on
 // either side, pos = c (1 - t) and neg = c t; for a response pos = alpha dy.
@@ -191,15 +189,14 @@ constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 //   c (softplus(z) - t z) = c log(1 + e) + (z >= 0 ? pos : -neg) z
 //   c (sigmoid(z) - t)    = d (z >= 0 ? pos - neg e : pos e - neg)
 // neither of which takes a difference of nearly equal numbers.  A NaN z is a
-// NaN e, and stays one.  BITS: z comes, and the loss goes, in units of log 2
-// (a product less per result).
-template <int MODE, bool BITS = false>
+// NaN e, and stays one.
+template <int MODE>
 __device__ __forceinline__ float grad_of(int act, float z, float pos, float neg, float &loss) {
-    const float e = BITS ? __builtin_amdgcn_exp2f(-fabsf(z)) : __expf(-fabsf(z)), d = __builtin_amdgcn_rcpf(1.0f + e);
+    const float e = __expf(-fabsf(z)), d = __builtin_amdgcn_rcpf(1.0f + e);
     if constexpr (MODE == kLoss) {
         const bool up = z >= 0.0f;
         const float near = up ? pos : -neg, far = up ? -neg : pos;
-        loss = __builtin_fmaf((pos + neg) * e, log1p_over(e, BITS ? kLog2E : 1.0f), __builtin_fmaf(near, z, loss));
+        loss = __builtin_fmaf((pos + neg) * e, log1p_over(e), __builtin_fmaf(near, z, loss));
         return d * __builtin_fmaf(far, e, near);
     } else {
         return act == SC_ACT_SIGMOID ? pos * e * d * d : pos;
@@ -641,13 +638,13 @@ __device__ __forceinline__ void wide_grad(const LrArgs &a, const WideUnit &u, co
     if (MODE == kGrad && a.res_kind == SC_RES_FULL && on) store_dres(a, u, o, r, q, col, t.dy);
     if (t.whole) {
 #pragma unroll
-        for (int k = 0; k < 4; k++) g[k] = grad_of<MODE, __is_same(T, BF16)>(a.act, z[k], pos[k], neg[k], sum_l);
+        for (int k = 0; k < 4; k++) g[k] = grad_of<MODE>(a.act, z[k], pos[k], neg[k], sum_l);
     } else {
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             const bool there = u.present && __shfl(t.v.idx, q * 4 + k, 64) >= 0;
             float l = sum_l;
-            const float gk = grad_of<MODE, __is_same(T, BF16)>(a.act, z[k], pos[k], neg[k], l);
+            const float gk = grad_of<MODE>(a.act, z[k], pos[k], neg[k], l);
             g[k] = there ? gk : 0.0f;
             sum_l = there ? l : sum_l;
             if (!there) t.xc[k] = PlacePair<T>{};
@@ -749,12 +746,13 @@ __device__ __forceinline__ void split3(float v, unsigned &a, unsigned &b, unsign
 // two high halves -> one register, `lo` first
 __device__ __forceinline__ unsigned pack(unsigned lo, unsigned hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
 
-// a lane's 8 weights in units of 1 / log 2 (z comes in units of log 2 then)
+// a lane's 8 weights (as they are: times log 2's inverse, for an exponential with
+// a product less, the largest would be infinite)
 __device__ __forceinline__ void split_weights(const float (&wf)[8], uint4_v (&w)[3]) {
 #pragma unroll
     for (int k = 0; k < 4; k++) {
         unsigned lo[3], hi[3];
-        const float a = kLog2E * wf[2 * k], b = kLog2E * wf[2 * k + 1];
+        const float a = wf[2 * k], b = wf[2 * k + 1];
         split3(a, lo[0], lo[1], lo[2]);
         split3(b, hi[0], hi[1], hi[2]);
         if (__builtin_isinf(a)) lo[1] = lo[2] = 0;  // (an infinite weight's response is no NaN)
@@ -782,7 +780,7 @@ __global__ __launch_bounds__(64 * kWideWaves) void lr_wide_bf16_kernel(LrArgs a)
     load4(a.w + col * kDesc + 8 * q, on, wf);
     load4(a.w + col * kDesc + 8 * q + 4, on, wf + 4);
     split_weights(wf, w);
-    const float bias = on && a.b ? kLog2E * a.b[col] : 0.0f;
+    const float bias = on && a.b ? a.b[col] : 0.0f;
     const WideOffsets o = wide_offsets<T>(a, u, i, q, col);
     float4_v acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
     float sum_g = 0.0f, sum_l = 0.0f;
@@ -838,7 +836,7 @@ __global__ __launch_bounds__(64 * kWideWaves) void lr_wide_bf16_kernel(LrArgs a)
         m1 = wide_meta<MODE>(a, u, r + 112, i);
         products(r + 32, t[2], t[3]);
     }
-    wide_store<MODE>(a, acc, sum_g, kLn2 * sum_l, i, q, (long long)u.m * a.H + u.h0 + 4 * q, a.H - u.h0 - 4 * q, on, col);
+    wide_store<MODE>(a, acc, sum_g, sum_l, i, q, (long long)u.m * a.H + u.h0 + 4 * q, a.H - u.h0 - 4 * q, on, col);
 }
 
 // Up to 8 sets of 16-bit samples, a wave owns two neighbouring learners, lane i's
@@ -888,11 +886,8 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void lr_pair_kernel(LrArgs a) {
     uint4_v w[3];
 #pragma unroll
     for (int k = 0; k < 2; k++) load4(a.w + col * kDesc + WideRow<T>::place(q, k), on, wf + 4 * k);
-    float bias = on && a.b ? a.b[col] : 0.0f;
-    if constexpr (kBf16) {
-        bias *= kLog2E;
-        split_weights(wf, w);
-    }
+    const float bias = on && a.b ? a.b[col] : 0.0f;
+    if constexpr (kBf16) split_weights(wf, w);
     const WideOffsets o = wide_offsets<T>(a, u, i, q, col);
     float4_v acc[2][2] = {};
     float sum_g = 0.0f, sum_l = 0.0f;
@@ -950,11 +945,11 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void lr_pair_kernel(LrArgs a) {
                 pos = a.alpha * t.dy[k];
             }
             if (t.whole) {
-                g[k] = grad_of<MODE, kBf16>(a.act, zk, pos, neg, sum_l);
+                g[k] = grad_of<MODE>(a.act, zk, pos, neg, sum_l);
             } else {
                 const bool row = __shfl(t.v.idx, q * 4 + k, 64) >= 0;
                 float l = sum_l;
-                const float gk = grad_of<MODE, kBf16>(a.act, zk, pos, neg, l);
+                const float gk = grad_of<MODE>(a.act, zk, pos, neg, l);
                 g[k] = row && here ? gk : 0.0f;
                 sum_l = row && here ? l : sum_l;
                 if (!(row && present[0])) t.xc[0][k] = PlacePair<T>{};
@@ -1011,7 +1006,6 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void lr_pair_kernel(LrArgs a) {
         ahead = wide_meta<MODE>(a, u, r + 48, i);
         products(r + 16, two);
     }
-    if constexpr (kBf16) sum_l *= kLn2;
 #pragma unroll
     for (int half = 0; half < 2; half++) acc[0][half] = q >> 1 ? acc[1][half] : acc[0][half];
     // lane (i, q): places 2i and 2i+1 of the sets 4 (q % 2) .. of learner q / 2; sums: of its own set
