@@ -736,7 +736,10 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void lr_wide_kernel(LrArgs a) {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 // v = a + b + c, each a bfloat16 (8 + 8 + 8 bits of 24): the high halves (an
-// infinite v: a, and NaN for what is left of it)
+// infinite v: a, and NaN for what is left of it).  The products of an infinite
+// sample with the parts are NaN where a part is 0; a chunk whose sums come out
+// not finite is therefore summed again, `exact`: only v's first part meets such
+// samples, the others 0 in their place.
 __device__ __forceinline__ void split3(float v, unsigned &a, unsigned &b, unsigned &c) {
     a = __float_as_uint(v) & 0xffff0000u;
     const float r = v - __uint_as_float(a);
@@ -745,6 +748,45 @@ __device__ __forceinline__ void split3(float v, unsigned &a, unsigned &b, unsign
 }
 // two high halves -> one register, `lo` first
 __device__ __forceinline__ unsigned pack(unsigned lo, unsigned hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
+
+// two samples a register, 0 where they are infinite or NaN
+__device__ __forceinline__ unsigned finite_pair(unsigned v) {
+    if ((v & 0x7f80u) == 0x7f80u) v &= 0xffff0000u;
+    if ((v & 0x7f800000u) == 0x7f800000u) v &= 0xffffu;
+    return v;
+}
+template <class V>
+__device__ __forceinline__ V finite_pairs(V v) {
+#pragma unroll
+    for (unsigned k = 0; k < sizeof(V) / 4; k++) v[k] = finite_pair(v[k]);
+    return v;
+}
+
+// g's parts of two results
+template <bool EXACT>
+__device__ __forceinline__ void split_grads(float g0, float g1, unsigned &p0, unsigned &p1, unsigned &p2) {
+    unsigned lo[3], hi[3];
+    split3(g0, lo[0], lo[1], lo[2]);
+    split3(g1, hi[0], hi[1], hi[2]);
+    if constexpr (EXACT) {
+        if (__builtin_isinf(g0)) lo[1] = lo[2] = 0;
+        if (__builtin_isinf(g1)) hi[1] = hi[2] = 0;
+    }
+    p0 = pack(lo[0], hi[0]);
+    p1 = pack(lo[1], hi[1]);
+    p2 = pack(lo[2], hi[2]);
+}
+
+// whether a wave's sums are not all finite
+template <int N>
+__device__ __forceinline__ bool any_infinite(const float4_v (&acc)[N], float sum_g) {
+    float t = 0.0f * sum_g;
+#pragma unroll
+    for (int n = 0; n < N; n++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) t = __builtin_fmaf(acc[n][k], 0.0f, t);
+    return __any(t != t);
+}
 
 // a lane's 8 weights (as they are: times log 2's inverse, for an exponential with
 // a product less, the largest would be infinite)
@@ -784,17 +826,18 @@ __global__ __launch_bounds__(64 * kWideWaves) void lr_wide_bf16_kernel(LrArgs a)
     const WideOffsets o = wide_offsets<T>(a, u, i, q, col);
     float4_v acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
     float sum_g = 0.0f, sum_l = 0.0f;
-    auto dot = [&](const WideTile<T> &t) {
-        const bf16x8 x = __builtin_bit_cast(bf16x8, t.x.a);
+    auto dot = [&](const WideTile<T> &t, auto exact) {
+        const uint4_v rest = exact ? finite_pairs(t.x.a) : t.x.a;
         float4_v z = {bias, bias, bias, bias};
 #pragma unroll
         for (int e = 2; e >= 0; e--)
-            z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(bf16x8, w[e]), z, 0, 0, 0);
+            z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, e ? rest : t.x.a),
+                                                        __builtin_bit_cast(bf16x8, w[e]), z, 0, 0, 0);
         return z;
     };
     // the 32 rows of two tiles: k of the second product = (tile, row 4q + k)
-    auto products = [&](int r, WideTile<T> &one, WideTile<T> &two) {
-        const float4_v z1 = dot(one), z2 = dot(two);
+    auto products = [&](int r, WideTile<T> &one, WideTile<T> &two, auto exact) {
+        const float4_v z1 = dot(one, exact), z2 = dot(two, exact);
         float g[2][4];
         wide_grad<T, MODE>(a, u, o, one, z1, r, q, on, col, g[0], sum_g, sum_l);
         wide_grad<T, MODE>(a, u, o, two, z2, r + 16, q, on, col, g[1], sum_g, sum_l);
@@ -802,21 +845,24 @@ __global__ __launch_bounds__(64 * kWideWaves) void lr_wide_bf16_kernel(LrArgs a)
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             const int tile = k >> 1, e = 2 * (k & 1);
-            unsigned lo[3], hi[3];
-            split3(g[tile][e], lo[0], lo[1], lo[2]);
-            split3(g[tile][e + 1], hi[0], hi[1], hi[2]);
-#pragma unroll
-            for (int p = 0; p < 3; p++) gs[p][k] = pack(lo[p], hi[p]);
+            unsigned p0, p1, p2;
+            split_grads<exact>(g[tile][e], g[tile][e + 1], p0, p1, p2);
+            gs[0][k] = p0;
+            gs[1][k] = p1;
+            gs[2][k] = p2;
             const WideTile<T> &t = tile ? two : one;
             xs[0][k] = __builtin_amdgcn_perm(t.xc[e + 1], t.xc[e], 0x05040100u);  // the low halves
             xs[1][k] = pack(t.xc[e], t.xc[e + 1]);
         }
 #pragma unroll
-        for (int p = 2; p >= 0; p--)
+        for (int half = 0; half < 2; half++) {
+            const uint4_v rest = exact ? finite_pairs(xs[half]) : xs[half];
 #pragma unroll
-            for (int half = 0; half < 2; half++)
+            for (int p = 2; p >= 0; p--)
                 acc[half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, gs[p]),
-                                                                    __builtin_bit_cast(bf16x8, xs[half]), acc[half], 0, 0, 0);
+                                                                    __builtin_bit_cast(bf16x8, p ? rest : xs[half]),
+                                                                    acc[half], 0, 0, 0);
+        }
     };
     WideTile<T> t[4];
     auto load = [&](int r, int k, const WideMeta &m0, const WideMeta &m1) {
@@ -829,12 +875,20 @@ __global__ __launch_bounds__(64 * kWideWaves) void lr_wide_bf16_kernel(LrArgs a)
         load(r + 32, 2, m0, m1);
         m0 = wide_meta<MODE>(a, u, r + 64, i);
         m1 = wide_meta<MODE>(a, u, r + 80, i);
-        products(r, t[0], t[1]);
+        products(r, t[0], t[1], std::false_type{});
         if (r + 32 >= u.r1) break;
         load(r + 64, 0, m0, m1);
         m0 = wide_meta<MODE>(a, u, r + 96, i);
         m1 = wide_meta<MODE>(a, u, r + 112, i);
-        products(r + 32, t[2], t[3]);
+        products(r + 32, t[2], t[3], std::false_type{});
+    }
+    if (any_infinite(acc, sum_g)) {
+        acc[0] = acc[1] = float4_v{0, 0, 0, 0};
+        sum_g = sum_l = 0.0f;
+        for (int r = u.r0; r < u.r1; r += 32) {
+            load(r, 0, wide_meta<MODE>(a, u, r, i), wide_meta<MODE>(a, u, r + 16, i));
+            products(r, t[0], t[1], std::true_type{});
+        }
     }
     wide_store<MODE>(a, acc, sum_g, sum_l, i, q, (long long)u.m * a.H + u.h0 + 4 * q, a.H - u.h0 - 4 * q, on, col);
 }
@@ -915,15 +969,16 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void lr_pair_kernel(LrArgs a) {
         }
         if constexpr (MODE == kGrad) load_dy(a, u, o, r, q, col, t.dy);
     };
-    auto products = [&](int r, PairTile<T> &t) {
+    auto products = [&](int r, PairTile<T> &t, auto exact) {
         float4_v z[2];
 #pragma unroll
         for (int l = 0; l < 2; l++) {
             z[l] = float4_v{bias, bias, bias, bias};
             if constexpr (kBf16) {
+                const uint4_v rest = exact ? finite_pairs(t.x[l].a) : t.x[l].a;
 #pragma unroll
                 for (int e = 2; e >= 0; e--)
-                    z[l] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, t.x[l].a),
+                    z[l] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, e ? rest : t.x[l].a),
                                                                    __builtin_bit_cast(bf16x8, w[e]), z[l], 0, 0, 0);
             } else {
                 float f[8];
@@ -961,11 +1016,11 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void lr_pair_kernel(LrArgs a) {
             uint2_v gs[3];
 #pragma unroll
             for (int k = 0; k < 2; k++) {
-                unsigned lo[3], hi[3];
-                split3(g[2 * k], lo[0], lo[1], lo[2]);
-                split3(g[2 * k + 1], hi[0], hi[1], hi[2]);
-#pragma unroll
-                for (int p = 0; p < 3; p++) gs[p][k] = pack(lo[p], hi[p]);
+                unsigned p0, p1, p2;
+                split_grads<exact>(g[2 * k], g[2 * k + 1], p0, p1, p2);
+                gs[0][k] = p0;
+                gs[1][k] = p1;
+                gs[2][k] = p2;
             }
 #pragma unroll
             for (int l = 0; l < 2; l++) {
@@ -976,12 +1031,14 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void lr_pair_kernel(LrArgs a) {
                     xs[1][k] = pack(t.xc[l][2 * k], t.xc[l][2 * k + 1]);
                 }
 #pragma unroll
-                for (int p = 2; p >= 0; p--)
+                for (int half = 0; half < 2; half++) {
+                    const uint2_v rest = exact ? finite_pairs(xs[half]) : xs[half];
 #pragma unroll
-                    for (int half = 0; half < 2; half++)
-                        acc[l][half] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(short4_v, gs[p]),
-                                                                                 __builtin_bit_cast(short4_v, xs[half]),
-                                                                                 acc[l][half], 0, 0, 0);
+                    for (int p = 2; p >= 0; p--)
+                        acc[l][half] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(
+                            __builtin_bit_cast(short4_v, gs[p]), __builtin_bit_cast(short4_v, p ? rest : xs[half]),
+                            acc[l][half], 0, 0, 0);
+                }
             }
         } else {
 #pragma unroll
@@ -1000,11 +1057,22 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void lr_pair_kernel(LrArgs a) {
     for (int r = u.r0; r < u.r1; r += 32) {
         load(r + 16, ahead, two);
         ahead = wide_meta<MODE>(a, u, r + 32, i);
-        products(r, one);
+        products(r, one, std::false_type{});
         if (r + 16 >= u.r1) break;
         load(r + 32, ahead, one);
         ahead = wide_meta<MODE>(a, u, r + 48, i);
-        products(r + 16, two);
+        products(r + 16, two, std::false_type{});
+    }
+    if constexpr (kBf16) {
+        if (any_infinite(acc[0], sum_g) || any_infinite(acc[1], sum_g)) {
+            for (int k = 0; k < 4; k++) acc[k >> 1][k & 1] = float4_v{0, 0, 0, 0};
+            sum_g = sum_l = 0.0f;
+            for (int r = u.r0; r < u.r1; r += 16) {
+                PairTile<T> t;
+                load(r, wide_meta<MODE>(a, u, r, i), t);
+                products(r, t, std::true_type{});
+            }
+        }
     }
 #pragma unroll
     for (int half = 0; half < 2; half++) acc[0][half] = q >> 1 ? acc[1][half] : acc[0][half];
