@@ -317,8 +317,9 @@ int sc_sample_workspace(int b, int v, int s, size_t *bytes);
  *   index[i * index_ld + j] = the smallest place whose kept weights up to and
  *                             with it sum to more than u[i * u_ld + j] * all
  * or -1 for a row without a place to draw; kept[i] (kept may be NULL) = the
- * kept places.  Weights are 64-bit doubles, sums 64-bit integers of at least
- * 36 bits after the point (51 for short rows), so they have no order. */
+ * kept places.  Weights are 64-bit doubles, sums 64-bit integers, so they have
+ * no order; their unit is at most 2^-47 of the best place's weight in rows to
+ * 32768 scores, and at most 2^-51 of it or 2^-61 of the row's sum in longer ones. */
 int sc_sample(sc_trainer *t, const void *scores, int dtype, int b, int v, int64_t ld,
               const int32_t *lens, const sc_sample_params *prm, const double *u, int s,
               int64_t u_ld, int32_t *index, int64_t index_ld, int32_t *kept, void *ws,

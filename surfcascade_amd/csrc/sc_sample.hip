@@ -29,7 +29,7 @@
 // before.  Measured (one MI355X):
 //   960 scores, 960 draws                                 7 us, top_k and top_p 13
 //   32 rows x 20011, top_k 2000, top_p, min_p, 128 draws  30 us (split: 60)
-//   1000003 scores, top_k 500000, top_p, 16384 draws      63 us
+//   1000003 scores, top_k 500000, top_p, 16384 draws      65 us
 //   64 rows x 128256, one draw, no trim 50 us, top_p 121 us
 #include <hip/hip_runtime.h>
 
@@ -641,7 +641,7 @@ __global__ __launch_bounds__(kTrimThreads) void sample_trim_kernel(SampleArgs a)
 //
 // A row is cut into parts of 64 x 64 x f places, one workgroup each, and the
 // same steps run as one launch each; what a step finds is read by the next:
-//   extent  : each part's smallest and largest key and its count
+//   extent  : each part's smallest and largest key, its count and its weights' sum
 //   level 1 : bins over the row's key range: counts (top_k), masses (top_p)
 //   level 2, 3 of top_k, level 2, 3 of top_p : bins over the one bin the
 //             descent is in; every workgroup finds that bin itself from the
@@ -650,6 +650,12 @@ __global__ __launch_bounds__(kTrimThreads) void sample_trim_kernel(SampleArgs a)
 //             group of 64 f places
 //   draw    : one wave per draw: part, group and place by three searches
 // Bins are shared by atomics on integers, so their order does not matter.
+//
+// The unit of mass is chosen from the row's own sum of weights (to 4 digits, in 32
+// bits), not from what its length could bring: a long row of one heavy place and
+// many light ones would have units in which the light ones are 0, all of them
+// together 2^-12 of the best at 2^26 places.  (1000003 scores, top_k and top_p:
+// 63.3 us with the unit from the length, 64.7 with this.)
 
 constexpr int kPartThreads = 512;  // (256: 10 to 30 % slower to 200 parts; 1024: 50 % slower from 2000)
 constexpr int kDrawThreads = 256;
@@ -670,6 +676,7 @@ struct Descent {
 
 struct RowState {
     unsigned kmin, kmax, count;
+    int shift;     // a weight of 1 is 2^shift units of mass
     unsigned thr;  // set by the sums, as quota
     u64 quota;
     Descent k, p;
@@ -689,6 +696,7 @@ __device__ __forceinline__ void copy(RowState &to, const RowState &from) {
     to.kmin = from.kmin;
     to.kmax = from.kmax;
     to.count = from.count;
+    to.shift = from.shift;
     to.thr = from.thr;
     to.quota = from.quota;
     copy(to.k, from.k);
@@ -698,13 +706,25 @@ __device__ __forceinline__ void copy(RowState &to, const RowState &from) {
 struct Split {  // workspace of one row
     int parts, f;
     RowState *state;  // one per launch step
-    unsigned *extent;  // [parts][3]
+    unsigned *extent;  // [parts][4]: keys, count, sum of weights beside the part's largest (float)
     u64 *bins;         // [kBinArrays][kBins]
     u64 *group_mass;   // [parts][kGroups], places above the threshold
     unsigned *group_ties;
     u64 *part_mass;
     unsigned *part_kept, *part_ties;
 };
+
+// A weight beside another to 4 digits, or more than it is where the difference of
+// the scores or their `rate` (finite) passes 32 bits.
+__device__ __forceinline__ float weight_beside(float score, float best, float rate) {
+    return score == best ? 1.0f : __expf(fmaxf(score - best, -3.4028235e38f) * rate);
+}
+
+// the unit with which weights of this sum (1 or more; 0: none) stay below 2^62
+__device__ __forceinline__ int mass_shift(float sum) {
+    const int lg = ((int)(__float_as_uint(sum) >> 23) & 255) - 126;  // sum < 2^lg
+    return 62 - lg < 51 ? 62 - lg : 51;
+}
 
 enum Step { kExtent, kLevel1, kK2Step, kK3Step, kP2Step, kP3Step, kSums, kSteps };
 
@@ -715,7 +735,7 @@ __host__ __device__ inline int split_f(int V) {
 __host__ __device__ inline int split_parts(int V) { return (V + kGroups * 64 * split_f(V) - 1) / (kGroups * 64 * split_f(V)); }
 
 __host__ __device__ inline size_t split_row_bytes(int parts) {
-    size_t n = kSteps * sizeof(RowState) + (size_t)kBinArrays * kBins * 8 + (size_t)parts * (kGroups * 12 + 8 + 20);
+    size_t n = kSteps * sizeof(RowState) + (size_t)kBinArrays * kBins * 8 + (size_t)parts * (kGroups * 12 + 8 + 24);
     return (n + 255) & ~(size_t)255;
 }
 
@@ -855,6 +875,19 @@ __device__ __forceinline__ void fill_bins(SplitShared &s, PartKeys &keys, int f,
     }
 }
 
+// sum over a workgroup's threads, in each of them, always in the same order
+__device__ __forceinline__ float block_sum(float v, float *s_wave) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s_wave[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kPartThreads / 64; k++) v += s_wave[k];
+    return v;
+}
+
 template <int STEP>
 __global__ __launch_bounds__(kPartThreads) void sample_step_kernel(SampleArgs a) {
     __shared__ SplitShared s;
@@ -865,6 +898,7 @@ __global__ __launch_bounds__(kPartThreads) void sample_step_kernel(SampleArgs a)
     const int size = kGroups * 64 * w.f;
     const long long base = row * a.ld;
     const bool use_k = a.top_k > 0 || a.temperature == 0.0, use_p = a.top_p < 1.0;  // (the launches that run)
+    const float rate32 = (float)fmin(1.0 / a.temperature, 3.4028235e38);
     PartKeys keys{a, base, part * size, n, w.f, {}};
     keys.start(0);
 
@@ -874,16 +908,26 @@ __global__ __launch_bounds__(kPartThreads) void sample_step_kernel(SampleArgs a)
         if (use_k || use_p)
             for (int i = part * kPartThreads + tid; i < words; i += w.parts * kPartThreads) w.bins[i] = 0;
         unsigned lo = 0xffffffffu, hi = 0, c = 0;
+        float best = 0.0f, sum = 0.0f;  // of this thread's weights, beside the best so far
         for (int jj = 0; jj < w.f; jj++) {
             if (jj) keys.load(jj);
 #pragma unroll
             for (int j = 0; j < kPartKeys; j++) extend(keys.key[j], lo, hi, c);
+            if (!hi) continue;
+            if (sum > 0.0f) sum *= weight_beside(best, score_of(hi), rate32);
+            best = score_of(hi);
+#pragma unroll
+            for (int j = 0; j < kPartKeys; j++)
+                sum += keys.key[j] ? weight_beside(score_of(keys.key[j]), best, rate32) : 0.0f;
         }
         block_extent<kPartThreads>(lo, hi, c, reinterpret_cast<unsigned *>(s.bins));
+        if (sum > 0.0f) sum *= weight_beside(best, score_of(hi), rate32);
+        sum = block_sum(sum, reinterpret_cast<float *>(s.wave));
         if (tid == 0) {
-            w.extent[part * 3] = lo;
-            w.extent[part * 3 + 1] = hi;
-            w.extent[part * 3 + 2] = c;
+            w.extent[part * 4] = lo;
+            w.extent[part * 4 + 1] = hi;
+            w.extent[part * 4 + 2] = c;
+            w.extent[part * 4 + 3] = __float_as_uint(sum);
         }
         return;
     }
@@ -901,14 +945,27 @@ __global__ __launch_bounds__(kPartThreads) void sample_step_kernel(SampleArgs a)
     const int before_sums = use_p ? kP3Step : use_k ? kK3Step : kLevel1;
     if (STEP == kLevel1 || (STEP == kSums && before_sums == kLevel1)) {  // no trim: the sums are the second step
         unsigned lo = 0xffffffffu, hi = 0, c = 0;
-        for (int k = tid; k < w.parts; k += kPartThreads) {
-            const unsigned l = w.extent[k * 3], h = w.extent[k * 3 + 1];
+        constexpr int kShare = kMostParts / kPartThreads;
+        unsigned top[kShare];
+        float sums[kShare], sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kShare; i++) {
+            const int k = i * kPartThreads + tid;
+            const bool in = k < w.parts;
+            const unsigned l = in ? w.extent[k * 4] : 0xffffffffu;
+            top[i] = in ? w.extent[k * 4 + 1] : 0;
+            sums[i] = in ? __uint_as_float(w.extent[k * 4 + 3]) : 0.0f;
             lo = l < lo ? l : lo;
-            hi = h > hi ? h : hi;
-            c += w.extent[k * 3 + 2];
+            hi = top[i] > hi ? top[i] : hi;
+            c += in ? w.extent[k * 4 + 2] : 0;
         }
         block_extent<kPartThreads>(lo, hi, c, reinterpret_cast<unsigned *>(s.bins));
+#pragma unroll
+        for (int i = 0; i < kShare; i++)
+            if (top[i]) sum += sums[i] * weight_beside(score_of(top[i]), score_of(hi), rate32);
+        sum = block_sum(sum, reinterpret_cast<float *>(s.wave));
         __syncthreads();
+        st.shift = mass_shift(sum);
         st.thr = 0;
         st.quota = 0;
         st.k.done = st.p.done = 0;
@@ -929,7 +986,7 @@ __global__ __launch_bounds__(kPartThreads) void sample_step_kernel(SampleArgs a)
         constexpr int kBefore = STEP == kK2Step ? kLevel1 : STEP == kK3Step ? kK2Step : STEP == kP3Step ? kP2Step : -1;
         copy(st, w.state[STEP == kP2Step ? (use_k ? kK3Step : kLevel1) : STEP == kSums ? before_sums : kBefore]);
     }
-    const Weigh wg{score_of(st.kmax), 1.0 / a.temperature, ldexp(1.0, a.shift)};
+    const Weigh wg{score_of(st.kmax), 1.0 / a.temperature, ldexp(1.0, st.shift)};
     auto down = [&](Descent &d, const Bins &b, double share) {
         int at;
         u64 before, above;
@@ -1064,7 +1121,7 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a,
     const RowState &st = w.state[kSums];
     const unsigned thr = st.thr, count = st.count;
     const u64 quota = st.quota;
-    const Weigh wg{score_of(st.kmax), 1.0 / a.temperature, ldexp(1.0, a.shift)};
+    const Weigh wg{score_of(st.kmax), 1.0 / a.temperature, ldexp(1.0, st.shift)};
     const u64 each = thr ? wg.mass(wg.weight(thr)) : 0;
     const int n = row_length(a, row);
     // cumulated by part: mass above the threshold, and ties, of which the first

@@ -67,7 +67,7 @@ struct SampleArgs {
     const int *lens;  // NULL: V each; clamped to [0, V]
     double temperature, top_p, min_p;
     int top_k;
-    int shift;  // a weight of 1 is 2^shift units of mass (sample_shift)
+    int shift;  // a weight of 1 is 2^shift units of mass (sample_shift; rows of one workgroup)
     const double *u;
     int S;
     long long u_ld;
@@ -86,8 +86,10 @@ SamplePlan sample_plan(const SampleArgs &a);
 constexpr int kMaxPool = 1 << 26;
 
 // Masses are 64-bit integers, so that sums do not depend on their order: a
-// weight w in [0, 1] is rint(w * 2^shift), the largest shift with which V
-// weights of 1 stay below 2^62 (51 at most: a double's mantissa).
+// weight w in [0, 1] is rint(w * 2^shift), with sums below 2^62 and a shift of 51
+// at most (a double's mantissa).  Rows of one workgroup, 32768 scores at most, take
+// the largest that V weights of 1 leave room for; longer ones (many workgroups)
+// measure their own sum of weights first.
 inline int sample_shift(int V) {
     int lg = 0;
     while ((1 << lg) < V) lg++;
