@@ -35,7 +35,7 @@ class Trainer:
 
     Results carry no autograd history: `response_grad` and `loss` return the
     gradients, and operands that ask for one are refused (detach them, or call
-    under torch.no_grad())."""
+    under torch.no_grad()), as are operands with a forward-mode tangent."""
 
     def __init__(self, device: int = 0):
         import torch
@@ -46,6 +46,7 @@ class Trainer:
         self._dev = torch.device("cuda", self.device)
         self._f32, self._f64, self._i32 = torch.float32, torch.float64, torch.int32
         self._like = torch.empty_like
+        self._fwd = torch.autograd.forward_ad
         self._ws = None
         h = ctypes.c_void_p()
         _check(self._L.sc_trainer_create(self.device, ctypes.byref(h)))
@@ -113,10 +114,17 @@ class Trainer:
             raise ValueError("results carry no autograd history: detach the operands (response_grad and loss "
                              "return gradients)")
 
+    def _no_tangents(self, *operands):
+        """Of forward-mode differentiation (no_grad leaves it on)."""
+        if any(t is not None and self._fwd.unpack_dual(t).tangent is not None for t in operands):
+            raise ValueError("results carry no forward-mode tangents: detach the operands")
+
     def _operands(self, samples, w, b, patch, rows):
         f32, i32 = self._f32, self._i32
         if w.requires_grad or samples.requires_grad or (b is not None and b.requires_grad):
             self._no_grad(True)
+        if self._fwd._current_level >= 0:
+            self._no_tangents(samples, w, b)
         dtype = self._dtypes.get(samples.dtype)
         if dtype is None or samples.get_device() != self.device:
             raise ValueError("samples must be float32, float16 or bfloat16 on cuda:%d (got %s on %s)"
@@ -175,6 +183,8 @@ class Trainer:
         res, kind, res_ld = None, 0, 0
         if residual is not None:
             self._no_grad(residual.requires_grad)
+            if self._fwd._current_level >= 0:
+                self._no_tangents(residual)
             if residual.dim() == 1:
                 kind, res_ld = 1, residual.stride(0)
                 if residual.shape[0] != r or residual.dtype is not self._f32 \
@@ -202,6 +212,8 @@ class Trainer:
         self._follow()
         x, k, r, sets, cols = self._operands(samples, w, b, patch, rows)
         self._no_grad(grad_out.requires_grad)
+        if self._fwd._current_level >= 0:
+            self._no_tangents(grad_out)
         dy, dy_ld = self._rowwise(grad_out, self._f32, r, cols, "grad_out")
         kind = _RES[residual]
         dw, db, dres, dr = self._like(w), w.new_empty(sets) if b is None else self._like(b), None, None
@@ -225,6 +237,8 @@ class Trainer:
         self._follow()
         x, k, r, sets, cols = self._operands(samples, w, b, patch, rows)
         self._no_grad(target.requires_grad, weight is not None and weight.requires_grad)
+        if self._fwd._current_level >= 0:
+            self._no_tangents(target, weight)
         n = samples.shape[0]
         t = self._need(target, self._f32, (n,), "target")
         c = None if weight is None else self._need(weight, self._f32, (n,), "weight") or None
@@ -252,6 +266,8 @@ class Trainer:
         (sc_sample).  lens: int32 [b], the length of each row."""
         self._follow()
         self._no_grad(scores.requires_grad)
+        if self._fwd._current_level >= 0:
+            self._no_tangents(scores)
         dtype, dim = self._dtypes.get(scores.dtype), scores.dim()
         if dtype is None or scores.get_device() != self.device:
             raise ValueError("scores must be float32, float16 or bfloat16 on cuda:%d (got %s on %s)"
