@@ -177,7 +177,7 @@ class Trainer:
         """alpha * act(x . w + b) + beta * residual for every row and learner
         -> float32 [r, m] or [r, m, h] (sc_lr_response).  residual: None, one
         value per row [r], or one per result; out may be the latter, and
-        overlaps no other operand."""
+        overlaps no other operand (it counts as written in place)."""
         self._follow()
         x, k, r, sets, cols = self._operands(samples, w, b, patch, rows)
         res, kind, res_ld = None, 0, 0
@@ -198,7 +198,12 @@ class Trainer:
             out = w.new_empty((r,) + sets)
             y, y_ld = out.data_ptr(), cols
         else:
+            self._no_grad(out.requires_grad)
+            if self._fwd._current_level >= 0:
+                self._no_tangents(out)
             y, y_ld = self._rowwise(out, self._f32, r, cols, "out")
+            if not out.is_inference():  # (what autograd saved of it is no longer that)
+                self._torch.autograd.graph.increment_version(out)
         rc = self._L.sc_lr_response(self._h, x, k, _ACT[activation], alpha, res, kind, res_ld, beta, y, y_ld)
         if rc:
             _check(rc)

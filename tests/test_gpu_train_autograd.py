@@ -47,3 +47,37 @@ def test_forward_tangents_are_refused(tr):
             got = call(fwd.unpack_dual(dual).primal)
         for a, e in zip(got if isinstance(got, tuple) else (got,), want if isinstance(want, tuple) else (want,)):
             assert (a is None and e is None) or torch.equal(a, e)
+
+
+def test_out_is_an_in_place_write(tr):
+    """A buffer that asks for gradients is refused, and what autograd had saved of
+    another is known to be gone."""
+    x, w, b = _operands()
+    want = tr.response(x, w, b)
+    leaf = torch.zeros(9, 3, 2, device="cuda", requires_grad=True)
+    for out in (leaf, leaf * 2):
+        with pytest.raises(ValueError, match="autograd"):
+            tr.response(x, w, b, out=out)
+        assert not out.any()
+    with torch.no_grad():
+        assert torch.equal(tr.response(x, w, b, out=leaf), want)
+    saved = torch.ones(9, 3, 2, device="cuda")
+    a = torch.ones(9, 3, 2, device="cuda", requires_grad=True)
+    product = (a * saved).sum()
+    tr.response(x, w, b, out=saved)
+    with pytest.raises(RuntimeError, match="inplace"):
+        product.backward()
+    assert a.grad is None
+    with fwd.dual_level():
+        dual = fwd.make_dual(torch.zeros(9, 3, 2, device="cuda"), torch.ones(9, 3, 2, device="cuda"))
+        with pytest.raises(ValueError, match="tangent"):
+            tr.response(x, w, b, out=dual)
+    with torch.inference_mode():
+        out = torch.empty(9, 3, 2, device="cuda")
+        assert torch.equal(tr.response(x, w, b, out=out), want)
+    # a view's write is its base's
+    base = torch.ones(9, 8, device="cuda")
+    product = (torch.ones(9, 8, device="cuda", requires_grad=True) * base).sum()
+    tr.response(x, w, b, out=base[:, 1:7])
+    with pytest.raises(RuntimeError, match="inplace"):
+        product.backward()
