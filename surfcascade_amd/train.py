@@ -291,7 +291,7 @@ class Trainer:
         index = u.new_empty(shape, dtype=self._i32)
         kept = index.new_empty(b)
         most = 2**31 - 1  # (a C int; the library refuses rows that long, and such a top_k keeps all)
-        prm = _SampleParams(temperature, min(top_k, most), top_p, min_p)
+        prm = _SampleParams(temperature, max(-1, min(top_k, most)), top_p, min_p)
         if v > most or s > most or b > most:
             raise ValueError("more than 2^31 - 1 rows, scores or draws")
 
