@@ -5,7 +5,7 @@ GentleAdaboost::Train does with the descriptors a Miner leaves on the GPU
     miner.mine_batch_device(frames, capacity, samples)    # [n, n_patches, 32]
     tr = Trainer()
     rows, _ = tr.sample(log_weight, u)                    # the roulette wheel
-    loss, dw, db = tr.loss(samples, w, target, b, rows=rows[0])
+    loss, dw, db = tr.loss(samples, w, target, b, rows=rows)
     score = tr.response(samples, w, b, residual=score, alpha=1 / k, beta=1 - 1 / k)
 """
 from __future__ import annotations
@@ -14,8 +14,23 @@ import ctypes
 
 from . import _check, _SampleParams, _Samples, _WeakBank, load_library
 
-_ACT = {"none": 0, "sigmoid": 1}
-_RES = {None: 0, "none": 0, "row": 1, "full": 2}
+class UnknownName(KeyError, ValueError):
+    """An activation or kind of residual that does not exist: refused as a wrong
+    value, and as the missing key it is."""
+
+    def __str__(self):
+        return ValueError.__str__(self)
+
+
+class _Names(dict):
+    def __missing__(self, name):
+        raise UnknownName("%s must be one of %s (got %r)" % (self.what, ", ".join(map(repr, self)), name))
+
+
+_ACT = _Names(none=0, sigmoid=1)
+_ACT.what = "activation"
+_RES = _Names({None: 0, "none": 0, "row": 1, "full": 2})
+_RES.what = "residual"
 
 
 class Trainer:
@@ -179,6 +194,7 @@ class Trainer:
         value per row [r], or one per result; out may be the latter, and
         overlaps no other operand (it counts as written in place)."""
         self._follow()
+        act = _ACT[activation]
         x, k, r, sets, cols = self._operands(samples, w, b, patch, rows)
         res, kind, res_ld = None, 0, 0
         if residual is not None:
@@ -204,7 +220,7 @@ class Trainer:
             y, y_ld = self._rowwise(out, self._f32, r, cols, "out")
             if not out.is_inference():  # (what autograd saved of it is no longer that)
                 self._torch.autograd.graph.increment_version(out)
-        rc = self._L.sc_lr_response(self._h, x, k, _ACT[activation], alpha, res, kind, res_ld, beta, y, y_ld)
+        rc = self._L.sc_lr_response(self._h, x, k, act, alpha, res, kind, res_ld, beta, y, y_ld)
         if rc:
             _check(rc)
         return out
@@ -215,19 +231,19 @@ class Trainer:
         (dw like w, db [m] or [m, h], dres or None) (sc_lr_response_grad).
         residual: None or "none", "row" or "full", the residual's kind."""
         self._follow()
+        act, kind = _ACT[activation], _RES[residual]
         x, k, r, sets, cols = self._operands(samples, w, b, patch, rows)
         self._no_grad(grad_out.requires_grad)
         if self._fwd._current_level >= 0:
             self._no_tangents(grad_out)
         dy, dy_ld = self._rowwise(grad_out, self._f32, r, cols, "grad_out")
-        kind = _RES[residual]
         dw, db, dres, dr = self._like(w), w.new_empty(sets) if b is None else self._like(b), None, None
         if kind:
             dres = w.new_empty((r,) if kind == 1 else (r,) + sets)
             dr = dres.data_ptr()
 
         def call(ws, ws_bytes):
-            return self._L.sc_lr_response_grad(self._h, x, k, _ACT[activation], alpha, dy, dy_ld, dw.data_ptr(),
+            return self._L.sc_lr_response_grad(self._h, x, k, act, alpha, dy, dy_ld, dw.data_ptr(),
                                                db.data_ptr(), kind, beta, dr, 1 if kind == 1 else cols, ws, ws_bytes)
 
         if self._workspace(call(None, 0), lambda: self._lr_bytes(x, k)):
