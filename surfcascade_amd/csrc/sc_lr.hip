@@ -737,9 +737,11 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 // v = a + b + c, each a bfloat16 (8 + 8 + 8 bits of 24): the high halves (an
 // infinite v: a, and NaN for what is left of it).  The products of an infinite
-// sample with the parts are NaN where a part is 0; a chunk whose sums come out
-// not finite is therefore summed again, `exact`: only v's first part meets such
-// samples, the others 0 in their place.
+// sample with the parts are NaN where a part is 0, and of a small g the bits
+// below a bfloat16's least, 2^-133, are in no part.  A chunk whose sums come out
+// not finite or that small is therefore summed again, `exact`: only the first
+// part meets infinite samples, the others 0 in their place, and small sums' g are
+// split 2^16 times as large (the other sets' sums get the bits they had).
 __device__ __forceinline__ void split3(float v, unsigned &a, unsigned &b, unsigned &c) {
     a = __float_as_uint(v) & 0xffff0000u;
     const float r = v - __uint_as_float(a);
@@ -764,8 +766,14 @@ __device__ __forceinline__ V finite_pairs(V v) {
 
 // g's parts of two results
 template <bool EXACT>
-__device__ __forceinline__ void split_grads(float g0, float g1, unsigned &p0, unsigned &p1, unsigned &p2) {
+__device__ __forceinline__ void split_grads(float g0, float g1, float scale, float &most, unsigned &p0, unsigned &p1,
+                                            unsigned &p2) {
     unsigned lo[3], hi[3];
+    if constexpr (EXACT) {
+        most = fmaxf(most, fmaxf(fabsf(g0), fabsf(g1)));
+        g0 *= scale;
+        g1 *= scale;
+    }
     split3(g0, lo[0], lo[1], lo[2]);
     split3(g1, hi[0], hi[1], hi[2]);
     if constexpr (EXACT) {
@@ -777,15 +785,38 @@ __device__ __forceinline__ void split_grads(float g0, float g1, unsigned &p0, un
     p2 = pack(lo[2], hi[2]);
 }
 
-// whether a wave's sums are not all finite
+// Whether a wave has to sum again; `scale` of its lane's set then.  (Of 2^11 rows
+// the bits below 2^-133 are one in 2^24 of sums below 2^-98.)
 template <int N>
-__device__ __forceinline__ bool any_infinite(const float4_v (&acc)[N], float sum_g) {
+__device__ __forceinline__ bool again(const float4_v (&acc)[N], float sum_g, float &scale) {
     float t = 0.0f * sum_g;
 #pragma unroll
     for (int n = 0; n < N; n++)
 #pragma unroll
         for (int k = 0; k < 4; k++) t = __builtin_fmaf(acc[n][k], 0.0f, t);
-    return __any(t != t);
+    sum_g += __shfl_xor(sum_g, 16, 64);
+    sum_g += __shfl_xor(sum_g, 32, 64);
+    scale = sum_g != 0.0f && fabsf(sum_g) < 3.1554436e-30f ? 65536.0f : 1.0f;
+    return __any(t != t || scale != 1.0f);
+}
+// Large g that cancel leave a small sum as well, but do not bear the scale (`most`
+// of them; their sums' bits are far above): whether a set has to go without
+__device__ __forceinline__ bool without(float most, float &scale) {
+    most = fmaxf(most, __shfl_xor(most, 16, 64));
+    most = fmaxf(most, __shfl_xor(most, 32, 64));
+    const bool large = scale != 1.0f && most > 1.0f;
+    if (large) scale = 1.0f;
+    return __any(large);
+}
+// the sums of the sets 4q .. as they are
+template <int N>
+__device__ __forceinline__ void unscale(float4_v (&acc)[N], float scale, int q) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const float by = 1.0f / __shfl(scale, q * 4 + k, 64);  // (a power of two)
+#pragma unroll
+        for (int n = 0; n < N; n++) acc[n][k] *= by;
+    }
 }
 
 // a lane's 8 weights (as they are: times log 2's inverse, for an exponential with
@@ -825,7 +856,7 @@ __global__ __launch_bounds__(64 * kWideWaves) void lr_wide_bf16_kernel(LrArgs a)
     const float bias = on && a.b ? a.b[col] : 0.0f;
     const WideOffsets o = wide_offsets<T>(a, u, i, q, col);
     float4_v acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-    float sum_g = 0.0f, sum_l = 0.0f;
+    float sum_g = 0.0f, sum_l = 0.0f, scale, most;
     auto dot = [&](const WideTile<T> &t, auto exact) {
         const uint4_v rest = exact ? finite_pairs(t.x.a) : t.x.a;
         float4_v z = {bias, bias, bias, bias};
@@ -846,7 +877,7 @@ __global__ __launch_bounds__(64 * kWideWaves) void lr_wide_bf16_kernel(LrArgs a)
         for (int k = 0; k < 4; k++) {
             const int tile = k >> 1, e = 2 * (k & 1);
             unsigned p0, p1, p2;
-            split_grads<exact>(g[tile][e], g[tile][e + 1], p0, p1, p2);
+            split_grads<exact>(g[tile][e], g[tile][e + 1], scale, most, p0, p1, p2);
             gs[0][k] = p0;
             gs[1][k] = p1;
             gs[2][k] = p2;
@@ -882,13 +913,14 @@ __global__ __launch_bounds__(64 * kWideWaves) void lr_wide_bf16_kernel(LrArgs a)
         m1 = wide_meta<MODE>(a, u, r + 112, i);
         products(r + 32, t[2], t[3], std::false_type{});
     }
-    if (any_infinite(acc, sum_g)) {
+    for (bool more = again(acc, sum_g, scale); more; more = without(most, scale)) {
         acc[0] = acc[1] = float4_v{0, 0, 0, 0};
-        sum_g = sum_l = 0.0f;
+        sum_g = sum_l = most = 0.0f;
         for (int r = u.r0; r < u.r1; r += 32) {
             load(r, 0, wide_meta<MODE>(a, u, r, i), wide_meta<MODE>(a, u, r + 16, i));
             products(r, t[0], t[1], std::true_type{});
         }
+        unscale(acc, scale, q);
     }
     wide_store<MODE>(a, acc, sum_g, sum_l, i, q, (long long)u.m * a.H + u.h0 + 4 * q, a.H - u.h0 - 4 * q, on, col);
 }
@@ -944,7 +976,7 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void lr_pair_kernel(LrArgs a) {
     if constexpr (kBf16) split_weights(wf, w);
     const WideOffsets o = wide_offsets<T>(a, u, i, q, col);
     float4_v acc[2][2] = {};
-    float sum_g = 0.0f, sum_l = 0.0f;
+    float sum_g = 0.0f, sum_l = 0.0f, scale, most;
     auto load = [&](int r, const WideMeta &v, PairTile<T> &t) {
         t.v = v;
         t.whole = u.present && __ballot(v.idx < 0) == 0;
@@ -1017,7 +1049,7 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void lr_pair_kernel(LrArgs a) {
 #pragma unroll
             for (int k = 0; k < 2; k++) {
                 unsigned p0, p1, p2;
-                split_grads<exact>(g[2 * k], g[2 * k + 1], p0, p1, p2);
+                split_grads<exact>(g[2 * k], g[2 * k + 1], scale, most, p0, p1, p2);
                 gs[0][k] = p0;
                 gs[1][k] = p1;
                 gs[2][k] = p2;
@@ -1064,14 +1096,16 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void lr_pair_kernel(LrArgs a) {
         products(r + 16, two, std::false_type{});
     }
     if constexpr (kBf16) {
-        if (any_infinite(acc[0], sum_g) || any_infinite(acc[1], sum_g)) {
+        for (bool more = again(acc[0], sum_g, scale) | again(acc[1], sum_g, scale); more; more = without(most, scale)) {
             for (int k = 0; k < 4; k++) acc[k >> 1][k & 1] = float4_v{0, 0, 0, 0};
-            sum_g = sum_l = 0.0f;
+            sum_g = sum_l = most = 0.0f;
             for (int r = u.r0; r < u.r1; r += 16) {
                 PairTile<T> t;
                 load(r, wide_meta<MODE>(a, u, r, i), t);
                 products(r, t, std::true_type{});
             }
+            unscale(acc[0], scale, q);
+            unscale(acc[1], scale, q);
         }
     }
 #pragma unroll
