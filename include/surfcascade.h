@@ -271,8 +271,8 @@ int sc_lr_response(sc_trainer *t, const sc_samples *x, const sc_weak_bank *k, in
                    const float *res, int res_kind, int64_t res_ld, float beta, float *y,
                    int64_t y_ld);
 
-/* Workspace of sc_lr_response_grad and sc_lr_loss for these sizes (pointers
- * other than rows are not looked at). */
+/* Workspace of sc_lr_response_grad and sc_lr_loss for these sizes (of the
+ * pointers, only whether rows and patch are NULL counts). */
 int sc_lr_workspace(const sc_samples *x, const sc_weak_bank *k, size_t *bytes);
 
 /* The backward pass of sc_lr_response for dy[r * dy_ld + j*h + k]:
@@ -281,7 +281,8 @@ int sc_lr_workspace(const sc_samples *x, const sc_weak_bank *k, size_t *bytes);
  *   dres = beta * dy, summed over a row's results for SC_RES_ROW
  * (dres NULL with SC_RES_NONE; no result overlaps another operand).  Sums over
  * rows in 32 bits over a chunk of rows (at most 2048 to a running sum, and at
- * most four of these), in 64 bits over the chunks; dres sums in 64 bits.  A g that is
+ * most four of these; of 5 and more sets of bfloat16 samples, a row's g beside
+ * large ones counts to 2^-133), in 64 bits over the chunks; dres sums in 64 bits.  A g that is
  * infinite or NaN leaves its learner's and set's dw and db so.  There is no
  * gradient of the descriptors: they are read off images. */
 int sc_lr_response_grad(sc_trainer *t, const sc_samples *x, const sc_weak_bank *k, int act,

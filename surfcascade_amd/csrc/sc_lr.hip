@@ -10,9 +10,9 @@
 // A (row, patch) descriptor is 128 B (64 B in 16 bits) that feeds 64 flops per
 // parameter set (128 with its gradient), so up to 16 sets the matrix' own bytes
 // are the bound: each descriptor is read once from memory and everything is done
-// on it in registers.  Sums over rows are in 32 bits within a chunk of them (a
-// wave's: 2048 at most); the chunks are joined in 64 bits in a fixed order (no atomics: the same call gives
-// the same bits).
+// on it in registers.  Sums over rows are in 32 bits within a chunk of them (2048
+// of a wave at most); the chunks are joined in 64 bits in a fixed order (no
+// atomics: the same call gives the same bits).
 //
 // Up to kNarrowSets sets, the narrow form: one descriptor on LPI = 8 lanes (4 in
 // 16 bits), 16 B each, so a wave's load is 8 (16) neighbouring descriptors of one
@@ -24,13 +24,14 @@
 // up to 16.  The borders, on 8191 x 608: responses of f32 with 5 sets 153 us
 // narrow and 205 wide (with 7 275: its stores are not whole 16-B pieces), with 8
 // sets 191 and 182; the gradient with 4 sets 150 us narrow, with 5 241 and 206
-// wide; the loss with 5 sets 184 and 208 in f32, 155 and 105 in bf16.
+// wide; the loss with 5 sets 184 and 208 in f32, 155 and 105 in bf16.  (One border
+// serves gradients and losses of every type: it costs the f32 loss of 5 sets 24 us.)
 //
 // Measured (one MI355X; a 2 GiB copy moves 4.9 TB/s there, reads and writes):
 //   responses, 16384 x 608, f32, 1 set          221 us, 5.9 TB/s
 //   loss and gradient, 16384 x 608, f32, 1 set  219 us, 5.8 TB/s
 //   responses, 2001 x 608, f16, 16 sets          60 us, 3.5 TB/s
-//   loss and gradient, 8191 x 608, bf16, 16 sets 130 us, 2.5 TB/s (the VALU, 68 %
+//   loss and gradient, 8191 x 608, bf16, 16 sets 131 us, 2.5 TB/s (the VALU, 68 %
 //     of the cycles: the sigmoid, its loss and the operand splits of 80 M results)
 //   gradient, 480 x 11870, bf16, 8 sets, dres   171 us, 4.4 TB/s
 #include <hip/hip_runtime.h>
@@ -838,7 +839,8 @@ __device__ __forceinline__ void split_weights(const float (&wf)[8], uint4_v (&w)
 // Gradient and loss of bfloat16 samples on the bfloat16 matrix cores (16x16x32,
 // a fifth of the f32 ones' time for these products): the samples are exact
 // there, and the weights and g go in as sums of three bfloat16 each, their 24
-// bits whole, so every product is exact and the sums are f32 as before.
+// bits whole (but for what lies below 2^-133 of a g beside large ones), so every
+// product is exact and the sums are f32 as before.
 template <int MODE>
 __global__ __launch_bounds__(64 * kWideWaves) void lr_wide_bf16_kernel(LrArgs a) {
     using T = BF16;
@@ -929,9 +931,9 @@ __global__ __launch_bounds__(64 * kWideWaves) void lr_wide_bf16_kernel(LrArgs a)
 // results being those of set i % 8 of learner i / 8: every learner has its own
 // products, half of which is left (a descriptor's NaN stays its learner's), but
 // dy, dres and the arithmetic of g fill the wave.  8191 x 608 x 8, alone and in
-// pairs: loss 127 and 108 us in bf16, 189 and 159 in f16, gradient 143 and 103,
+// pairs: loss 127 and 106 us in bf16, 189 and 159 in f16, gradient 143 and 103,
 // 168 and 146; f32 206 and 253, 197 and 196 (it has no registers for two).  480 x
-// 11870 x 8 with dres: 198 and 171.
+// 11870 x 8 with dres: 205 and 171.
 template <class T>
 struct PairTile {
     WideMeta v;
@@ -1118,9 +1120,9 @@ __global__ __launch_bounds__(64 * kWideWaves, 4) void lr_pair_kernel(LrArgs a) {
 // What follows the row chunks, in one launch.  The first `joins` workgroups join
 // their partial sums: WORDS neighbouring ones each, every one of SUBS rows of
 // threads walks every SUBS-th chunk, in 64 bits; where the rows take several
-// launches, acc carries the sums from one's join to the next's.  The others write the gradient
-// of a residual of one value per row, beta * the sum of the row's dy: `lanes` of
-// a wave a row, in 64 bits.  (Loss of 8191 x 608 x 16: 13 chunks, 17 MB of
+// launches, acc carries the sums from one's join to the next's.  The others, in
+// the last launch, write the gradient of a residual of one value per row, beta *
+// the sum of the row's dy: `lanes` of a wave a row, in 64 bits.  (Loss of 8191 x 608 x 16: 13 chunks, 17 MB of
 // partial sums, 7.2 us; with 8 rows of 32 threads 8.5.)
 template <int SUBS, int WORDS>
 __global__ __launch_bounds__(WORDS * SUBS) void lr_tail_kernel(LrArgs a, int loss, int joins, int lanes, int last) {

@@ -1206,6 +1206,8 @@ constexpr int kRowScores = 8192, kTrimScores = 32768, kSplitRows = 512, kGridRow
 // (one row of 20011, top_k 2001 alone: 128 draws 25 us trimmed and 32 split, 4096
 // draws 31 and 34, with top_k 6670 43 and 34, with top_p too 35 and 50; 16 rows of
 // 32768, 4096 draws, top_k 3276: 42 and 64)
+// (Rows of one workgroup make all their draws there, however many: 2^20 of them take
+// 1.4 ms from 960 scores and 4.3 ms from 8192, where 8193 scores, split, take 0.4.)
 static bool trim(const SampleArgs &a) {
     const bool few = a.temperature == 0.0 || (a.top_k > 0 && a.top_k <= kTrimKept);
     const bool light = a.V <= kTrimScores / 2 || a.S <= 1024 || a.B >= 8 || a.top_p < 1.0 || a.temperature == 0.0;

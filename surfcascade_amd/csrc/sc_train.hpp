@@ -77,7 +77,8 @@ struct SampleArgs {
     void *ws;   // sample_plan's bytes (NULL: none)
 };
 
-// the launch shape of the draws, from B, V and S alone
+// the launch shape of the draws, from their sizes and trims; the most that any
+// trims need without one (temperature above 0, top_k 0)
 struct SamplePlan {
     size_t ws_bytes;
 };
