@@ -282,9 +282,10 @@ int sc_lr_workspace(const sc_samples *x, const sc_weak_bank *k, size_t *bytes);
  * (dres NULL with SC_RES_NONE; no result overlaps another operand).  Sums over
  * rows in 32 bits over a chunk of rows (at most 2048 to a running sum, and at
  * most four of these; of 5 and more sets of bfloat16 samples, a row's g beside
- * large ones counts to 2^-133), in 64 bits over the chunks; dres sums in 64 bits.  A g that is
- * infinite or NaN leaves its learner's and set's dw and db so.  There is no
- * gradient of the descriptors: they are read off images. */
+ * large ones, or in a sum of 0, counts to 2^-133) and in 64 bits over the
+ * chunks, dres sums in 64 bits.  A g that is infinite or NaN leaves its learner's
+ * and set's dw and db so.  There is no gradient of the descriptors: they are read
+ * off images. */
 int sc_lr_response_grad(sc_trainer *t, const sc_samples *x, const sc_weak_bank *k, int act,
                         float alpha, const float *dy, int64_t dy_ld, float *dw, float *db,
                         int res_kind, float beta, float *dres, int64_t dres_ld, void *ws,

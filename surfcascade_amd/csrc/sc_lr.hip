@@ -839,8 +839,8 @@ __device__ __forceinline__ void split_weights(const float (&wf)[8], uint4_v (&w)
 // Gradient and loss of bfloat16 samples on the bfloat16 matrix cores (16x16x32,
 // a fifth of the f32 ones' time for these products): the samples are exact
 // there, and the weights and g go in as sums of three bfloat16 each, their 24
-// bits whole (but for what lies below 2^-133 of a g beside large ones), so every
-// product is exact and the sums are f32 as before.
+// bits whole (but for what lies below 2^-133 of a g beside large ones or in a sum
+// of 0), so every product is exact and the sums are f32 as before.
 template <int MODE>
 __global__ __launch_bounds__(64 * kWideWaves) void lr_wide_bf16_kernel(LrArgs a) {
     using T = BF16;
